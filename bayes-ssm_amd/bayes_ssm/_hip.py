@@ -34,6 +34,7 @@ _BWD_FULL = _BWD_HEAD + [_P] * 8 + [_L, _L, _L, _F, _P]
 _BWD_SIX = _BWD_HEAD + [_P] * 6 + [_L, _L, _L, _F, _P]
 _BWD_LEAN = _BWD_HEAD + [_P] * 3 + [_L, _L, _L, _F, _P]
 _BWD_SAVED_HEAD = [_I, _I] + [_P] * 10 + [_P] * 5 + [_P] * 3
+_SELECT_HEAD = [_I, _P, _L, _L, _L, _I, _P, _L, _L, _P] + [_P, _L, _L, _L] * 2 + [_P, _P, _I, _P]
 _SIGNATURES = {
     "bssm_forward_chunked": _FWD,
     "bssm_forward_chunked_fixed": _FWD,
@@ -75,11 +76,23 @@ _SIGNATURES = {
     "bssm_mixer_block_forward": [_P, _L, _P, _P, _P, _F] + [_P] * 9 + [_L, _L, _L, _L, _F, _P],
     "bssm_mixer_block_backward": [_P, _L, _P, _P, _P, _P, _F] + [_P] * 10 + [_L] + [_P] * 6 + [_I]
                                  + [_P] * 2 + [_L, _L, _L, _L, _F, _P],
+    "bssm_short_conv_forward": [_I] * 4 + [_P, _L, _L] + [_P] * 6 + [_L] * 3 + [_P],
+    "bssm_short_conv_backward": [_I] * 4 + [_P, _L, _L] + [_P] * 11 + [_L] * 3 + [_P],
+    "bssm_short_conv_partial_rows": [_I, _L, _L, _L],
+    "bssm_layer_norm_forward": [_I, _I, _P, _L, _P, _P, _F] + [_P] * 3 + [_L, _L, _P],
+    "bssm_layer_norm_backward": [_I, _I, _P, _L] + [_P] * 8 + [_L, _L, _P],
+    "bssm_layer_norm_partial_rows": [_I, _L, _L],
+    "bssm_distill_forward": [_I, _I, _P, _L, _P, _P, _F] + [_P] * 3 + [_L] * 3 + [_P],
+    "bssm_distill_backward": [_I, _I, _P, _L, _P, _P, _F] + [_P] * 3 + [_I, _P] + [_L] * 3 + [_P],
+    "bssm_select_forward": _SELECT_HEAD + [_P] * 5 + [_L] * 6 + [_P],
+    "bssm_select_backward": _SELECT_HEAD + [_P] * 15 + [_L] * 6 + [_P],
+    "bssm_select_sizes": [_I, _I] + [_L] * 6,
+    "bssm_select_step": [_I] * 4 + [_P, _L, _I, _P, _L] + [_P] * 7 + [_I] + [_P] * 3 + [_L] * 5 + [_P],
     "bssm_supported": [_I, _I],
     "bssm_preferred_checkpoint": [_I],
     "bssm_abi_version": [],
 }
-ABI_VERSION = 10
+ABI_VERSION = 11
 ANY_SHAPE = 1 << 32  # or-ed into the mixer entry points' chunk (BSSM_ANY_SHAPE)
 ROW_KERNELS = 1 << 33  # the same (BSSM_ROW_KERNELS)
 
@@ -114,6 +127,8 @@ def load() -> ctypes.CDLL:
                 fn.restype = ctypes.c_int
             lib.bssm_value_stats_workspace.restype = ctypes.c_int64
             lib.bssm_small_batch_limit.restype = ctypes.c_int64
+            for name in ("bssm_short_conv_partial_rows", "bssm_layer_norm_partial_rows", "bssm_select_sizes"):
+                getattr(lib, name).restype = ctypes.c_int64
             lib.bssm_last_error.argtypes = []
             lib.bssm_last_error.restype = ctypes.c_char_p
             version = lib.bssm_abi_version()

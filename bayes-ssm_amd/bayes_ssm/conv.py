@@ -17,6 +17,12 @@ transposed view, so the mixer's ``.transpose(1, 2)`` gives back a contiguous
 Inputs the kernels do not take (other devices or dtypes, a contiguous
 ``[B, C, T]`` layout, rows not 16-byte multiples) run the reference's
 elementwise formula in torch.
+
+``causal_conv`` is the filter of a selective state space block
+(``bayes_ssm.selective``): 2 to 4 taps over ``[batch, time, channels]`` rows,
+with bias, SiLU, inputs carried from an earlier call and rows of unequal
+length, on ``bssm_short_conv_forward/backward`` (any number of channels,
+strided rows).
 """
 from __future__ import annotations
 
@@ -114,4 +120,138 @@ class CausalDepthwise4(nn.Module):
         return causal_depthwise4(x, self.weight)
 
 
-__all__ = ["CausalDepthwise4", "causal_depthwise4"]
+def _check_lengths(lengths: Optional[Tensor], batch: int, device: torch.device) -> Optional[Tensor]:
+    """``lengths`` as the kernels read them (int64, contiguous), checked without reading their values."""
+    if lengths is None:
+        return None
+    if not isinstance(lengths, Tensor) or lengths.is_floating_point() or lengths.dtype == torch.bool:
+        raise TypeError("lengths must be an integer tensor")
+    if tuple(lengths.shape) != (batch,):
+        raise ValueError(f"lengths must have shape [{batch}], got {tuple(lengths.shape)}")
+    if lengths.device != device:
+        raise ValueError("lengths must be on the inputs' device")
+    return lengths.long().contiguous()
+
+
+def _short_conv_formula(x: Tensor, weight: Tensor, bias: Optional[Tensor], silu: bool, state: Optional[Tensor],
+                        lengths: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    """``causal_conv`` in torch operations, in float32 (float64 for float64 inputs), rounded once."""
+    b, t, c = x.shape
+    w = weight.shape[1]
+    wide = torch.promote_types(x.dtype, torch.float32)
+    carried = x.new_zeros(b, w - 1, c) if state is None else state
+    row = torch.cat((carried, x), 1)
+    wide_row, taps = row.to(wide), weight.to(wide)
+    y = sum(wide_row[:, j:j + t] * taps[:, j] for j in range(w))
+    if bias is not None:
+        y = y + bias.to(wide)
+    if silu:
+        y = F.silu(y)
+    if lengths is None:
+        return y.to(x.dtype), row[:, t:].clone()
+    cut = lengths.clamp(0, t)
+    y = y.masked_fill((torch.arange(t, device=x.device) >= cut[:, None])[..., None], 0.0)
+    last = cut[:, None] + torch.arange(w - 1, device=x.device)
+    return y.to(x.dtype), row.gather(1, last[..., None].expand(b, w - 1, c))
+
+
+def _rows(x: Tensor) -> tuple[Tensor, int, int]:
+    """``x`` [B, T, C] as the kernels read it: channels contiguous; its batch and row stride (elements)."""
+    b, t, c = x.shape
+    if c > 1 and x.stride(2) != 1 or t > 1 and x.stride(1) < c:
+        x = x.contiguous()
+    return x, (x.stride(0) if b > 1 else 0), (x.stride(1) if t > 1 else 0)
+
+
+class _ShortConvFunction(torch.autograd.Function):
+    """Autograd boundary of the short filter (C ABI ``bssm_short_conv_*``)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, lengths, silu):
+        b, t, c = x.shape
+        w = weight.shape[1]
+        x, batch_stride, row_stride = _rows(x)
+        weight, bias, state = (None if z is None else z.contiguous() for z in (weight, bias, state))
+        y = torch.empty(b, t, c, device=x.device, dtype=x.dtype)
+        final = torch.empty(b, w - 1, c, device=x.device, dtype=x.dtype)
+        P = _hip.ptr
+        _hip.launch(x.device, "bssm_short_conv_forward", int(x.dtype == torch.bfloat16),
+                    int(weight.dtype == torch.bfloat16), w, int(silu), P(x), batch_stride, row_stride, P(weight),
+                    P(bias), P(state), P(lengths), P(y), P(final), b, t, c, _hip.stream_of(x.device))
+        ctx.save_for_backward(x, weight, bias, state, lengths)
+        ctx.silu = silu
+        ctx.set_materialize_grads(False)
+        return y, final
+
+    @staticmethod
+    def backward(ctx, grad_y, grad_final):
+        x, weight, bias, state, lengths = ctx.saved_tensors
+        b, t, c = x.shape
+        w = weight.shape[1]
+        need = ctx.needs_input_grad
+        dev = x.device
+        x, batch_stride, row_stride = _rows(x)
+        gy = None if grad_y is None else grad_y.contiguous()
+        gf = None if grad_final is None else grad_final.contiguous()
+        gx = torch.empty(b, t, c, device=dev, dtype=x.dtype)
+        gs = torch.empty_like(state) if need[3] else None
+        gw = torch.zeros_like(weight) if b == 0 else torch.empty_like(weight)
+        gb = None if bias is None else torch.zeros_like(bias) if b == 0 else torch.empty_like(bias)
+        bf16 = int(x.dtype == torch.bfloat16)
+        rows = _hip.function("bssm_short_conv_partial_rows")(bf16, b, t, c)
+        partials = torch.empty(rows, w + 1, c, device=dev, dtype=torch.float32)
+        P = _hip.ptr
+        _hip.launch(dev, "bssm_short_conv_backward", bf16, int(weight.dtype == torch.bfloat16), w, int(ctx.silu), P(x),
+                    batch_stride, row_stride, P(weight), P(bias), P(state), P(lengths), P(gy), P(gf), P(gx), P(gs),
+                    P(partials), P(gw), P(gb), b, t, c, _hip.stream_of(dev))
+        return gx if need[0] else None, gw if need[1] else None, gb if need[2] else None, gs, None, None
+
+
+def causal_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activation: Optional[str] = None,
+                initial_state: Optional[Tensor] = None, lengths: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+    """Short causal depthwise filter over ``x [batch, time, channels]``; returns ``(y, final_state)``.
+
+    ``y[t] = act(bias + sum_j weight[:, j] x[t - W + 1 + j])`` with ``weight``
+    [channels, W] (or [channels, 1, W]), W = 2, 3 or 4, and ``activation``
+    None or "silu".  ``initial_state`` [batch, W-1, channels] holds the inputs
+    before the first token (zeros by default), oldest first; ``final_state``
+    is what the next call takes for it.  ``lengths`` [batch] (integers)
+    shortens rows: their tokens from there on give 0, take no part, and the
+    final state ends before them.
+
+    On a GPU, bfloat16 and float32 rows (any channel count; the rows of a
+    wider tensor in place) run on the HIP kernels, in float32 and rounded
+    once; other devices and dtypes run the formula in torch.
+    """
+    if not all(isinstance(z, Tensor) for z in (x, weight)):
+        raise TypeError("x and weight must be torch tensors")
+    if x.ndim != 3 or not x.is_floating_point():
+        raise ValueError("x must be floating point with shape [batch, time, channels]")
+    b, t, c = x.shape
+    if weight.ndim == 3 and weight.shape[1] == 1:
+        weight = weight.squeeze(1)
+    if weight.ndim != 2 or weight.shape[0] != c or weight.shape[1] not in (2, 3, 4):
+        raise ValueError(f"weight must have shape [{c}, W] with W = 2, 3 or 4, got {tuple(weight.shape)}")
+    if bias is not None and tuple(bias.shape) != (c,):
+        raise ValueError(f"bias must have shape [{c}], got {tuple(bias.shape)}")
+    if activation not in (None, "silu"):
+        raise ValueError('activation must be None or "silu"')
+    w = weight.shape[1]
+    if initial_state is not None:
+        if tuple(initial_state.shape) != (b, w - 1, c):
+            raise ValueError(f"initial_state must have shape {(b, w - 1, c)}, got {tuple(initial_state.shape)}")
+        if initial_state.dtype != x.dtype:
+            raise TypeError("initial_state must have x's dtype")
+    if any(z is not None and z.device != x.device for z in (weight, bias, initial_state)):
+        raise ValueError("x, weight, bias and initial_state must be on one device")
+    lengths = _check_lengths(lengths, b, x.device)
+    silu = activation == "silu"
+    if x.device.type != "cuda" or x.dtype not in (torch.bfloat16, torch.float32):
+        return _short_conv_formula(x, weight, bias, silu, initial_state, lengths)
+    _hip.load()  # on a GPU the kernels never degrade silently
+    if weight.dtype not in (torch.bfloat16, torch.float32) or (bias is not None and bias.dtype != weight.dtype):
+        weight, bias = weight.float(), None if bias is None else bias.float()
+    return _ShortConvFunction.apply(x, weight, bias, initial_state, lengths, silu)
+
+
+__all__ = ["CausalDepthwise4", "causal_conv", "causal_depthwise4"]

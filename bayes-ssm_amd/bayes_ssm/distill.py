@@ -1,0 +1,125 @@
+"""Distillation from a teacher's top logits on HIP kernels (C ABI ``bssm_distill_*``).
+
+A student's row of vocabulary logits is drawn toward the distribution that a
+teacher gives to a short list of entries.  With ``p = softmax(teacher / tau)``
+over the list and ``q = softmax(logits / tau)`` over the vocabulary,
+
+    loss = tau^2 sum_k p_k (log p_k - log q[index_k]),    gradient = tau (q - p).
+
+``tau^2`` keeps the gradient's scale as tau changes.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+from torch import Tensor
+
+from . import _hip
+
+MAX_TEACHER = 1024  # entries of a teacher's list that the kernels take
+
+
+def _formula(logits: Tensor, teacher: Tensor, index: Tensor, tau: float) -> tuple[Tensor, Tensor]:
+    """Losses of the rows in torch operations, float32 (float64 for float64 logits), and which rows have a teacher."""
+    x = logits.to(torch.promote_types(logits.dtype, torch.float32))
+    t = teacher.detach().to(x.dtype)
+    there = (index >= 0) & (index < x.shape[-1]) & (t != -math.inf)
+    rows = there.any(-1)
+    # Rows and entries that do not count are replaced before the softmax: no NaN comes out of them or their gradient.
+    x = torch.where(rows[:, None], x, torch.zeros_like(x))
+    t = torch.where(there, t, torch.full_like(t, -math.inf))
+    t = torch.where(rows[:, None], t, torch.zeros_like(t))
+    top = t.amax(-1, keepdim=True) if t.shape[-1] else t.new_zeros(t.shape[0], 1)
+    log_p = torch.log_softmax((t - top) / tau, -1)
+    p = torch.where(there, torch.exp(log_p), torch.zeros_like(t))
+    best = x.detach().amax(-1, keepdim=True)
+    best = torch.where(best == -math.inf, torch.zeros_like(best), best)
+    log_q = torch.log_softmax((x - best) / tau, -1).gather(-1, torch.where(there, index, torch.zeros_like(index)))
+    terms = torch.where(p > 0, p * (torch.where(p > 0, log_p, torch.zeros_like(p)) - log_q), p * 0.0)
+    return torch.where(rows, tau * tau * terms.sum(-1), torch.zeros_like(terms.sum(-1))), rows
+
+
+class _DistillFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher, index, tau, reduction):
+        r, v = logits.shape
+        k = index.shape[1]
+        dev = logits.device
+        loss = torch.empty(r, device=dev, dtype=torch.float32)
+        stats = torch.empty(r, 3, device=dev, dtype=torch.float32)
+        mean = None if reduction == "none" else torch.empty(3, device=dev, dtype=torch.float32)
+        P = _hip.ptr
+        kinds = int(logits.dtype == torch.bfloat16), int(teacher.dtype == torch.bfloat16)
+        _hip.launch(dev, "bssm_distill_forward", *kinds, P(logits), logits.stride(0), P(teacher), P(index), tau,
+                    P(loss), P(stats), P(mean), r, v, k, _hip.stream_of(dev))
+        ctx.save_for_backward(logits, teacher, index, stats, mean if reduction == "mean" else None)
+        ctx.tau, ctx.kinds, ctx.scalar = tau, kinds, reduction != "none"
+        return loss if mean is None else mean[0 if reduction == "mean" else 2].clone()
+
+    @staticmethod
+    def backward(ctx, grad):
+        logits, teacher, index, stats, mean = ctx.saved_tensors
+        r, v = logits.shape
+        dev = logits.device
+        out = torch.empty(r, v, device=dev, dtype=logits.dtype)
+        grad = grad.contiguous()
+        P = _hip.ptr
+        _hip.launch(dev, "bssm_distill_backward", *ctx.kinds, P(logits), logits.stride(0), P(teacher), P(index),
+                    ctx.tau, P(stats), P(mean), P(grad), int(ctx.scalar), P(out), r, v, index.shape[1],
+                    _hip.stream_of(dev))
+        return out, None, None, None, None
+
+
+def distillation_loss(logits: Tensor, teacher_logits: Tensor, teacher_index: Tensor, *, temperature: float = 1.0,
+                      reduction: str = "mean") -> Tensor:
+    """Distillation loss of ``logits [..., vocabulary]`` from a teacher's listed logits ``[..., entries]``.
+
+    ``teacher_index [..., entries]`` (integers) names each entry's place in
+    the vocabulary; entries outside [0, vocabulary) (conventionally -1) or
+    with a logit of -infinity do not count, and an index listed twice counts
+    twice.  A row without entries (prompt tokens, padding) has loss 0 and
+    gradient 0.  ``reduction``: "mean" over the rows that have entries, "sum",
+    or "none" (one loss a row).  The loss is float32, the gradient has the
+    logits' dtype; the teacher is a constant.
+
+    On a GPU, bfloat16 and float32 logits run on the HIP kernels (at most 1024
+    entries a row); other devices and dtypes run the formula in torch.
+    """
+    if not all(isinstance(z, Tensor) for z in (logits, teacher_logits, teacher_index)):
+        raise TypeError("logits, teacher_logits and teacher_index must be torch tensors")
+    if not (logits.is_floating_point() and teacher_logits.is_floating_point()):
+        raise TypeError("logits and teacher_logits must be floating point")
+    if teacher_index.is_floating_point() or teacher_index.dtype == torch.bool:
+        raise TypeError("teacher_index must hold integers")
+    if logits.ndim < 1 or logits.shape[-1] == 0:
+        raise ValueError("logits must have a vocabulary of at least one entry")
+    if teacher_index.shape != teacher_logits.shape or teacher_index.shape[:-1] != logits.shape[:-1]:
+        raise ValueError("teacher_logits and teacher_index must have the logits' leading axes and one shape")
+    if not (logits.device == teacher_logits.device == teacher_index.device):
+        raise ValueError("logits, teacher_logits and teacher_index must be on one device")
+    if not (math.isfinite(temperature) and temperature > 0):
+        raise ValueError("temperature must be positive and finite")
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError('reduction must be "mean", "sum" or "none"')
+    v, k, lead = logits.shape[-1], teacher_index.shape[-1], logits.shape[:-1]
+    rows = math.prod(lead)
+    x = logits.reshape(rows, v)
+    teacher, index = teacher_logits.detach().reshape(rows, k), teacher_index.reshape(rows, k).long()
+    if logits.device.type != "cuda" or logits.dtype not in (torch.bfloat16, torch.float32):
+        losses, has = _formula(x, teacher, index, float(temperature))
+        if reduction == "none":
+            return losses.reshape(lead)
+        return losses.sum() if reduction == "sum" else losses.sum() / has.sum().clamp_min(1)
+    if k > MAX_TEACHER:
+        raise ValueError(f"at most {MAX_TEACHER} teacher entries a row, got {k}")
+    _hip.load()  # on a GPU the kernels never degrade silently
+    if (v > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < v):
+        x = x.contiguous()
+    if teacher.dtype not in (torch.bfloat16, torch.float32):
+        teacher = teacher.float()
+    loss = _DistillFunction.apply(x, teacher.contiguous(), index.contiguous(), float(temperature), reduction)
+    return loss.reshape(lead) if reduction == "none" else loss
+
+
+__all__ = ["distillation_loss"]

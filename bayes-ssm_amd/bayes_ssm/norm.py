@@ -1,0 +1,120 @@
+"""Layer norm over the last axis on HIP kernels (C ABI ``bssm_layer_norm_*``).
+
+``y = (x - mean) / sqrt(variance + eps) * weight + bias`` with the statistics
+in float32, the row read once and the result rounded once.  The backward
+reduces the weight's and the bias's gradient in a fixed order, without atomics.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+import torch.nn as nn
+from torch import Tensor
+
+from . import _hip
+
+
+def _formula(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float) -> Tensor:
+    """``layer_norm`` in torch operations, in float32 (float64 for float64 inputs), rounded once."""
+    wide = x.to(torch.promote_types(x.dtype, torch.float32))
+    off = wide - wide.mean(-1, keepdim=True)
+    y = off * torch.rsqrt(off.square().mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        y = y * weight.to(y.dtype)
+    if bias is not None:
+        y = y + bias.to(y.dtype)
+    return y.to(x.dtype)
+
+
+class _LayerNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        r, d = x.shape
+        dev = x.device
+        y = torch.empty(r, d, device=dev, dtype=x.dtype)
+        keep = any(ctx.needs_input_grad)
+        stats = torch.empty(2, r, device=dev, dtype=torch.float32) if keep else None
+        mean, rstd = (None, None) if stats is None else (stats[0], stats[1])
+        weight, bias = (None if z is None else z.contiguous() for z in (weight, bias))
+        params = [z for z in (weight, bias) if z is not None]
+        param_bf16 = int(bool(params) and params[0].dtype == torch.bfloat16)
+        P = _hip.ptr
+        _hip.launch(dev, "bssm_layer_norm_forward", int(x.dtype == torch.bfloat16), param_bf16, P(x), x.stride(0),
+                    P(weight), P(bias), eps, P(y), P(mean), P(rstd), r, d, _hip.stream_of(dev))
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.param_bf16 = param_bf16
+        return y
+
+    @staticmethod
+    def backward(ctx, grad_y):
+        x, weight, bias, stats = ctx.saved_tensors
+        r, d = x.shape
+        dev = x.device
+        need = ctx.needs_input_grad
+        bf16 = int(x.dtype == torch.bfloat16)
+        gy = grad_y.contiguous()
+        gx = torch.empty(r, d, device=dev, dtype=x.dtype) if need[0] else None
+        gw = torch.empty_like(weight) if need[1] else None
+        gb = torch.empty_like(bias) if need[2] else None
+        partials = None
+        if gw is not None or gb is not None:
+            rows = _hip.function("bssm_layer_norm_partial_rows")(bf16, r, d)
+            partials = torch.empty(rows, 2, d, device=dev, dtype=torch.float32)
+            if r == 0:
+                partials = torch.empty(1, 2, d, device=dev, dtype=torch.float32)
+        P = _hip.ptr
+        _hip.launch(dev, "bssm_layer_norm_backward", bf16, ctx.param_bf16, P(x), x.stride(0), P(weight), P(stats[0]),
+                    P(stats[1]), P(gy), P(gx), P(partials), P(gw), P(gb), r, d, _hip.stream_of(dev))
+        return gx, gw, gb, None
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, *,
+               eps: float = 1e-5) -> Tensor:
+    """Layer norm of ``x [..., width]`` with ``weight`` and ``bias`` [width] (either may be absent).
+
+    On a GPU, bfloat16 and float32 rows of any width (rows of a wider tensor
+    in place) run on the HIP kernels; weight and bias may be bfloat16 or
+    float32, and their gradients come back in their own dtype.  Other devices
+    and dtypes run the formula in torch.
+    """
+    if not isinstance(x, Tensor) or not x.is_floating_point():
+        raise TypeError("x must be a floating-point tensor")
+    if x.ndim < 1 or x.shape[-1] == 0:
+        raise ValueError("x must have a last axis of at least one value")
+    d = x.shape[-1]
+    for z, name in ((weight, "weight"), (bias, "bias")):
+        if z is not None and tuple(z.shape) != (d,):
+            raise ValueError(f"{name} must have shape [{d}], got {tuple(z.shape)}")
+        if z is not None and z.device != x.device:
+            raise ValueError(f"{name} must be on x's device")
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError("eps must be finite and not negative")
+    if x.device.type != "cuda" or x.dtype not in (torch.bfloat16, torch.float32):
+        return _formula(x, weight, bias, eps)
+    _hip.load()  # on a GPU the kernels never degrade silently
+    kinds = {z.dtype for z in (weight, bias) if z is not None}
+    if len(kinds) > 1 or not kinds <= {torch.bfloat16, torch.float32}:
+        weight, bias = (None if z is None else z.float() for z in (weight, bias))
+    rows = x.reshape(-1, d)
+    if (d > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < d):
+        rows = rows.contiguous()
+    return _LayerNormFunction.apply(rows, weight, bias, float(eps)).reshape(x.shape)
+
+
+class LayerNorm(nn.Module):
+    """``layer_norm`` with learned weight and bias over ``width`` values."""
+
+    def __init__(self, width: int, *, eps: float = 1e-5, bias: bool = True,
+                 dtype: torch.dtype = torch.float32, device: torch.device | str | None = None):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(width, dtype=dtype, device=device))
+        self.bias = nn.Parameter(torch.zeros(width, dtype=dtype, device=device)) if bias else None
+
+    def forward(self, x: Tensor) -> Tensor:
+        return layer_norm(x, self.weight, self.bias, eps=self.eps)
+
+
+__all__ = ["LayerNorm", "layer_norm"]

@@ -1,0 +1,338 @@
+"""Selective state space scan and its single-token step on HIP kernels (C ABI ``bssm_select_*``).
+
+The other recurrent mixer that a language model may hold beside the Bayesian
+layer: per head a state [values, n] that decays by ``exp(step A)`` and takes
+in ``step x B^T``, with the time step, B and C chosen by each token:
+
+    step = softplus(dt + dt_bias)
+    h[t] = exp(step A) h[t-1] + step x[t] B[t]^T,      y[t] = h[t] C[t] + D x[t].
+
+``selective_scan`` runs prompts and training (with gradients),
+``selective_step`` one token from carried states, the short causal filter
+(``bayes_ssm.conv.causal_conv``) in front of it included.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn.functional as F
+from torch import Tensor
+
+from . import _hip
+from .conv import _check_lengths
+
+MAX_STATE = 128  # n that the kernels take
+
+
+def _scan_formula(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor],
+                  dt_bias: Optional[Tensor], softplus: bool, state: Optional[Tensor],
+                  lengths: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    """``selective_scan`` token by token in torch operations, float32 (float64 for float64 inputs), rounded once."""
+    b, t, h, p = x.shape
+    g, n = B.shape[2:]
+    wide = torch.promote_types(x.dtype, torch.float32)
+    xw, A = x.to(wide), A.to(wide)
+    step = dt.to(wide) if dt_bias is None else dt.to(wide) + dt_bias.to(wide)
+    if softplus:
+        step = F.softplus(step)
+    live = None
+    if lengths is not None:
+        live = (torch.arange(t, device=x.device) < lengths[:, None])[..., None]
+        step = step.masked_fill(~live, 0.0)
+        xw = xw.masked_fill(~live[..., None], 0.0)
+    Bw, Cw = (z.to(wide) if live is None else z.to(wide).masked_fill(~live[..., None], 0.0) for z in (B, C))
+    Bw, Cw = (z.repeat_interleave(h // g, 2) for z in (Bw, Cw))
+    h_t = xw.new_zeros(b, h, p, n) if state is None else state.to(wide)
+    ys = []
+    for i in range(t):
+        u = step[:, i, :, None] * xw[:, i]
+        h_t = torch.exp(step[:, i] * A)[..., None, None] * h_t + u[..., None] * Bw[:, i, :, None]
+        ys.append((h_t * Cw[:, i, :, None]).sum(-1))
+    y = torch.stack(ys, 1) if ys else torch.zeros_like(xw)
+    if D is not None:
+        y = y + D.to(wide)[:, None] * xw
+    if live is not None:
+        y = y.masked_fill(~live[..., None], 0.0)
+    return y.to(x.dtype), h_t
+
+
+def _strides(x: Tensor) -> list[int]:
+    """Strides of the leading axes (elements); 0 for an axis of one element, whose stride means nothing."""
+    return [s if n > 1 else 0 for s, n in zip(x.stride()[:-1], x.shape[:-1])]
+
+
+def _inner(x: Tensor) -> Tensor:
+    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+class _ScanFunction(torch.autograd.Function):
+    """Autograd boundary of the scan (C ABI ``bssm_select_forward/backward``)."""
+
+    @staticmethod
+    def _head(x, dt, A, B, C, D, dt_bias, softplus, lengths):
+        P = _hip.ptr
+        return (int(x.dtype == torch.bfloat16), P(x), *_strides(x), int(dt.dtype == torch.bfloat16), P(dt),
+                *_strides(dt), P(A), P(B), *_strides(B), P(C), *_strides(C), P(D), P(dt_bias), int(softplus),
+                P(lengths))
+
+    @staticmethod
+    def forward(ctx, x, dt, A, B, C, D, dt_bias, state, lengths, softplus):
+        b, t, h, p = x.shape
+        g, n = B.shape[2:]
+        dev = x.device
+        x, dt, B, C = (_inner(z) for z in (x, dt, B, C))
+        A, D, dt_bias, state = (None if z is None else _hip.aligned(z) for z in (A, D, dt_bias, state))
+        size = lambda what: _hip.function("bssm_select_sizes")(  # noqa: E731
+            what, int(x.dtype == torch.bfloat16), b, t, h, p, n, g)
+        keep = any(ctx.needs_input_grad)
+        y = torch.empty(b, t, h, p, device=dev, dtype=x.dtype)
+        last = torch.empty(b, h, p, n, device=dev, dtype=torch.float32)
+        states = torch.empty(b, h, size(0), p, n, device=dev, dtype=torch.float32) if keep else None
+        work = size(1)
+        segments = torch.empty(work, device=dev, dtype=torch.float32) if work else None
+        P = _hip.ptr
+        _hip.launch(dev, "bssm_select_forward", *_ScanFunction._head(x, dt, A, B, C, D, dt_bias, softplus, lengths),
+                    P(state), P(y), P(last), P(states), P(segments), b, t, h, p, n, g, _hip.stream_of(dev))
+        if keep:
+            ctx.save_for_backward(x, dt, A, B, C, D, dt_bias, lengths, states)
+            ctx.softplus = softplus
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    def backward(ctx, grad_y, grad_last):
+        x, dt, A, B, C, D, dt_bias, lengths, states = ctx.saved_tensors
+        b, t, h, p = x.shape
+        g, n = B.shape[2:]
+        dev = x.device
+        need = ctx.needs_input_grad
+        bf16 = int(x.dtype == torch.bfloat16)
+        size = lambda what: _hip.function("bssm_select_sizes")(what, bf16, b, t, h, p, n, g)  # noqa: E731
+        gy = torch.zeros(b, t, h, p, device=dev, dtype=x.dtype) if grad_y is None else _hip.aligned(grad_y)
+        gl = None if grad_last is None else _hip.aligned(grad_last.float())
+        records, work, parts = size(0), size(1), size(2)
+
+        def f32(*shape):
+            return torch.empty(*shape, device=dev, dtype=torch.float32)
+
+        adjoints = f32(b, h, records, p, n)
+        segments = f32(work) if work else None
+        partial = f32(parts, 2, b, t, g, n) if parts > 1 else None
+        rows = f32(max(1, b * records), 3, h)
+        gx = torch.empty(b, t, h, p, device=dev, dtype=x.dtype)
+        gdt = torch.empty(b, t, h, device=dev, dtype=dt.dtype)
+        gB, gC = (torch.empty(b, t, g, n, device=dev, dtype=x.dtype) for _ in range(2))
+        gA, gD, gbias = f32(h), None if D is None else f32(h), None if dt_bias is None else f32(h)
+        gstate = f32(b, h, p, n) if need[7] else None
+        if gstate is not None and b * t == 0:
+            gstate = torch.zeros_like(gstate) if gl is None else gl.clone()
+        P = _hip.ptr
+        _hip.launch(dev, "bssm_select_backward",
+                    *_ScanFunction._head(x, dt, A, B, C, D, dt_bias, ctx.softplus, lengths), P(states), P(gy), P(gl),
+                    P(adjoints), P(segments), P(partial), P(rows), P(gx), P(gdt), P(gA), P(gB), P(gC), P(gD), P(gbias),
+                    P(gstate), b, t, h, p, n, g, _hip.stream_of(dev))
+        grads = (gx, gdt, gA, gB, gC, gD, gbias, gstate)
+        return (*(z if need[i] else None for i, z in enumerate(grads)), None, None)
+
+
+def _check_heads(name: str, z: Optional[Tensor], heads: int, device: torch.device) -> Optional[Tensor]:
+    """A per-head parameter in float32."""
+    if z is None:
+        return None
+    if tuple(z.shape) != (heads,):
+        raise ValueError(f"{name} must have shape [{heads}], got {tuple(z.shape)}")
+    if z.device != device:
+        raise ValueError(f"{name} must be on the inputs' device")
+    return z
+
+
+def selective_scan(
+    x: Tensor,
+    dt: Tensor,
+    A: Tensor,
+    B: Tensor,
+    C: Tensor,
+    *,
+    D: Optional[Tensor] = None,
+    dt_bias: Optional[Tensor] = None,
+    dt_softplus: bool = True,
+    initial_state: Optional[Tensor] = None,
+    lengths: Optional[Tensor] = None,
+) -> tuple[Tensor, Tensor]:
+    """Selective state space scan over a sequence; returns ``(y, final_state)``.
+
+    x: [batch, time, heads, values]; dt: [batch, time, heads] (x's dtype or
+    float32); B, C: [batch, time, groups, n] in x's dtype, head i reads group
+    i // (heads / groups); A (negative), D and dt_bias: [heads].
+    ``initial_state`` [batch, heads, values, n] is float32 (zeros by default),
+    as is ``final_state``.  ``dt_softplus`` False takes dt + dt_bias as the
+    step.  ``lengths`` [batch] (integers) shortens rows: their tokens from
+    there on give 0, take no part and leave the state.
+
+    On a GPU, bfloat16 and float32 streams with n <= 128 run on the HIP
+    kernels, in place where the innermost axis is contiguous (column slices of
+    a projection); a larger n raises.  Every input has a gradient, also
+    through ``final_state``.  Other devices and dtypes run the recurrence in
+    torch, token by token.
+    """
+    if not all(isinstance(z, Tensor) and z.is_floating_point() for z in (x, dt, A, B, C)):
+        raise TypeError("x, dt, A, B and C must be floating-point tensors")
+    if x.ndim != 4 or B.ndim != 4 or C.ndim != 4:
+        raise ValueError("x must have shape [batch, time, heads, values], B and C [batch, time, groups, n]")
+    b, t, h, p = x.shape
+    g, n = B.shape[2:]
+    if h == 0 or p == 0 or n == 0 or g == 0 or h % g:
+        raise ValueError(f"heads ({h}) must be a positive multiple of groups ({g}), values and n positive")
+    if tuple(B.shape[:2]) != (b, t) or B.shape != C.shape:
+        raise ValueError(f"B and C must have shape [{b}, {t}, groups, n], got {tuple(B.shape)} and {tuple(C.shape)}")
+    if tuple(dt.shape) != (b, t, h):
+        raise ValueError(f"dt must have shape {(b, t, h)}, got {tuple(dt.shape)}")
+    if B.dtype != x.dtype or C.dtype != x.dtype:
+        raise TypeError("B and C must have x's dtype")
+    if any(z.device != x.device for z in (dt, B, C)):
+        raise ValueError("x, dt, B and C must be on one device")
+    A, D, dt_bias = (_check_heads(k, z, h, x.device) for k, z in (("A", A), ("D", D), ("dt_bias", dt_bias)))
+    if initial_state is not None:
+        if tuple(initial_state.shape) != (b, h, p, n):
+            raise ValueError(f"initial_state must have shape {(b, h, p, n)}, got {tuple(initial_state.shape)}")
+        if initial_state.device != x.device:
+            raise ValueError("initial_state must be on the inputs' device")
+    lengths = _check_lengths(lengths, b, x.device)
+    if x.device.type != "cuda" or x.dtype not in (torch.bfloat16, torch.float32):
+        return _scan_formula(x, dt, A, B, C, D, dt_bias, dt_softplus, initial_state, lengths)
+    if n > MAX_STATE:
+        raise ValueError(f"at most {MAX_STATE} states a value on the GPU, got {n}")
+    _hip.load()  # on a GPU the kernels never degrade silently
+    if dt.dtype not in (torch.bfloat16, torch.float32):
+        dt = dt.float()
+    A, D, dt_bias, initial_state = (None if z is None else z.float() for z in (A, D, dt_bias, initial_state))
+    return _ScanFunction.apply(x, dt, A, B, C, D, dt_bias, initial_state, lengths, bool(dt_softplus))
+
+
+def _step_formula(row: Tensor, dt: Tensor, conv_state: Tensor, state: Tensor, weight: Tensor, bias: Optional[Tensor],
+                  silu: bool, A: Tensor, D: Optional[Tensor], dt_bias: Optional[Tensor], softplus: bool,
+                  groups: int) -> tuple[Tensor, Tensor, Tensor]:
+    b, h, p, n = state.shape
+    wide = torch.promote_types(row.dtype, torch.float32)
+    rows = torch.cat((conv_state, row[:, None]), 1)
+    z = (rows.to(wide) * weight.to(wide).t()).sum(1)
+    if bias is not None:
+        z = z + bias.to(wide)
+    if silu:
+        z = F.silu(z)
+    x, B, C = z.split((h * p, groups * n, groups * n), -1)
+    y, last = _scan_formula(x.reshape(b, 1, h, p), dt[:, None], A, B.reshape(b, 1, groups, n),
+                            C.reshape(b, 1, groups, n), D, dt_bias, softplus, state, None)
+    return y[:, 0].to(row.dtype), rows[:, 1:].contiguous(), last.to(state.dtype)
+
+
+def _overlap(a: Tensor, b: Tensor) -> bool:
+    first, last = a.data_ptr(), a.data_ptr() + a.numel() * a.element_size()
+    return b.data_ptr() < last and first < b.data_ptr() + b.numel() * b.element_size()
+
+
+def selective_step(
+    row: Tensor,
+    dt: Tensor,
+    conv_state: Tensor,
+    state: Tensor,
+    conv_weight: Tensor,
+    A: Tensor,
+    *,
+    groups: int = 1,
+    conv_bias: Optional[Tensor] = None,
+    activation: Optional[str] = "silu",
+    D: Optional[Tensor] = None,
+    dt_bias: Optional[Tensor] = None,
+    dt_softplus: bool = True,
+    out_states: Optional[tuple[Tensor, Tensor]] = None,
+) -> tuple[Tensor, Tensor, Tensor]:
+    """One token of ``causal_conv`` and ``selective_scan``; returns ``(y, conv_state, state)``.
+
+    row: [batch, heads * values + 2 * groups * n], the filter's new inputs (the
+    heads' values, then every group's B, then every group's C; a column slice
+    of the token's projection is read in place); dt: [batch, heads];
+    conv_state [batch, W-1, columns] (row's dtype) and state [batch, heads,
+    values, n] (float32) as the two operators return them; conv_weight
+    [columns, W].  The new states are new tensors, or ``out_states``: the
+    second may be ``state`` itself (an update in place), the first may not
+    overlap ``conv_state``.
+
+    For inference: it records no gradients.  On a GPU one launch runs both
+    operators, with the filter's output kept in float32.
+    """
+    if torch.is_grad_enabled() and any(isinstance(z, Tensor) and z.requires_grad for z in (
+            row, dt, conv_state, state, conv_weight, A, conv_bias, D, dt_bias)):
+        raise RuntimeError("selective_step records no gradients: call it under torch.no_grad()")
+    if not all(isinstance(z, Tensor) and z.is_floating_point() for z in (row, dt, conv_state, state, conv_weight, A)):
+        raise TypeError("row, dt, conv_state, state, conv_weight and A must be floating-point tensors")
+    if state.ndim != 4 or row.ndim != 2:
+        raise ValueError("state must have shape [batch, heads, values, n] and row [batch, columns]")
+    b, h, p, n = state.shape
+    if groups <= 0 or h == 0 or p == 0 or n == 0 or h % groups:
+        raise ValueError(f"heads ({h}) must be a positive multiple of groups ({groups}), values and n positive")
+    c = h * p + 2 * groups * n
+    if tuple(row.shape) != (b, c):
+        raise ValueError(f"row must have shape {(b, c)}, got {tuple(row.shape)}")
+    if tuple(dt.shape) != (b, h):
+        raise ValueError(f"dt must have shape {(b, h)}, got {tuple(dt.shape)}")
+    if conv_weight.ndim == 3 and conv_weight.shape[1] == 1:
+        conv_weight = conv_weight.squeeze(1)
+    if conv_weight.ndim != 2 or conv_weight.shape[0] != c or conv_weight.shape[1] not in (2, 3, 4):
+        raise ValueError(f"conv_weight must have shape [{c}, W] with W = 2, 3 or 4, got {tuple(conv_weight.shape)}")
+    w = conv_weight.shape[1]
+    if tuple(conv_state.shape) != (b, w - 1, c) or conv_state.dtype != row.dtype:
+        raise ValueError(f"conv_state must have shape {(b, w - 1, c)} and row's dtype")
+    if conv_bias is not None and tuple(conv_bias.shape) != (c,):
+        raise ValueError(f"conv_bias must have shape [{c}], got {tuple(conv_bias.shape)}")
+    if activation not in (None, "silu"):
+        raise ValueError('activation must be None or "silu"')
+    if any(z is not None and z.device != row.device for z in (dt, conv_state, state, conv_weight, conv_bias)):
+        raise ValueError("all inputs must be on one device")
+    A, D, dt_bias = (_check_heads(k, z, h, row.device) for k, z in (("A", A), ("D", D), ("dt_bias", dt_bias)))
+    if out_states is not None:
+        for z, like, name in zip(out_states, (conv_state, state), ("conv_state", "state")):
+            if z.shape != like.shape or z.dtype != like.dtype or z.device != like.device or not z.is_contiguous():
+                raise ValueError(f"out_states must be contiguous tensors like conv_state and state ({name} is not)")
+        if _overlap(out_states[0], conv_state):
+            raise ValueError("the new conv_state may not overlap conv_state")
+        if out_states[1].data_ptr() != state.data_ptr() and _overlap(out_states[1], state):
+            raise ValueError("the new state must be state itself or not overlap it")
+    silu = activation == "silu"
+    fused = (row.device.type == "cuda" and row.dtype in (torch.bfloat16, torch.float32)
+             and state.dtype == torch.float32)
+    if not fused:
+        out = _step_formula(row, dt, conv_state, state, conv_weight, conv_bias, silu, A, D, dt_bias, dt_softplus,
+                            groups)
+        if out_states is None:
+            return out
+        for z, new in zip(out_states, out[1:]):
+            z.copy_(new)
+        return (out[0], *out_states)
+    if n > MAX_STATE:
+        raise ValueError(f"at most {MAX_STATE} states a value on the GPU, got {n}")
+    _hip.load()  # on a GPU the kernels never degrade silently
+    if row.stride(1) != 1:
+        row = row.contiguous()
+    dt, conv_state, state_in = _inner(dt), conv_state.contiguous(), state.contiguous()
+    if dt.dtype not in (torch.bfloat16, torch.float32):
+        dt = dt.float()
+    if conv_weight.dtype not in (torch.bfloat16, torch.float32) or (
+            conv_bias is not None and conv_bias.dtype != conv_weight.dtype):
+        conv_weight, conv_bias = conv_weight.float(), None if conv_bias is None else conv_bias.float()
+    conv_weight, conv_bias = (None if z is None else z.contiguous() for z in (conv_weight, conv_bias))
+    A, D, dt_bias = (None if z is None else z.float().contiguous() for z in (A, D, dt_bias))
+    dev = row.device
+    y = torch.empty(b, h, p, device=dev, dtype=row.dtype)
+    next_conv, next_state = (torch.empty_like(conv_state), torch.empty_like(state_in)) if out_states is None else out_states
+    P = _hip.ptr
+    _hip.launch(dev, "bssm_select_step", int(row.dtype == torch.bfloat16), int(conv_weight.dtype == torch.bfloat16), w,
+                int(silu), P(row), row.stride(0) if b > 1 else 0, int(dt.dtype == torch.bfloat16), P(dt),
+                dt.stride(0) if b > 1 else 0, P(conv_state), P(state_in), P(conv_weight), P(conv_bias), P(A), P(D),
+                P(dt_bias), int(dt_softplus), P(y), P(next_conv), P(next_state), b, h, p, n, groups,
+                _hip.stream_of(dev))
+    return y, next_conv, next_state
+
+
+__all__ = ["selective_scan", "selective_step"]

@@ -11,10 +11,13 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <cmath>
 #include <initializer_list>
+#include <utility>
 
 #include "../../include/bssm.h"
 #include "bssm_recurrence.h"
+#include "bssm_sequence.h"
 
 namespace {
 
@@ -263,7 +266,7 @@ extern "C" {
 
 const char* bssm_last_error(void) { return g_error; }
 
-int bssm_abi_version(void) { return 10; }
+int bssm_abi_version(void) { return 11; }
 
 int bssm_supported(int key_dim, int value_dim) { return supported(key_dim, value_dim) ? 1 : 0; }
 
@@ -1200,6 +1203,286 @@ int bssm_associative_static_scan_backward(const float* keys, const float* values
                           keys, values, queries, observation, mean0, cov0, grad_out, grad_mean_final, grad_cov_final,
                           workspace, grad_keys, grad_values, grad_queries, grad_observation, grad_mean0, grad_cov0, b,
                           t, key_dim, value_dim, static_cast<hipStream_t>(stream)));
+}
+
+
+}  // extern "C"
+
+// ---- short causal filter, layer norm, distillation loss, selective scan
+
+namespace {
+
+// One workgroup handles at least one element, so counts below 2^31 keep every grid in range.
+int check_size(const char* fn, int64_t elements) {
+  if (elements >= (int64_t)1 << 40) return fail(BSSM_ERR_ARGUMENT, "%s: too many elements (%lld)", fn, (long long)elements);
+  return BSSM_OK;
+}
+int check_grid(const char* fn, int64_t blocks) {
+  if (blocks >= (int64_t)1 << 31) return fail(BSSM_ERR_ARGUMENT, "%s: too many workgroups (%lld)", fn, (long long)blocks);
+  return BSSM_OK;
+}
+int need(const char* fn, std::initializer_list<std::pair<const void*, const char*>> ptrs) {
+  for (const auto& p : ptrs)
+    if (p.first == nullptr) return fail(BSSM_ERR_ARGUMENT, "%s: %s is null", fn, p.second);
+  return BSSM_OK;
+}
+
+int short_conv_check(const char* fn, const bssm::ShortConvArgs& a) {
+  if (a.w < 2 || a.w > 4) return fail(BSSM_ERR_UNSUPPORTED, "%s: width must be 2, 3 or 4, got %d", fn, a.w);
+  if (a.b < 0 || a.t < 0 || a.c < 0) return fail(BSSM_ERR_ARGUMENT, "%s: negative size", fn);
+  if (a.t > 1 && a.x_row < a.c) return fail(BSSM_ERR_ARGUMENT, "%s: x rows overlap", fn);
+  if (int rc = check_size(fn, a.b * (a.t + 1) * a.c)) return rc;
+  return check_grid(fn, a.b * a.c * (a.t / 4 + 1) / 64);
+}
+
+int layer_norm_check(const char* fn, const bssm::LayerNormArgs& a) {
+  if (a.r < 0 || a.d <= 0) return fail(BSSM_ERR_ARGUMENT, "%s: needs rows >= 0 and width >= 1", fn);
+  if (a.r > 1 && a.x_row < a.d) return fail(BSSM_ERR_ARGUMENT, "%s: x rows overlap", fn);
+  if (!(a.eps >= 0.f)) return fail(BSSM_ERR_ARGUMENT, "%s: eps must not be negative", fn);
+  if (int rc = check_size(fn, a.r * a.d)) return rc;
+  return check_grid(fn, a.r);
+}
+
+int distill_check(const char* fn, const bssm::DistillArgs& a) {
+  if (a.r < 0 || a.v <= 0 || a.k < 0) return fail(BSSM_ERR_ARGUMENT, "%s: needs rows >= 0, vocabulary >= 1, teacher >= 0", fn);
+  if (a.k > bssm::kDistillMaxTeacher)
+    return fail(BSSM_ERR_UNSUPPORTED, "%s: at most %d teacher entries a row, got %lld", fn, bssm::kDistillMaxTeacher,
+                (long long)a.k);
+  if (a.r > 1 && a.logits_row < a.v) return fail(BSSM_ERR_ARGUMENT, "%s: logits rows overlap", fn);
+  if (!(a.tau > 0.f) || !(a.tau < INFINITY)) return fail(BSSM_ERR_ARGUMENT, "%s: temperature must be positive and finite", fn);
+  if (int rc = check_size(fn, a.r * a.v)) return rc;
+  return check_grid(fn, a.r);
+}
+
+int select_check(const char* fn, int64_t b, int64_t t, int64_t h, int64_t p, int64_t n, int64_t g) {
+  if (b < 0 || t < 0 || h <= 0 || p <= 0 || n <= 0 || g <= 0)
+    return fail(BSSM_ERR_ARGUMENT, "%s: needs batch, tokens >= 0 and heads, values, states, groups >= 1", fn);
+  if (h % g != 0) return fail(BSSM_ERR_ARGUMENT, "%s: heads (%lld) must be a multiple of groups (%lld)", fn, (long long)h, (long long)g);
+  if (n > bssm::kSelectMaxState)
+    return fail(BSSM_ERR_UNSUPPORTED, "%s: at most %d states, got %lld", fn, bssm::kSelectMaxState, (long long)n);
+  if (int rc = check_size(fn, b * (t + 1) * h * (p + n))) return rc;
+  if (int rc = check_size(fn, b * h * p * n)) return rc;
+  return check_grid(fn, b * h * ((t + 63) / 64 + 1) * ((p + 7) / 8));
+}
+
+bssm::SelectArgs select_args(int bf16, const void* x, int64_t x_batch, int64_t x_row, int64_t x_head, int dt_bf16,
+                             const void* dt, int64_t dt_batch, int64_t dt_row, const float* rate, const void* bk,
+                             int64_t bk_batch, int64_t bk_row, int64_t bk_group, const void* cq, int64_t cq_batch,
+                             int64_t cq_row, int64_t cq_group, const float* skip, const float* dt_bias, int softplus,
+                             const int64_t* lengths, int64_t b, int64_t t, int64_t h, int64_t p, int64_t n, int64_t g) {
+  bssm::SelectArgs a{};
+  a.x = x; a.x_batch = x_batch; a.x_row = x_row; a.x_head = x_head;
+  a.dt = dt; a.dt_batch = dt_batch; a.dt_row = dt_row;
+  a.bk = bk; a.bk_batch = bk_batch; a.bk_row = bk_row; a.bk_group = bk_group;
+  a.cq = cq; a.cq_batch = cq_batch; a.cq_row = cq_row; a.cq_group = cq_group;
+  a.rate = rate; a.skip = skip; a.dt_bias = dt_bias; a.lengths = lengths;
+  a.b = b; a.t = t; a.h = h; a.p = p; a.n = n; a.g = g;
+  a.bf16 = bf16 != 0; a.dt_bf16 = dt_bf16 != 0; a.softplus = softplus != 0;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t bssm_short_conv_partial_rows(int bf16, int64_t batch, int64_t t, int64_t channels) {
+  return bssm::short_conv_partial_rows(batch, t, channels, bf16 != 0);
+}
+
+int bssm_short_conv_forward(int bf16, int param_bf16, int width, int silu, const void* x, int64_t x_batch,
+                            int64_t x_row, const void* weight, const void* bias, const void* state,
+                            const int64_t* lengths, void* y, void* final_state, int64_t batch, int64_t t,
+                            int64_t channels, void* stream) {
+  const char* fn = "bssm_short_conv_forward";
+  bssm::ShortConvArgs a{};
+  a.x = x; a.x_batch = x_batch; a.x_row = x_row; a.weight = weight; a.bias = bias; a.state = state;
+  a.lengths = lengths; a.y = y; a.final_state = final_state;
+  a.b = batch; a.t = t; a.c = channels; a.w = width; a.bf16 = bf16 != 0; a.param_bf16 = param_bf16 != 0; a.silu = silu != 0;
+  if (int rc = short_conv_check(fn, a)) return rc;
+  if (batch * channels == 0) return ok();
+  if (int rc = need(fn, {{weight, "weight"}})) return rc;
+  if (t > 0)
+    if (int rc = need(fn, {{x, "x"}, {y, "y"}})) return rc;
+  return launched(fn, bssm::launch_short_conv_forward(a, static_cast<hipStream_t>(stream)));
+}
+
+int bssm_short_conv_backward(int bf16, int param_bf16, int width, int silu, const void* x, int64_t x_batch,
+                             int64_t x_row, const void* weight, const void* bias, const void* state,
+                             const int64_t* lengths, const void* grad_y, const void* grad_final_state, void* grad_x,
+                             void* grad_state, float* partials, void* grad_weight, void* grad_bias, int64_t batch,
+                             int64_t t, int64_t channels, void* stream) {
+  const char* fn = "bssm_short_conv_backward";
+  bssm::ShortConvArgs a{};
+  a.x = x; a.x_batch = x_batch; a.x_row = x_row; a.weight = weight; a.bias = bias; a.state = state;
+  a.lengths = lengths; a.gy = grad_y; a.gfinal = grad_final_state; a.gx = grad_x; a.gstate = grad_state;
+  a.partials = partials; a.gweight = grad_weight; a.gbias = grad_bias;
+  a.b = batch; a.t = t; a.c = channels; a.w = width; a.bf16 = bf16 != 0; a.param_bf16 = param_bf16 != 0; a.silu = silu != 0;
+  if (int rc = short_conv_check(fn, a)) return rc;
+  if (batch * channels == 0) return ok();
+  if (int rc = need(fn, {{weight, "weight"}})) return rc;
+  if (t > 0)
+    if (int rc = need(fn, {{x, "x"}, {grad_x, "grad_x"}})) return rc;
+  if ((grad_weight != nullptr || grad_bias != nullptr) && partials == nullptr)
+    return fail(BSSM_ERR_ARGUMENT, "%s: the weight's and the bias's gradient need partials", fn);
+  return launched(fn, bssm::launch_short_conv_backward(a, static_cast<hipStream_t>(stream)));
+}
+
+int64_t bssm_layer_norm_partial_rows(int bf16, int64_t rows, int64_t width) {
+  return bssm::layer_norm_partial_rows(rows, width, bf16 != 0);
+}
+
+int bssm_layer_norm_forward(int bf16, int param_bf16, const void* x, int64_t x_row, const void* weight,
+                            const void* bias, float eps, void* y, float* mean, float* rstd, int64_t rows,
+                            int64_t width, void* stream) {
+  const char* fn = "bssm_layer_norm_forward";
+  bssm::LayerNormArgs a{};
+  a.x = x; a.x_row = x_row; a.weight = weight; a.bias = bias; a.eps = eps; a.y = y; a.mean = mean; a.rstd = rstd;
+  a.r = rows; a.d = width; a.bf16 = bf16 != 0; a.param_bf16 = param_bf16 != 0;
+  if (int rc = layer_norm_check(fn, a)) return rc;
+  if (rows == 0) return ok();
+  if (int rc = need(fn, {{x, "x"}, {y, "y"}})) return rc;
+  if ((mean == nullptr) != (rstd == nullptr)) return fail(BSSM_ERR_ARGUMENT, "%s: mean and rstd go together", fn);
+  return launched(fn, bssm::launch_layer_norm_forward(a, static_cast<hipStream_t>(stream)));
+}
+
+int bssm_layer_norm_backward(int bf16, int param_bf16, const void* x, int64_t x_row, const void* weight,
+                             const float* mean, const float* rstd, const void* grad_y, void* grad_x, float* partials,
+                             void* grad_weight, void* grad_bias, int64_t rows, int64_t width, void* stream) {
+  const char* fn = "bssm_layer_norm_backward";
+  bssm::LayerNormArgs a{};
+  a.x = x; a.x_row = x_row; a.weight = weight; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
+  a.gy = grad_y; a.gx = grad_x; a.gweight = grad_weight; a.gbias = grad_bias;
+  a.partials = grad_weight != nullptr || grad_bias != nullptr ? partials : nullptr;
+  a.r = rows; a.d = width; a.bf16 = bf16 != 0; a.param_bf16 = param_bf16 != 0;
+  if (int rc = layer_norm_check(fn, a)) return rc;
+  if (rows > 0)
+    if (int rc = need(fn, {{x, "x"}, {mean, "mean"}, {rstd, "rstd"}, {grad_y, "grad_y"}})) return rc;
+  if ((grad_weight != nullptr || grad_bias != nullptr) && partials == nullptr)
+    return fail(BSSM_ERR_ARGUMENT, "%s: the weight's and the bias's gradient need partials", fn);
+  return launched(fn, bssm::launch_layer_norm_backward(a, static_cast<hipStream_t>(stream)));
+}
+
+int bssm_distill_forward(int bf16, int teacher_bf16, const void* logits, int64_t logits_row, const void* teacher,
+                         const int64_t* index, float temperature, float* loss, float* stats, float* mean,
+                         int64_t rows, int64_t vocabulary, int64_t entries, void* stream) {
+  const char* fn = "bssm_distill_forward";
+  bssm::DistillArgs a{};
+  a.logits = logits; a.logits_row = logits_row; a.teacher = teacher; a.index = index; a.tau = temperature;
+  a.loss = loss; a.lse = stats; a.mean = mean; a.r = rows; a.v = vocabulary; a.k = entries;
+  a.bf16 = bf16 != 0; a.teacher_bf16 = teacher_bf16 != 0;
+  if (int rc = distill_check(fn, a)) return rc;
+  if (rows > 0) {
+    if (int rc = need(fn, {{logits, "logits"}, {loss, "loss"}, {stats, "stats"}})) return rc;
+    if (entries > 0)
+      if (int rc = need(fn, {{teacher, "teacher"}, {index, "index"}})) return rc;
+  }
+  return launched(fn, bssm::launch_distill_forward(a, static_cast<hipStream_t>(stream)));
+}
+
+int bssm_distill_backward(int bf16, int teacher_bf16, const void* logits, int64_t logits_row, const void* teacher,
+                          const int64_t* index, float temperature, const float* stats, const float* mean,
+                          const float* upstream, int upstream_scalar, void* grad_logits, int64_t rows,
+                          int64_t vocabulary, int64_t entries, void* stream) {
+  const char* fn = "bssm_distill_backward";
+  bssm::DistillArgs a{};
+  a.logits = logits; a.logits_row = logits_row; a.teacher = teacher; a.index = index; a.tau = temperature;
+  a.lse = const_cast<float*>(stats); a.mean = const_cast<float*>(mean); a.upstream = upstream;
+  a.upstream_scalar = upstream_scalar != 0; a.grad = grad_logits; a.r = rows; a.v = vocabulary; a.k = entries;
+  a.bf16 = bf16 != 0; a.teacher_bf16 = teacher_bf16 != 0;
+  if (int rc = distill_check(fn, a)) return rc;
+  if (rows == 0) return ok();
+  if (int rc = need(fn, {{logits, "logits"}, {stats, "stats"}, {upstream, "upstream"}, {grad_logits, "grad_logits"}}))
+    return rc;
+  if (entries > 0)
+    if (int rc = need(fn, {{teacher, "teacher"}, {index, "index"}})) return rc;
+  return launched(fn, bssm::launch_distill_backward(a, static_cast<hipStream_t>(stream)));
+}
+
+int64_t bssm_select_sizes(int what, int bf16, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t states,
+                          int64_t groups) {
+  bssm::SelectArgs a{};
+  a.b = batch; a.t = t; a.h = heads; a.p = values; a.n = states; a.g = groups < 1 ? 1 : groups; a.bf16 = bf16 != 0;
+  const int64_t record = bssm::select_record(a.bf16);
+  switch (what) {
+    case 0: return (t + record - 1) / record;
+    case 1: return bssm::select_segment_floats(a);
+    case 2: return bssm::select_parts(a);
+    default: return 0;
+  }
+}
+
+int bssm_select_forward(int bf16, const void* x, int64_t x_batch, int64_t x_row, int64_t x_head, int dt_bf16,
+                        const void* dt, int64_t dt_batch, int64_t dt_row, const float* rate, const void* bk,
+                        int64_t bk_batch, int64_t bk_row, int64_t bk_group, const void* cq, int64_t cq_batch,
+                        int64_t cq_row, int64_t cq_group, const float* skip, const float* dt_bias, int softplus,
+                        const int64_t* lengths, const float* state0, void* y, float* state_out, float* states,
+                        float* segments, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t n,
+                        int64_t groups, void* stream) {
+  const char* fn = "bssm_select_forward";
+  bssm::SelectArgs a = select_args(bf16, x, x_batch, x_row, x_head, dt_bf16, dt, dt_batch, dt_row, rate, bk, bk_batch,
+                                   bk_row, bk_group, cq, cq_batch, cq_row, cq_group, skip, dt_bias, softplus, lengths,
+                                   batch, t, heads, values, n, groups);
+  a.state0 = state0; a.y = y; a.state_out = state_out; a.states = states; a.segments = segments;
+  if (int rc = select_check(fn, batch, t, heads, values, n, groups)) return rc;
+  if (batch == 0) return ok();
+  if (int rc = need(fn, {{rate, "rate"}})) return rc;
+  if (t > 0)
+    if (int rc = need(fn, {{x, "x"}, {dt, "dt"}, {bk, "b"}, {cq, "c"}, {y, "y"}})) return rc;
+  if (bssm::select_segment_floats(a) > 0 && segments == nullptr)
+    return fail(BSSM_ERR_ARGUMENT, "%s: needs a workspace of %lld floats", fn, (long long)bssm::select_segment_floats(a));
+  return launched(fn, bssm::launch_select_forward(a, static_cast<hipStream_t>(stream)));
+}
+
+int bssm_select_backward(int bf16, const void* x, int64_t x_batch, int64_t x_row, int64_t x_head, int dt_bf16,
+                         const void* dt, int64_t dt_batch, int64_t dt_row, const float* rate, const void* bk,
+                         int64_t bk_batch, int64_t bk_row, int64_t bk_group, const void* cq, int64_t cq_batch,
+                         int64_t cq_row, int64_t cq_group, const float* skip, const float* dt_bias, int softplus,
+                         const int64_t* lengths, const float* states, const void* grad_y, const float* grad_state_out,
+                         float* adjoints, float* segments, float* parts, float* rows, void* grad_x, void* grad_dt,
+                         float* grad_rate, void* grad_b, void* grad_c, float* grad_skip, float* grad_dt_bias,
+                         float* grad_state0, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t n,
+                         int64_t groups, void* stream) {
+  const char* fn = "bssm_select_backward";
+  bssm::SelectArgs a = select_args(bf16, x, x_batch, x_row, x_head, dt_bf16, dt, dt_batch, dt_row, rate, bk, bk_batch,
+                                   bk_row, bk_group, cq, cq_batch, cq_row, cq_group, skip, dt_bias, softplus, lengths,
+                                   batch, t, heads, values, n, groups);
+  a.states = const_cast<float*>(states); a.gy = grad_y; a.gstate_out = grad_state_out; a.adjoints = adjoints;
+  a.segments = segments; a.gparts = parts; a.rows = rows; a.gx = grad_x; a.gdt = grad_dt; a.gbk = grad_b;
+  a.gcq = grad_c; a.grate = grad_rate; a.gskip = grad_skip; a.gdt_bias = grad_dt_bias; a.gstate0 = grad_state0;
+  if (int rc = select_check(fn, batch, t, heads, values, n, groups)) return rc;
+  if (batch > 0 && t > 0) {
+    if (int rc = need(fn, {{rate, "rate"}, {x, "x"}, {dt, "dt"}, {bk, "b"}, {cq, "c"}, {states, "states"},
+                           {grad_y, "grad_y"}, {adjoints, "adjoints"}, {rows, "rows"}, {grad_x, "grad_x"},
+                           {grad_dt, "grad_dt"}, {grad_b, "grad_b"}, {grad_c, "grad_c"}}))
+      return rc;
+    if (bssm::select_segment_floats(a) > 0 && segments == nullptr)
+      return fail(BSSM_ERR_ARGUMENT, "%s: needs a workspace of %lld floats", fn, (long long)bssm::select_segment_floats(a));
+    if (bssm::select_parts(a) > 1 && parts == nullptr)
+      return fail(BSSM_ERR_ARGUMENT, "%s: needs %lld parts of the gradients of b and c", fn, (long long)bssm::select_parts(a));
+  }
+  return launched(fn, bssm::launch_select_backward(a, static_cast<hipStream_t>(stream)));
+}
+
+int bssm_select_step(int bf16, int param_bf16, int width, int silu, const void* row, int64_t row_batch, int dt_bf16,
+                     const void* dt, int64_t dt_batch, const void* conv_state, const float* state, const void* weight,
+                     const void* conv_bias, const float* rate, const float* skip, const float* dt_bias, int softplus,
+                     void* y, void* conv_state_out, float* state_out, int64_t batch, int64_t heads, int64_t values,
+                     int64_t n, int64_t groups, void* stream) {
+  const char* fn = "bssm_select_step";
+  if (width < 2 || width > 4) return fail(BSSM_ERR_UNSUPPORTED, "%s: width must be 2, 3 or 4, got %d", fn, width);
+  if (int rc = select_check(fn, batch, 1, heads, values, n, groups)) return rc;
+  if (batch == 0) return ok();
+  if (int rc = need(fn, {{row, "row"}, {dt, "dt"}, {conv_state, "conv_state"}, {state, "state"}, {weight, "weight"},
+                         {rate, "rate"}, {y, "y"}, {conv_state_out, "conv_state_out"}, {state_out, "state_out"}}))
+    return rc;
+  if (conv_state_out == conv_state) return fail(BSSM_ERR_ARGUMENT, "%s: conv_state_out must not be conv_state", fn);
+  bssm::SelectStepArgs a{};
+  a.row = row; a.row_batch = row_batch; a.dt = dt; a.dt_batch = dt_batch; a.conv_state = conv_state; a.state = state;
+  a.weight = weight; a.conv_bias = conv_bias; a.rate = rate; a.skip = skip; a.dt_bias = dt_bias; a.y = y;
+  a.conv_state_out = conv_state_out; a.state_out = state_out;
+  a.b = batch; a.h = heads; a.p = values; a.n = n; a.g = groups; a.w = width; a.bf16 = bf16 != 0;
+  a.dt_bf16 = dt_bf16 != 0; a.param_bf16 = param_bf16 != 0; a.silu = silu != 0; a.softplus = softplus != 0;
+  return launched(fn, bssm::launch_select_step(a, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -1,0 +1,104 @@
+// Device helpers of the row and column kernels (short filter, layer norm,
+// distillation loss, selective scan): elements of either stream type as
+// float32, short vectors of them, sums over lanes, and the column sums of
+// partial results in a fixed order.
+#ifndef BSSM_LANE_H_
+#define BSSM_LANE_H_
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace bssm {
+namespace lane {
+
+constexpr int kWave = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ float widen(__bf16 x) { return static_cast<float>(x); }
+template <typename T>
+__device__ __forceinline__ T narrow(float x) {
+  return static_cast<T>(x);  // to nearest even
+}
+
+// N elements moved by one access (N * sizeof(T) bytes, aligned to that).
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+  T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
+  return *reinterpret_cast<const Pack<T, N>*>(p);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& x) {
+  *reinterpret_cast<Pack<T, N>*>(p) = x;
+}
+
+// A parameter (weight, bias) of either type.
+__device__ __forceinline__ float param(const void* p, int64_t i, int bf16) {
+  return bf16 ? widen(static_cast<const __bf16*>(p)[i]) : static_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void put_param(void* p, int64_t i, float x, int bf16) {
+  if (bf16) static_cast<__bf16*>(p)[i] = narrow<__bf16>(x);
+  else static_cast<float*>(p)[i] = x;
+}
+
+// 2^x and 1/x by the hardware's instructions (1 ulp each).
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float exp_(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+__device__ __forceinline__ float rcp_(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ __forceinline__ float sigmoid_(float x) { return rcp_(1.f + exp_(-x)); }
+// log(1 + e^x) without overflow and without loss for very negative x, and its
+// derivative.  Few values a call: the library's exponential, since exp_ loses
+// |x| 2^-24 of the value.
+__device__ __forceinline__ float softplus_(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
+__device__ __forceinline__ float softplus_slope_(float x) { return 1.f / (1.f + expf(-x)); }
+
+template <int WIDTH = kWave>
+__device__ __forceinline__ float lanes_sum(float x) {
+#pragma unroll
+  for (int o = WIDTH / 2; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
+  return x;
+}
+template <int WIDTH = kWave>
+__device__ __forceinline__ float lanes_max(float x) {
+#pragma unroll
+  for (int o = WIDTH / 2; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, kWave));
+  return x;
+}
+
+// Column sums of partials [rows, cols] (float32): a block of 256 threads takes
+// 32 columns, its 8 row groups every 8th row with four loads in flight, and
+// they meet in LDS in a fixed order.  put(column, sum).
+constexpr int kFoldColumns = 32;
+template <typename Put>
+__device__ __forceinline__ void fold_columns(const float* __restrict__ part, int64_t rows, int64_t cols, int64_t block,
+                                             Put put) {
+  constexpr int kGroups = 256 / kFoldColumns;
+  __shared__ float red[256];
+  const int cl = threadIdx.x % kFoldColumns, g = threadIdx.x / kFoldColumns;
+  const int64_t c = block * kFoldColumns + cl;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < cols) {
+    int64_t r = g;
+    for (; r + 3 * kGroups < rows; r += 4 * kGroups)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += part[(r + i * kGroups) * cols + c];
+    for (; r < rows; r += kGroups) s[0] += part[r * cols + c];
+  }
+  red[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (g == 0 && c < cols) {
+    float sum = red[cl];
+#pragma unroll
+    for (int k = 1; k < kGroups; ++k) sum += red[k * kFoldColumns + cl];
+    put(c, sum);
+  }
+}
+
+}  // namespace lane
+}  // namespace bssm
+
+#endif  // BSSM_LANE_H_

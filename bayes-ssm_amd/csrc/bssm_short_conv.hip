@@ -1,0 +1,320 @@
+// Short causal filter of W = 2, 3 or 4 taps over rows of channels, with bias,
+// SiLU, carried inputs and rows of unequal length, gfx950.
+//
+//   pre[t, c] = bias[c] + sum_j w[c, j] x[t - W + 1 + j, c],   y = pre or pre * sigmoid(pre)
+// where x before token 0 are the W - 1 carried rows (zeros without them).  A
+// row of length n gives y = 0 from token n on, and the carried rows that it
+// leaves are the last W - 1 inputs before token n.
+// Reverse, with g[t] = gy[t] act'(pre[t]) (0 from token n on):
+//   gx[s] = sum_j w[c, j] g[s + W - 1 - j],  gw[c, j] = sum g[t] x[t - W + 1 + j],  gbias = sum g.
+// The reverse computes pre again from x: that costs W multiply-adds, where
+// keeping it would cost a write and a read of the whole stream.
+//
+// Bound by memory: one read and one write a stream.  A thread owns a 16-byte
+// group of channels (one channel where C, the strides or an address do not
+// allow that) and walks a segment of tokens with the last W - 1 rows in
+// registers, so only the W - 1 rows in front of a segment (and, in the
+// reverse, behind it) are read twice.
+#include "bssm_lane.h"
+#include "bssm_sequence.h"
+
+namespace bssm {
+namespace short_conv {
+namespace {
+
+using lane::Pack;
+using lane::kWave;
+
+constexpr int kWaves = 4;
+
+__device__ __forceinline__ int64_t row_length(const ShortConvArgs& a, int64_t b) {
+  if (a.lengths == nullptr) return a.t;
+  const int64_t n = a.lengths[b];
+  return n < 0 ? 0 : n > a.t ? a.t : n;
+}
+
+// Channels [c0, c0 + N) of input row t (t may lie before the sequence).
+template <typename T, int N, int W>
+__device__ __forceinline__ void input_row(const ShortConvArgs& a, int64_t b, int64_t t, int64_t c0, float (&x)[N]) {
+  const T* p = nullptr;
+  if (t >= 0) p = static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_row + c0;
+  else if (a.state != nullptr) p = static_cast<const T*>(a.state) + (b * (W - 1) + t + W - 1) * a.c + c0;
+  if (p == nullptr) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = 0.f;
+    return;
+  }
+  const Pack<T, N> r = lane::load_pack<T, N>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = lane::widen(r.v[i]);
+}
+
+template <int N, int W>
+struct Taps {
+  float w[N][W], bias[N];
+  __device__ __forceinline__ Taps(const ShortConvArgs& a, int64_t c0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) w[i][j] = lane::param(a.weight, (c0 + i) * W + j, a.param_bf16);
+      bias[i] = a.bias == nullptr ? 0.f : lane::param(a.bias, c0 + i, a.param_bf16);
+    }
+  }
+};
+
+template <typename T, int N, int W>
+__global__ __launch_bounds__(256) void forward_kernel(ShortConvArgs a, int seg) {
+  constexpr int kAhead = 4;  // rows loaded before their sums
+  const int64_t groups = a.c / N, segs = a.t > 0 ? (a.t + seg - 1) / seg : 1;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (id >= a.b * segs * groups) return;
+  const int64_t c0 = id % groups * N, s = id / groups % segs, b = id / groups / segs;
+  const int64_t n = row_length(a, b), t0 = s * seg, t1 = t0 + seg < a.t ? t0 + seg : a.t;
+  const Taps<N, W> k(a, c0);
+  float h[W][N];  // h[j] = x[t - W + 1 + j]
+#pragma unroll
+  for (int j = 1; j < W; ++j) input_row<T, N, W>(a, b, t0 - W + j, c0, h[j]);
+  T* y = static_cast<T*>(a.y) + b * a.t * a.c + c0;
+  const T* x = static_cast<const T*>(a.x) + b * a.x_batch + c0;
+  for (int64_t t = t0; t < t1; t += kAhead) {
+    Pack<T, N> raw[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (t + u < t1) raw[u] = lane::load_pack<T, N>(x + (t + u) * a.x_row);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (t + u >= t1) break;
+      Pack<T, N> out;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int j = 0; j + 1 < W; ++j) h[j][i] = h[j + 1][i];
+        h[W - 1][i] = lane::widen(raw[u].v[i]);
+        float p = k.bias[i];
+#pragma unroll
+        for (int j = 0; j < W; ++j) p = fmaf(k.w[i][j], h[j][i], p);
+        if (a.silu) p *= lane::sigmoid_(p);
+        out.v[i] = lane::narrow<T>(t + u < n ? p : 0.f);
+      }
+      lane::store_pack<T, N>(y + (t + u) * a.c, out);
+    }
+  }
+  if (s == 0 && a.final_state != nullptr) {
+    T* f = static_cast<T*>(a.final_state) + b * (W - 1) * a.c + c0;
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+      float r[N];
+      input_row<T, N, W>(a, b, n - W + 1 + j, c0, r);
+      Pack<T, N> out;
+#pragma unroll
+      for (int i = 0; i < N; ++i) out.v[i] = lane::narrow<T>(r[i]);
+      lane::store_pack<T, N>(f + j * a.c, out);
+    }
+  }
+}
+
+// Block: 64 channel groups x 4 waves, each wave its own segment of tokens;
+// the waves' weight and bias sums meet in LDS, one row of partials a block.
+template <typename T, int N, int W>
+__global__ __launch_bounds__(kWave * kWaves) void backward_kernel(ShortConvArgs a, int seg, int64_t blocks_t) {
+  constexpr int kAhead = 4;
+  __shared__ float red[kWaves - 1][W + 1][N][kWave];
+  const int wave = threadIdx.x / kWave, ln = threadIdx.x % kWave;
+  const int64_t groups = a.c / N, cblocks = (groups + kWave - 1) / kWave;
+  const int64_t g = blockIdx.x % cblocks * kWave + ln, part = blockIdx.x / cblocks;
+  const int64_t b = part / blocks_t, t0 = (part % blocks_t * kWaves + wave) * seg;
+  const bool active = g < groups;
+  const int64_t c0 = (active ? g : 0) * N;
+  float gw[W + 1][N];
+#pragma unroll
+  for (int j = 0; j <= W; ++j)
+#pragma unroll
+    for (int i = 0; i < N; ++i) gw[j][i] = 0.f;
+  if (active && (t0 < a.t || (t0 == 0 && a.gstate != nullptr))) {
+    const int64_t n = row_length(a, b), t1 = t0 + seg < a.t ? t0 + seg : a.t;
+    const Taps<N, W> k(a, c0);
+    const T* x = static_cast<const T*>(a.x) + b * a.x_batch + c0;
+    const T* gy = static_cast<const T*>(a.gy) + b * a.t * a.c + c0;
+    float h[W][N], q[W][N];  // h[j] = x[t - W + 1 + j], q[j] = g[t - W + 1 + j]
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+#pragma unroll
+      for (int i = 0; i < N; ++i) q[j][i] = 0.f;
+#pragma unroll
+    for (int j = 1; j < W; ++j) {
+      if (t0 - W + j < n) input_row<T, N, W>(a, b, t0 - W + j, c0, h[j]);
+      else
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[j][i] = 0.f;
+    }
+    const int64_t end = t1 + W - 1;
+    for (int64_t t = t0; t < end; t += kAhead) {
+      Pack<T, N> rx[kAhead], rg[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (t + u < n && t + u < end) {
+          rx[u] = lane::load_pack<T, N>(x + (t + u) * a.x_row);
+          if (a.gy != nullptr) rg[u] = lane::load_pack<T, N>(gy + (t + u) * a.c);
+        }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int64_t tt = t + u;
+        if (tt >= end) break;
+        const bool live = tt < n, mine = tt < t1;
+        const int64_t s = tt - (W - 1);
+        Pack<T, N> out;
+        float gf[N];
+        const int64_t jf = s - n + W - 1;  // row of the final state that input s is
+        const bool from_final = a.gfinal != nullptr && jf >= 0 && jf < W - 1;
+        if (from_final) {
+          const Pack<T, N> r = lane::load_pack<T, N>(static_cast<const T*>(a.gfinal) + (b * (W - 1) + jf) * a.c + c0);
+#pragma unroll
+          for (int i = 0; i < N; ++i) gf[i] = lane::widen(r.v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+#pragma unroll
+          for (int j = 0; j + 1 < W; ++j) {
+            h[j][i] = h[j + 1][i];
+            q[j][i] = q[j + 1][i];
+          }
+          h[W - 1][i] = live ? lane::widen(rx[u].v[i]) : 0.f;
+          float gi = live && a.gy != nullptr ? lane::widen(rg[u].v[i]) : 0.f;
+          if (a.silu) {
+            float p = k.bias[i];
+#pragma unroll
+            for (int j = 0; j < W; ++j) p = fmaf(k.w[i][j], h[j][i], p);
+            const float sg = lane::sigmoid_(p);
+            gi *= sg * fmaf(p, 1.f - sg, 1.f);
+            if (!live) gi = 0.f;
+          }
+          q[W - 1][i] = gi;
+          if (mine) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) gw[j][i] = fmaf(gi, h[j][i], gw[j][i]);
+            gw[W][i] += gi;
+          }
+          float o = from_final ? gf[i] : 0.f;
+#pragma unroll
+          for (int j = 0; j < W; ++j) o = fmaf(k.w[i][j], q[W - 1 - j][i], o);
+          out.v[i] = lane::narrow<T>(o);
+        }
+        if (s >= t0) lane::store_pack<T, N>(static_cast<T*>(a.gx) + (b * a.t + s) * a.c + c0, out);
+        else if (t0 == 0 && a.gstate != nullptr)
+          lane::store_pack<T, N>(static_cast<T*>(a.gstate) + (b * (W - 1) + s + W - 1) * a.c + c0, out);
+      }
+    }
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int j = 0; j <= W; ++j)
+#pragma unroll
+      for (int i = 0; i < N; ++i) red[wave - 1][j][i][ln] = gw[j][i];
+  }
+  __syncthreads();
+  if (wave == 0 && active && a.partials != nullptr) {
+#pragma unroll
+    for (int j = 0; j <= W; ++j)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float sum = gw[j][i];
+#pragma unroll
+        for (int w = 0; w < kWaves - 1; ++w) sum += red[w][j][i][ln];
+        a.partials[(part * (W + 1) + j) * a.c + c0 + i] = sum;
+      }
+  }
+}
+
+__global__ __launch_bounds__(256) void fold_kernel(ShortConvArgs a, int64_t rows) {
+  lane::fold_columns(a.partials, rows, a.c * (a.w + 1), blockIdx.x, [&](int64_t col, float sum) {
+    const int64_t j = col / a.c, c = col % a.c;
+    if (j < a.w) {
+      if (a.gweight != nullptr) lane::put_param(a.gweight, c * a.w + j, sum, a.param_bf16);
+    } else if (a.gbias != nullptr) {
+      lane::put_param(a.gbias, c, sum, a.param_bf16);
+    }
+  });
+}
+
+// Tokens a thread walks: the rows around a segment are read twice, so long
+// segments save reads, but a call needs some thousand waves to keep the
+// memory busy.
+int forward_segment(int64_t b, int64_t t, int64_t groups) {
+  int seg = 32;
+  while (seg > 4 && b * ((t + seg - 1) / seg) * groups < (int64_t)1 << 18) seg /= 2;
+  return seg;
+}
+int backward_segment(int64_t b, int64_t t, int64_t groups) {
+  int seg = 64;
+  while (seg > 8 && b * ((t + seg - 1) / seg) * groups < (int64_t)1 << 17) seg /= 2;
+  return seg;
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// 16-byte groups need every row of every stream on a 16-byte boundary.
+bool vectors(const ShortConvArgs& a) {
+  const int n = a.bf16 ? 8 : 4;
+  return a.c % n == 0 && a.x_row % n == 0 && a.x_batch % n == 0 && aligned(a.x) && aligned(a.state) && aligned(a.y) &&
+         aligned(a.final_state) && aligned(a.gy) && aligned(a.gfinal) && aligned(a.gx) && aligned(a.gstate);
+}
+
+template <typename T, int N, int W>
+hipError_t forward(const ShortConvArgs& a, hipStream_t stream) {
+  const int64_t groups = a.c / N;
+  const int seg = forward_segment(a.b, a.t, groups);
+  // With no tokens the carried rows still pass through.
+  const int64_t segs = a.t == 0 ? 1 : (a.t + seg - 1) / seg;
+  const int64_t blocks = (a.b * segs * groups + 255) / 256;
+  hipLaunchKernelGGL((forward_kernel<T, N, W>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a, seg);
+  return hipGetLastError();
+}
+template <typename T, int N, int W>
+hipError_t backward(const ShortConvArgs& a, hipStream_t stream) {
+  const int64_t groups = a.c / N, cblocks = (groups + kWave - 1) / kWave;
+  // The segment follows from the sizes alone, so that the partial rows do.
+  const int seg = backward_segment(a.b, a.t, a.c / (a.bf16 ? 8 : 4) + 1);
+  const int64_t blocks_t = (a.t + kWaves * seg - 1) / (kWaves * seg), bt = blocks_t > 0 ? blocks_t : 1;
+  hipLaunchKernelGGL((backward_kernel<T, N, W>), dim3(static_cast<unsigned>(a.b * bt * cblocks)), dim3(kWave * kWaves),
+                     0, stream, a, seg, bt);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  if (a.gweight == nullptr && a.gbias == nullptr) return hipSuccess;
+  const int64_t cols = a.c * (a.w + 1);
+  hipLaunchKernelGGL(fold_kernel, dim3(static_cast<unsigned>((cols + lane::kFoldColumns - 1) / lane::kFoldColumns)),
+                     dim3(256), 0, stream, a, a.b * bt);
+  return hipGetLastError();
+}
+
+template <typename T, int N>
+hipError_t taps(const ShortConvArgs& a, bool back, hipStream_t stream) {
+  switch (a.w) {
+    case 2: return back ? backward<T, N, 2>(a, stream) : forward<T, N, 2>(a, stream);
+    case 3: return back ? backward<T, N, 3>(a, stream) : forward<T, N, 3>(a, stream);
+    default: return back ? backward<T, N, 4>(a, stream) : forward<T, N, 4>(a, stream);
+  }
+}
+hipError_t types(const ShortConvArgs& a, bool back, hipStream_t stream) {
+  if (vectors(a)) return a.bf16 ? taps<__bf16, 8>(a, back, stream) : taps<float, 4>(a, back, stream);
+  return a.bf16 ? taps<__bf16, 1>(a, back, stream) : taps<float, 1>(a, back, stream);
+}
+
+}  // namespace
+}  // namespace short_conv
+
+int64_t short_conv_partial_rows(int64_t b, int64_t t, int64_t c, int bf16) {
+  const int seg = short_conv::backward_segment(b, t, c / (bf16 ? 8 : 4) + 1);
+  const int64_t n = (t + short_conv::kWaves * seg - 1) / (short_conv::kWaves * seg);
+  return b * (n > 0 ? n : 1);
+}
+
+hipError_t launch_short_conv_forward(const ShortConvArgs& a, hipStream_t stream) {
+  if (a.b * a.c == 0) return hipSuccess;
+  return short_conv::types(a, false, stream);
+}
+
+hipError_t launch_short_conv_backward(const ShortConvArgs& a, hipStream_t stream) {
+  if (a.b * a.c == 0) return hipSuccess;
+  return short_conv::types(a, true, stream);
+}
+
+}  // namespace bssm

@@ -659,6 +659,127 @@ int bssm_mixer_block_backward(const void* projected, int64_t ld_projected, const
                               int64_t batch, int64_t t, int64_t heads, int64_t chunk,
                               float denominator_floor, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Operators around a selective state space block (no reference counterpart).
+ * `bf16` and its kin give a stream's type: 0 float32, else bfloat16; strides
+ * and sizes count elements and the innermost axis is contiguous; `lengths`
+ * (NULL: all rows full) holds int64 row lengths in device memory, which the
+ * kernels clamp to [0, t].  Streams whose rows do not start on 16-byte
+ * boundaries are valid and run narrower accesses.
+ *
+ * Short causal filter of `width` (2..4) taps with bias and SiLU:
+ *   pre[b,s,c] = bias[c] + sum_j weight[c,j] x[b, s - width + 1 + j, c],
+ *   y = silu ? pre sigmoid(pre) : pre
+ * x [batch, t, channels] (row and batch stride given); weight [channels,
+ * width] and bias [channels] or NULL, of the type `param_bf16` gives.  Inputs
+ * before token 0 are state [batch, width-1, channels] (NULL: zeros), oldest
+ * first.  Tokens from a row's length on give y = 0; final_state (NULL: not
+ * wanted) receives the last width-1 inputs before it. */
+int bssm_short_conv_forward(int bf16, int param_bf16, int width, int silu, const void* x, int64_t x_batch,
+                            int64_t x_row, const void* weight, const void* bias, const void* state,
+                            const int64_t* lengths, void* y, void* final_state, int64_t batch, int64_t t,
+                            int64_t channels, void* stream);
+
+/* Gradients of the above.  grad_y and grad_final_state may be NULL (zero);
+ * grad_state may be NULL.  grad_weight and grad_bias (parameter type, either
+ * may be NULL) are summed in a fixed order from the workspace partials
+ * [bssm_short_conv_partial_rows(...), width + 1, channels] (float32). */
+int bssm_short_conv_backward(int bf16, int param_bf16, int width, int silu, const void* x, int64_t x_batch,
+                             int64_t x_row, const void* weight, const void* bias, const void* state,
+                             const int64_t* lengths, const void* grad_y, const void* grad_final_state, void* grad_x,
+                             void* grad_state, float* partials, void* grad_weight, void* grad_bias, int64_t batch,
+                             int64_t t, int64_t channels, void* stream);
+int64_t bssm_short_conv_partial_rows(int bf16, int64_t batch, int64_t t, int64_t channels);
+
+/* Layer norm of rows [rows, width] (row stride x_row): y = (x - mean) rstd
+ * weight + bias, rstd = 1 / sqrt(variance + eps); weight and bias [width] may
+ * be NULL.  mean and rstd [rows] (float32) are kept for the backward; both
+ * NULL where there is none. */
+int bssm_layer_norm_forward(int bf16, int param_bf16, const void* x, int64_t x_row, const void* weight,
+                            const void* bias, float eps, void* y, float* mean, float* rstd, int64_t rows,
+                            int64_t width, void* stream);
+
+/* Gradients: grad_x (may be NULL), grad_weight and grad_bias (parameter type,
+ * either may be NULL; zeros for rows = 0), these two summed in a fixed order
+ * from partials [bssm_layer_norm_partial_rows(...), 2, width] (float32). */
+int bssm_layer_norm_backward(int bf16, int param_bf16, const void* x, int64_t x_row, const void* weight,
+                             const float* mean, const float* rstd, const void* grad_y, void* grad_x, float* partials,
+                             void* grad_weight, void* grad_bias, int64_t rows, int64_t width, void* stream);
+int64_t bssm_layer_norm_partial_rows(int bf16, int64_t rows, int64_t width);
+
+/* Distillation loss of logits [rows, vocabulary] (row stride logits_row) from
+ * a teacher's listed logits [rows, entries] at index [rows, entries] (int64):
+ *   loss = temperature^2 sum_k p_k (log p_k - log q[index_k]),
+ * p = softmax(teacher / temperature) over the entries with 0 <= index <
+ * vocabulary and a logit above -infinity, q = softmax(logits / temperature).
+ * A row without such entries has loss 0 and gradient 0.  At most 1024
+ * entries.  stats [rows, 3] is kept for the backward; mean (NULL: not wanted)
+ * receives (mean over the rows with entries, 1 / their number, sum). */
+int bssm_distill_forward(int bf16, int teacher_bf16, const void* logits, int64_t logits_row, const void* teacher,
+                         const int64_t* index, float temperature, float* loss, float* stats, float* mean,
+                         int64_t rows, int64_t vocabulary, int64_t entries, void* stream);
+
+/* grad_logits [rows, vocabulary] = upstream * temperature * (q - p), upstream
+ * one value (upstream_scalar) or one a row, float32 in device memory; with
+ * `mean` from the forward also divided by the number of rows with entries. */
+int bssm_distill_backward(int bf16, int teacher_bf16, const void* logits, int64_t logits_row, const void* teacher,
+                          const int64_t* index, float temperature, const float* stats, const float* mean,
+                          const float* upstream, int upstream_scalar, void* grad_logits, int64_t rows,
+                          int64_t vocabulary, int64_t entries, void* stream);
+
+/* Selective state space scan.  Per sequence, head (its group's b and c: heads
+ * / groups heads share them) and token, with step = softplus(dt + dt_bias)
+ * (softplus = 0: dt + dt_bias):
+ *   h = exp(step rate) h + step x b^T,    y = h c + skip x
+ * x [batch, t, heads, values], dt [batch, t, heads], b and c [batch, t,
+ * groups, n] (n <= 128), rate (negative), skip and dt_bias [heads] float32 (the last two
+ * may be NULL), state0 [batch, heads, values, n] float32 or NULL (zeros).
+ * Tokens from a row's length on give y = 0 and leave the state.  state_out
+ * (NULL: not wanted) receives the last state.  For a backward, states [batch,
+ * heads, bssm_select_sizes(0, ...), values, n] keeps states along the way
+ * (NULL: none).  segments: workspace of bssm_select_sizes(1, ...) floats (may
+ * be NULL for 0). */
+int bssm_select_forward(int bf16, const void* x, int64_t x_batch, int64_t x_row, int64_t x_head, int dt_bf16,
+                        const void* dt, int64_t dt_batch, int64_t dt_row, const float* rate, const void* b,
+                        int64_t b_batch, int64_t b_row, int64_t b_group, const void* c, int64_t c_batch,
+                        int64_t c_row, int64_t c_group, const float* skip, const float* dt_bias, int softplus,
+                        const int64_t* lengths, const float* state0, void* y, float* state_out, float* states,
+                        float* segments, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t n,
+                        int64_t groups, void* stream);
+
+/* Gradients of the above, contiguous, of the inputs' types.  grad_y
+ * [batch, t, heads, values] contiguous; grad_state_out may be NULL (zero).
+ * Workspaces (float32): adjoints of the size of states; segments as in the
+ * forward; parts [bssm_select_sizes(2, ...), 2, batch, t, groups, n] (may be
+ * NULL where that is 1); rows [batch * bssm_select_sizes(0, ...), 3, heads].
+ * grad_rate, grad_skip, grad_dt_bias [heads] and grad_state0 may be NULL. */
+int bssm_select_backward(int bf16, const void* x, int64_t x_batch, int64_t x_row, int64_t x_head, int dt_bf16,
+                         const void* dt, int64_t dt_batch, int64_t dt_row, const float* rate, const void* b,
+                         int64_t b_batch, int64_t b_row, int64_t b_group, const void* c, int64_t c_batch,
+                         int64_t c_row, int64_t c_group, const float* skip, const float* dt_bias, int softplus,
+                         const int64_t* lengths, const float* states, const void* grad_y, const float* grad_state_out,
+                         float* adjoints, float* segments, float* parts, float* rows, void* grad_x, void* grad_dt,
+                         float* grad_rate, void* grad_b, void* grad_c, float* grad_skip, float* grad_dt_bias,
+                         float* grad_state0, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t n,
+                         int64_t groups, void* stream);
+
+/* Sizes of the scan's buffers: what = 0 kept states a sequence and head, 1
+ * floats of the segments' workspace, 2 parts of the gradients of b and c. */
+int64_t bssm_select_sizes(int what, int bf16, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t n,
+                          int64_t groups);
+
+/* One token through the short filter and the scan.  row [batch, heads *
+ * values + 2 groups n] (batch stride row_batch): the filter's new inputs, the
+ * heads' values, then every group's b, then every group's c; conv_state
+ * [batch, width-1, the same columns] and state [batch, heads, values, n]
+ * (float32) are the carried ones.  state_out may be state; conv_state_out may
+ * not overlap conv_state. */
+int bssm_select_step(int bf16, int param_bf16, int width, int silu, const void* row, int64_t row_batch, int dt_bf16,
+                     const void* dt, int64_t dt_batch, const void* conv_state, const float* state, const void* weight,
+                     const void* conv_bias, const float* rate, const float* skip, const float* dt_bias, int softplus,
+                     void* y, void* conv_state_out, float* state_out, int64_t batch, int64_t heads, int64_t values,
+                     int64_t n, int64_t groups, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
