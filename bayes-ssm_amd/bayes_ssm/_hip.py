@@ -84,8 +84,8 @@ _SIGNATURES = {
     "bssm_layer_norm_partial_rows": [_I, _L, _L],
     "bssm_distill_forward": [_I, _I, _P, _L, _P, _P, _F] + [_P] * 3 + [_L] * 3 + [_P],
     "bssm_distill_backward": [_I, _I, _P, _L, _P, _P, _F] + [_P] * 3 + [_I, _P] + [_L] * 3 + [_P],
-    "bssm_select_forward": _SELECT_HEAD + [_P] * 5 + [_L] * 6 + [_P],
-    "bssm_select_backward": _SELECT_HEAD + [_P] * 15 + [_L] * 6 + [_P],
+    "bssm_select_forward": _SELECT_HEAD + [_P] * 6 + [_L] * 6 + [_P],
+    "bssm_select_backward": _SELECT_HEAD + [_P] * 17 + [_L] * 6 + [_P],
     "bssm_select_sizes": [_I, _I] + [_L] * 6,
     "bssm_select_step": [_I] * 4 + [_P, _L, _I, _P, _L] + [_P] * 7 + [_I] + [_P] * 3 + [_L] * 5 + [_P],
     "bssm_supported": [_I, _I],

@@ -58,8 +58,12 @@ def _scan_formula(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Opt
 
 
 def _strides(x: Tensor) -> list[int]:
-    """Strides of the leading axes (elements); 0 for an axis of one element, whose stride means nothing."""
-    return [s if n > 1 else 0 for s, n in zip(x.stride()[:-1], x.shape[:-1])]
+    """Strides of the leading axes (elements); an axis of one element, whose stride means nothing, as if contiguous."""
+    out, dense = [], x.shape[-1]
+    for s, n in zip(reversed(x.stride()[:-1]), reversed(x.shape[:-1])):
+        out.append(s if n > 1 else dense)
+        dense *= n
+    return out[::-1]
 
 
 def _inner(x: Tensor) -> Tensor:
@@ -91,18 +95,19 @@ class _ScanFunction(torch.autograd.Function):
         states = torch.empty(b, h, size(0), p, n, device=dev, dtype=torch.float32) if keep else None
         work = size(1)
         segments = torch.empty(work, device=dev, dtype=torch.float32) if work else None
+        steps = torch.empty(size(3), device=dev, dtype=torch.float32)
         P = _hip.ptr
         _hip.launch(dev, "bssm_select_forward", *_ScanFunction._head(x, dt, A, B, C, D, dt_bias, softplus, lengths),
-                    P(state), P(y), P(last), P(states), P(segments), b, t, h, p, n, g, _hip.stream_of(dev))
+                    P(state), P(y), P(last), P(states), P(steps), P(segments), b, t, h, p, n, g, _hip.stream_of(dev))
         if keep:
-            ctx.save_for_backward(x, dt, A, B, C, D, dt_bias, lengths, states)
+            ctx.save_for_backward(x, dt, A, B, C, D, dt_bias, lengths, states, steps)
             ctx.softplus = softplus
         ctx.set_materialize_grads(False)
         return y, last
 
     @staticmethod
     def backward(ctx, grad_y, grad_last):
-        x, dt, A, B, C, D, dt_bias, lengths, states = ctx.saved_tensors
+        x, dt, A, B, C, D, dt_bias, lengths, states, steps = ctx.saved_tensors
         b, t, h, p = x.shape
         g, n = B.shape[2:]
         dev = x.device
@@ -118,6 +123,7 @@ class _ScanFunction(torch.autograd.Function):
 
         adjoints = f32(b, h, records, p, n)
         segments = f32(work) if work else None
+        token_sums = f32(size(4))
         partial = f32(parts, 2, b, t, g, n) if parts > 1 else None
         rows = f32(max(1, b * records), 3, h)
         gx = torch.empty(b, t, h, p, device=dev, dtype=x.dtype)
@@ -129,8 +135,8 @@ class _ScanFunction(torch.autograd.Function):
             gstate = torch.zeros_like(gstate) if gl is None else gl.clone()
         P = _hip.ptr
         _hip.launch(dev, "bssm_select_backward",
-                    *_ScanFunction._head(x, dt, A, B, C, D, dt_bias, ctx.softplus, lengths), P(states), P(gy), P(gl),
-                    P(adjoints), P(segments), P(partial), P(rows), P(gx), P(gdt), P(gA), P(gB), P(gC), P(gD), P(gbias),
+                    *_ScanFunction._head(x, dt, A, B, C, D, dt_bias, ctx.softplus, lengths), P(states), P(steps), P(gy),
+                    P(gl), P(adjoints), P(segments), P(token_sums), P(partial), P(rows), P(gx), P(gdt), P(gA), P(gB), P(gC), P(gD), P(gbias),
                     P(gstate), b, t, h, p, n, g, _hip.stream_of(dev))
         grads = (gx, gdt, gA, gB, gC, gD, gbias, gstate)
         return (*(z if need[i] else None for i, z in enumerate(grads)), None, None)

@@ -1407,6 +1407,8 @@ int64_t bssm_select_sizes(int what, int bf16, int64_t batch, int64_t t, int64_t 
     case 0: return (t + record - 1) / record;
     case 1: return bssm::select_segment_floats(a);
     case 2: return bssm::select_parts(a);
+    case 3: return bssm::select_step_floats(a);
+    case 4: return bssm::select_token_floats(a);
     default: return 0;
   }
 }
@@ -1416,18 +1418,19 @@ int bssm_select_forward(int bf16, const void* x, int64_t x_batch, int64_t x_row,
                         int64_t bk_batch, int64_t bk_row, int64_t bk_group, const void* cq, int64_t cq_batch,
                         int64_t cq_row, int64_t cq_group, const float* skip, const float* dt_bias, int softplus,
                         const int64_t* lengths, const float* state0, void* y, float* state_out, float* states,
-                        float* segments, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t n,
-                        int64_t groups, void* stream) {
+                        float* steps, float* segments, int64_t batch, int64_t t, int64_t heads, int64_t values,
+                        int64_t n, int64_t groups, void* stream) {
   const char* fn = "bssm_select_forward";
   bssm::SelectArgs a = select_args(bf16, x, x_batch, x_row, x_head, dt_bf16, dt, dt_batch, dt_row, rate, bk, bk_batch,
                                    bk_row, bk_group, cq, cq_batch, cq_row, cq_group, skip, dt_bias, softplus, lengths,
                                    batch, t, heads, values, n, groups);
   a.state0 = state0; a.y = y; a.state_out = state_out; a.states = states; a.segments = segments;
+  a.steps = steps;
   if (int rc = select_check(fn, batch, t, heads, values, n, groups)) return rc;
   if (batch == 0) return ok();
   if (int rc = need(fn, {{rate, "rate"}})) return rc;
   if (t > 0)
-    if (int rc = need(fn, {{x, "x"}, {dt, "dt"}, {bk, "b"}, {cq, "c"}, {y, "y"}})) return rc;
+    if (int rc = need(fn, {{x, "x"}, {dt, "dt"}, {bk, "b"}, {cq, "c"}, {y, "y"}, {steps, "steps"}})) return rc;
   if (bssm::select_segment_floats(a) > 0 && segments == nullptr)
     return fail(BSSM_ERR_ARGUMENT, "%s: needs a workspace of %lld floats", fn, (long long)bssm::select_segment_floats(a));
   return launched(fn, bssm::launch_select_forward(a, static_cast<hipStream_t>(stream)));
@@ -1437,8 +1440,8 @@ int bssm_select_backward(int bf16, const void* x, int64_t x_batch, int64_t x_row
                          const void* dt, int64_t dt_batch, int64_t dt_row, const float* rate, const void* bk,
                          int64_t bk_batch, int64_t bk_row, int64_t bk_group, const void* cq, int64_t cq_batch,
                          int64_t cq_row, int64_t cq_group, const float* skip, const float* dt_bias, int softplus,
-                         const int64_t* lengths, const float* states, const void* grad_y, const float* grad_state_out,
-                         float* adjoints, float* segments, float* parts, float* rows, void* grad_x, void* grad_dt,
+                         const int64_t* lengths, const float* states, const float* steps, const void* grad_y,
+                         const float* grad_state_out, float* adjoints, float* segments, float* token_sums, float* parts, float* rows, void* grad_x, void* grad_dt,
                          float* grad_rate, void* grad_b, void* grad_c, float* grad_skip, float* grad_dt_bias,
                          float* grad_state0, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t n,
                          int64_t groups, void* stream) {
@@ -1447,12 +1450,12 @@ int bssm_select_backward(int bf16, const void* x, int64_t x_batch, int64_t x_row
                                    bk_row, bk_group, cq, cq_batch, cq_row, cq_group, skip, dt_bias, softplus, lengths,
                                    batch, t, heads, values, n, groups);
   a.states = const_cast<float*>(states); a.gy = grad_y; a.gstate_out = grad_state_out; a.adjoints = adjoints;
-  a.segments = segments; a.gparts = parts; a.rows = rows; a.gx = grad_x; a.gdt = grad_dt; a.gbk = grad_b;
+  a.steps = const_cast<float*>(steps); a.token_sums = token_sums; a.segments = segments; a.gparts = parts; a.rows = rows; a.gx = grad_x; a.gdt = grad_dt; a.gbk = grad_b;
   a.gcq = grad_c; a.grate = grad_rate; a.gskip = grad_skip; a.gdt_bias = grad_dt_bias; a.gstate0 = grad_state0;
   if (int rc = select_check(fn, batch, t, heads, values, n, groups)) return rc;
   if (batch > 0 && t > 0) {
     if (int rc = need(fn, {{rate, "rate"}, {x, "x"}, {dt, "dt"}, {bk, "b"}, {cq, "c"}, {states, "states"},
-                           {grad_y, "grad_y"}, {adjoints, "adjoints"}, {rows, "rows"}, {grad_x, "grad_x"},
+                           {steps, "steps"}, {token_sums, "token_sums"}, {grad_y, "grad_y"}, {adjoints, "adjoints"}, {rows, "rows"}, {grad_x, "grad_x"},
                            {grad_dt, "grad_dt"}, {grad_b, "grad_b"}, {grad_c, "grad_c"}}))
       return rc;
     if (bssm::select_segment_floats(a) > 0 && segments == nullptr)

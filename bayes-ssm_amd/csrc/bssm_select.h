@@ -1,16 +1,18 @@
 // Shared parts of the selective scan's kernels (bssm_select_fwd.hip,
-// bssm_select_bwd.hip): 16 x 16 tile products with 32 values of the summed
+// bssm_select_bwd.hip): 32 x 32 tile products with 16 values of the summed
 // index, on bfloat16 or float32 operands, and the tiles' ways into LDS.
 //
-// Operand layout.  A lane l of a wave holds row (column) l % 16 of an operand
-// and 8 values of the summed index k, group g = l / 16.  Two orders of k are
+// Operand layout.  A lane l of a wave holds row (column) l % 32 of an operand
+// and 8 values of the summed index k, half g = l / 32.  Two orders of k are
 // used, each for both operands of a product:
 //   plain:  element e is k = 8 g + e;
-//   folded: element e is k = 4 g + e for e < 4, else 16 + 4 g + e - 4.
-// A product's result has row 4 g + r (r = 0..3), column l % 16 in lane l, so
-// that two results below each other are an operand in the folded order, with
-// their rows as k, without any move between lanes.
-// bfloat16: one v_mfma_f32_16x16x32_bf16; float32: 8 v_mfma_f32_16x16x4_f32.
+//   folded: element e is k = 4 g + e for e < 4, else 8 + 4 g + e - 4.
+// A product's result has row 8 (r / 4) + 4 g + r % 4 (r = 0..15), column
+// l % 32 in lane l, so that its elements 0..7 and 8..15 are two operands in
+// the folded order, with its rows as k, without any move between lanes.
+// bfloat16: one v_mfma_f32_32x32x16_bf16; float32: 8 v_mfma_f32_32x32x2_f32.
+// 32 x 32 tiles take half the LDS reads of 16 x 16 ones for the same product,
+// and LDS reads are what the scan's kernels do most.
 #ifndef BSSM_SELECT_H_
 #define BSSM_SELECT_H_
 
@@ -21,12 +23,26 @@ namespace bssm {
 namespace select_scan {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef __bf16 v4b __attribute__((ext_vector_type(4)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 
 using lane::kWave;
 using lane::Pack;
+
+constexpr int kTile = 32;   // rows and columns of a product
+constexpr int kDepth = 16;  // its summed index
+constexpr int kTileP = 64;  // values of P that a workgroup holds
+
+// x again, as a value that the compiler has not seen: addresses that are made
+// of it are made anew where they are used, instead of being kept in registers
+// across a loop, and, when those run out, in memory (each column of a permuted
+// tile has its own address; the backward kept 300 of them).
+__device__ __forceinline__ int anew(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 template <typename T>
 struct Operand;
@@ -43,125 +59,205 @@ struct Operand<float> {
   __device__ __forceinline__ void set(int e, float x) { v[e] = x; }
 };
 
-__device__ __forceinline__ void mma(v4f& acc, const Operand<__bf16>& a, const Operand<__bf16>& b) {
-  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, acc, 0, 0, 0);
+__device__ __forceinline__ void mma(v16f& acc, const Operand<__bf16>& a, const Operand<__bf16>& b) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, acc, 0, 0, 0);
 }
-__device__ __forceinline__ void mma(v4f& acc, const Operand<float>& a, const Operand<float>& b) {
+__device__ __forceinline__ void mma(v16f& acc, const Operand<float>& a, const Operand<float>& b) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], acc, 0, 0, 0);
+  for (int e = 0; e < 8; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], acc, 0, 0, 0);
+}
+__device__ __forceinline__ v16f zeros() {
+  v16f z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+// Row of element r of a product's result in the half g.
+__device__ __forceinline__ constexpr int result_row(int r, int g) { return 8 * (r / 4) + 4 * g + r % 4; }
+
+// Computed float32 values as operands.  What feeds float32 results is kept in
+// kParts parts: float32 itself, or three bfloat16 values, each the nearest to
+// what the ones before leave, which is all of the 24 bits (two left errors of
+// 2e-6 in the state).  What feeds bfloat16 results is one operand.
+template <typename T>
+constexpr int kParts = sizeof(T) == 2 ? 3 : 1;
+
+// A tile in LDS, ROWS rows of W values without padding.  Rows are cut into
+// 16-byte units, and a row's units are permuted (unit u lies at u xor turn(row))
+// so that both ways of reading meet all 64 banks: one unit of 16 rows (along),
+// and 4 units of 4 rows, 8 bytes a lane (across).
+template <typename T, int W>
+struct Lds {
+  static constexpr int kUnit = 16 / static_cast<int>(sizeof(T)), kUnits = W / kUnit;
+  static __device__ __forceinline__ int turn(int row) {
+    if constexpr (kUnits >= 16) return (row & 3) << 2 | (row >> 2 & 3);
+    else if constexpr (kUnits == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+    else return row >> 2 & 3;
+  }
+  static __device__ __forceinline__ int at(int row, int col) {
+    return row * W + ((col / kUnit ^ turn(row)) * kUnit + col % kUnit);
+  }
+};
+
+// The operand whose row is the LDS row `row` (of lane l % 32) and whose k are the columns from c0 on, plain order.
+template <int W, typename T>
+__device__ __forceinline__ Operand<T> along(const T* tile, int row, int c0, int g) {
+  Operand<T> o;
+  if constexpr (sizeof(T) == 2) {
+    o.v = *reinterpret_cast<const v8b*>(tile + Lds<T, W>::at(row, c0 + 8 * g));
+  } else {
+    const v4f a = *reinterpret_cast<const v4f*>(tile + Lds<T, W>::at(row, c0 + 8 * g)),
+              b = *reinterpret_cast<const v4f*>(tile + Lds<T, W>::at(row, c0 + 8 * g + 4));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o.v[e] = a[e];
+      o.v[e + 4] = b[e];
+    }
+  }
+  return o;
 }
 
-// A computed float32 operand: in float32 itself; in bfloat16 as the nearest
-// value (16 of the 24 bits are lost with PLANES = 1), or as a sum of three,
-// each the nearest to what the ones before leave (PLANES = 3, all 24 bits),
-// which is what feeds float32 results.
-template <typename T, int PLANES>
-struct Computed {
-  static constexpr int kPlanes = sizeof(T) == 4 ? 1 : PLANES;
-  Operand<T> part[kPlanes];
-  __device__ __forceinline__ void set(int e, float x) {
+// The operand whose row is the LDS column c0 + l % 32 and whose k are the LDS
+// rows from k0 (a multiple of 16) on.  bfloat16 takes the transposing LDS
+// read: 16 lanes give 4 rows of 16 columns by 8 bytes each and get a column's
+// 4 rows.
+template <bool FOLDED, int W, typename T>
+__device__ __forceinline__ Operand<T> across(const T* tile, int k0, int c0, int ln) {
+  const int g = ln / 32;
+  const int r0 = FOLDED ? 4 * g : 8 * g, r1 = FOLDED ? 8 + 4 * g : 8 * g + 4;
+  Operand<T> o;
+  if constexpr (sizeof(T) == 2) {
+    typedef __attribute__((address_space(3))) v4s* At;
+    const int dr = ln % 16 / 4, dc = ln / 16 % 2 * 16 + ln % 4 * 4;
+    // k0 is a multiple of 16, the rows' permutation repeats with 16.
+    const T *p0 = tile + k0 * W + Lds<T, W>::at(r0 + dr, c0 + dc), *p1 = tile + k0 * W + Lds<T, W>::at(r1 + dr, c0 + dc);
+    const v4b a = __builtin_bit_cast(v4b, __builtin_amdgcn_ds_read_tr16_b64_v4i16((At)p0));
+    const v4b b = __builtin_bit_cast(v4b, __builtin_amdgcn_ds_read_tr16_b64_v4i16((At)p1));
 #pragma unroll
-    for (int i = 0; i < kPlanes; ++i) {
-      part[i].set(e, x);
-      x -= part[i].get(e);
+    for (int e = 0; e < 4; ++e) {
+      o.v[e] = a[e];
+      o.v[e + 4] = b[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o.v[e] = tile[k0 * W + Lds<T, W>::at(r0 + e, c0 + ln % 32)];
+      o.v[e + 4] = tile[k0 * W + Lds<T, W>::at(r1 + e, c0 + ln % 32)];
+    }
+  }
+  return o;
+}
+
+// The wave's number in its workgroup, as the scalar that it is.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
+
+// Memory through a descriptor whose range check gives zeros for what lies past
+// it, and drops stores there: kPast is past every range used here (each is
+// below 2^31 bytes, and so are the offsets that are added to it).
+typedef __amdgpu_buffer_rsrc_t Window;
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+constexpr uint32_t kPast = 0x80000000u;
+__device__ __forceinline__ Window window(const void* base, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes < 0 ? 0 : bytes), 0x00020000);
+}
+__device__ __forceinline__ v4f load16(Window w, uint32_t at) {
+  return __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(w, static_cast<int>(at), 0, 0));
+}
+__device__ __forceinline__ void store4(Window w, uint32_t at, const Pack<float, 4>& x) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, x), w, static_cast<int>(at), 0, 0);
+}
+__device__ __forceinline__ void store4(Window w, uint32_t at, const Pack<__bf16, 4>& x) {
+  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, x), w, static_cast<int>(at), 0, 0);
+}
+
+// ROWS rows of W columns of a stream, held by the workgroup's registers
+// between their loads and their way into LDS, 8 values a piece.
+template <typename T, int ROWS, int W, int THREADS>
+struct Rows {
+  static constexpr int kCols = W / 8, kAll = ROWS * kCols, kPieces = (kAll + THREADS - 1) / THREADS, kStep = THREADS / kCols;
+  static_assert(kAll % THREADS == 0 || kAll < THREADS, "whole pieces a thread, or one for some");
+  static_assert(THREADS % kCols == 0, "a thread keeps its columns");
+  static __device__ __forceinline__ bool idle(int thread) { return kAll < THREADS && thread >= kAll; }
+  static __device__ __forceinline__ int row(int piece, int thread) { return piece * kStep + thread / kCols; }
+  static constexpr int kUnits = static_cast<int>(sizeof(T)) / 2;
+  v4f v[kPieces][kUnits];
+  // Row r at src + r * st; rows from `rows` on and columns from n on are 0.
+  // FAST (see fast_streams): 16-byte units on their boundaries, the window's 32-bit offsets.
+  template <bool FAST>
+  __device__ __forceinline__ void load(const T* src, int64_t st, int64_t rows, int64_t c0, int64_t n) {
+    const int thread = anew(threadIdx.x), c = thread % kCols * 8, r = thread / kCols;
+    if constexpr (FAST) {
+      const int64_t here = rows < ROWS ? rows : ROWS;
+      const uint32_t size = sizeof(T), row = static_cast<uint32_t>(st) * size;
+      const Window w = window(src, here > 0 ? (here - 1) * static_cast<int64_t>(row) + n * size : 0);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int col = static_cast<int>(c0) + c + u * 8 / kUnits;
+        const uint32_t at = col < n && !idle(thread) ? r * row + col * size : kPast;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) v[i][u] = load16(w, at + i * kStep * row);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        T* one = reinterpret_cast<T*>(&v[i][0]);
+        const int64_t at = (r + i * kStep) * st + c0 + c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {  // what is not there is read at the first element, which is
+          const bool there = r + i * kStep < rows && c0 + c + e < n && !idle(thread);
+          const T x = rows > 0 ? src[there ? at + e : 0] : static_cast<T>(0.f);
+          one[e] = there ? x : static_cast<T>(0.f);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* lds) const {
+    const int thread = anew(threadIdx.x), c = thread % kCols * 8;
+    if (idle(thread)) return;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u)
+        *reinterpret_cast<v4f*>(lds + Lds<T, W>::at(row(i, thread), c + u * Lds<T, W>::kUnit)) = v[i][u];
+  }
+  // Each row times its weight (of piece i: weight[i]), as the parts of a Computed operand.
+  __device__ __forceinline__ void store_weighted(T (*planes)[ROWS * W], const float (&weight)[kPieces]) const {
+    const int thread = anew(threadIdx.x), c = thread % kCols * 8;
+    if (idle(thread)) return;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const T* x = reinterpret_cast<const T*>(&v[i][0]);
+      float rest[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) rest[e] = lane::widen(x[e]) * weight[i];
+#pragma unroll
+      for (int s = 0; s < kParts<T>; ++s) {
+        Pack<T, 8> o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          o.v[e] = lane::narrow<T>(rest[e]);
+          rest[e] -= lane::widen(o.v[e]);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+          *reinterpret_cast<v4f*>(planes[s] + Lds<T, W>::at(row(i, thread), c + u * Lds<T, W>::kUnit)) =
+              reinterpret_cast<const v4f*>(&o)[u];
+      }
     }
   }
 };
-template <typename T, int PLANES>
-__device__ __forceinline__ void mma(v4f& acc, const Operand<T>& a, const Computed<T, PLANES>& b) {
-#pragma unroll
-  for (int i = 0; i < Computed<T, PLANES>::kPlanes; ++i) mma(acc, a, b.part[i]);
-}
 
-// Tiles in LDS: rows of W values, PITCH apart; 16 bytes more than W, so that
-// 16 rows at one column lie in different banks.
-template <typename T>
-constexpr int pitch(int w) {
-  return w + 16 / static_cast<int>(sizeof(T));
-}
-
-// The operand whose row is an LDS row and whose k is a column, plain order:
-// p points at (row of lane l % 16, column k0).
-template <typename T>
-__device__ __forceinline__ Operand<T> along(const T* p, int g) {
-  Operand<T> o;
-  if constexpr (sizeof(T) == 2) {
-    o.v = *reinterpret_cast<const v8b*>(p + g * 8);
-  } else {
-    const v4f a = *reinterpret_cast<const v4f*>(p + g * 8), b = *reinterpret_cast<const v4f*>(p + g * 8 + 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      o.v[e] = a[e];
-      o.v[e + 4] = b[e];
-    }
-  }
-  return o;
-}
-
-// The operand whose row is an LDS column and whose k is an LDS row: tile
-// points at (row k0, first column) and has the pitch ld.  bfloat16 takes the
-// transposing LDS read: 16 lanes give 4 rows of 16 columns by 8 bytes each
-// and get a column's 4 rows.
-template <bool FOLDED, typename T>
-__device__ __forceinline__ Operand<T> across(const T* tile, int ld, int ln) {
-  const int g = ln / 16;
-  const int r0 = FOLDED ? 4 * g : 8 * g, r1 = FOLDED ? 16 + 4 * g : 8 * g + 4;
-  Operand<T> o;
-  if constexpr (sizeof(T) == 2) {
-    typedef __attribute__((address_space(3))) v4s* Lds;
-    const T* p = tile + (ln % 16) / 4 * ld + (ln % 4) * 4;
-    const v4b a = __builtin_bit_cast(v4b, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(p + r0 * ld)));
-    const v4b b = __builtin_bit_cast(v4b, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(p + r1 * ld)));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      o.v[e] = a[e];
-      o.v[e + 4] = b[e];
-    }
-  } else {
-    const T* p = tile + ln % 16;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      o.v[e] = p[(r0 + e) * ld];
-      o.v[e + 4] = p[(r1 + e) * ld];
-    }
-  }
-  return o;
-}
-
-// 8 values of a global row from column c on; zeros from column n on.
-template <typename T>
-__device__ __forceinline__ Pack<T, 8> row_piece(const T* row, int64_t c, int64_t n, bool vec) {
-  Pack<T, 8> p;
-  if (vec && c + 8 <= n) {
-    const auto* q = reinterpret_cast<const v4f*>(row + c);
-    auto* o = reinterpret_cast<v4f*>(&p);
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) o[i] = q[i];
+// The same 4 consecutive columns from c on of row `row` of an output [.., n] whose rows are st apart.
+template <bool FAST, typename T>
+__device__ __forceinline__ void put4(Window w, T* base, int64_t row, int64_t st, int c, int64_t n, bool row_there,
+                                     const Pack<T, 4>& x) {
+  if constexpr (FAST) {
+    store4(w, c < n ? static_cast<uint32_t>((row * st + c) * sizeof(T)) : kPast, x);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p.v[i] = c + i < n ? row[c + i] : static_cast<T>(0.f);
-  }
-  return p;
-}
-template <typename T>
-__device__ __forceinline__ void put_piece(T* lds, const Pack<T, 8>& p) {
-  const auto* q = reinterpret_cast<const v4f*>(&p);
-  auto* o = reinterpret_cast<v4f*>(lds);
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) o[i] = q[i];
-}
-
-// ROWS rows of a stream (stride st), columns [c0, c0 + W) of n, into LDS; rows from `rows` on and columns from n on are 0.
-template <int ROWS, int W, int THREADS, typename T>
-__device__ __forceinline__ void stage(T* lds, const T* src, int64_t st, int64_t rows, int64_t c0, int64_t n, bool vec) {
-  constexpr int kPieces = W / 8;
-  static_assert(ROWS * kPieces % THREADS == 0 || ROWS * kPieces < THREADS, "whole pieces a thread");
-#pragma unroll
-  for (int i = threadIdx.x; i < ROWS * kPieces; i += THREADS) {
-    const int r = i / kPieces, c = i % kPieces * 8;
-    Pack<T, 8> p{};
-    if (r < rows) p = row_piece(src + r * st, c0 + c, n, vec);
-    put_piece(lds + r * pitch<T>(W) + c, p);
+    for (int e = 0; e < 4; ++e)
+      if (row_there && c + e < n) base[row * st + c + e] = x.v[e];
   }
 }
 
@@ -171,16 +267,23 @@ __device__ __forceinline__ int64_t row_length(const SelectArgs& a, int64_t b) {
   return n < 0 ? 0 : n > a.t ? a.t : n;
 }
 
-// The time step of token t: (step, derivative of the step by dt).
-__device__ __forceinline__ float time_step(const SelectArgs& a, int64_t b, int64_t t, int64_t h, float& slope) {
-  const int64_t at = b * a.dt_batch + t * a.dt_row + h;
-  float v = lane::param(a.dt, at, a.dt_bf16);
-  if (a.dt_bias != nullptr) v += a.dt_bias[h];
-  slope = 1.f;
-  if (!a.softplus) return v;
-  slope = lane::softplus_slope_(v);
-  return lane::softplus_(v);
-}
+// The tokens' steps d and running sums s of d A (to base 2), from steps_kernel.
+// The sums are kept so that differences of near tokens are exact to float32: a
+// sum of -100 has steps of 8e-6, which would be the relative error of every
+// decay in a fast head.  near[t] is the sum from the start of t's 16 tokens,
+// base[i] (float64) the sum before the i'th 16 tokens from the last multiple of
+// kSpan tokens.  The time axis is padded to kSpan with d = 0.
+constexpr int kSpan = 128, kNear = 16;
+struct Steps {
+  const float *step, *near;
+  const double* base;
+  __device__ __forceinline__ Steps(const SelectArgs& a, int64_t b, int64_t h) {
+    const int64_t tp = (a.t + kSpan - 1) / kSpan * kSpan, all = a.b * a.h, at = b * a.h + h;
+    base = reinterpret_cast<const double*>(a.steps) + at * (tp / kNear);
+    step = a.steps + 2 * all * (tp / kNear) + at * tp;
+    near = step + all * tp;
+  }
+};
 
 // Inclusive sum over the wave's lanes.
 template <typename V>
@@ -193,37 +296,6 @@ __device__ __forceinline__ V lanes_prefix(V x) {
   }
   return x;
 }
-
-// The running sums s of d A (to base 2) of L tokens, kept so that differences
-// of near tokens are exact to float32: a sum of -100 has steps of 8e-6, which
-// would be the relative error of every decay in a fast head.  near[t] is the
-// sum from t's 16 tokens' start, base[i] (float64) the sum before those.
-template <int L>
-struct Sums {
-  alignas(16) float near[L];
-  double base[L / 16];
-  // s_i - s_j for tokens of the 16-token blocks bi and bj is
-  // (near[i] + between(bi, bj)) - near[j].
-  __device__ __forceinline__ float between(int bi, int bj) const { return static_cast<float>(base[bi] - base[bj]); }
-  __device__ __forceinline__ double at(int t) const { return base[t / 16] + near[t]; }
-  // By one wave: a lane gives the steps' logarithms of PER tokens from PER * lane on.
-  template <int PER>
-  __device__ __forceinline__ void fill(const float (&log2_fade)[PER]) {
-    const int ln = threadIdx.x % kWave;
-    double own = 0.;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) own += log2_fade[e];
-    double s = lanes_prefix(own) - own;
-    const int first = PER * ln / 16 * 16 / PER;  // the lane that the 16 tokens start in
-    const double start = __shfl(s, first, kWave);
-    if (PER * ln % 16 == 0) base[PER * ln / 16] = s;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      s += log2_fade[e];
-      near[PER * ln + e] = static_cast<float>(s - start);
-    }
-  }
-};
 
 }  // namespace select_scan
 }  // namespace bssm

@@ -20,9 +20,15 @@
 // it goes through the heads (and through P 64 values at a time, which are
 // heads of their own as far as the sums are concerned) with the gradients of B
 // and C in registers, so that those leave once a part instead of once a head.
-// A wave owns 16 tokens: as j for gu and gB, as i for gC; E, S and G are
-// formed in the layout of a product's result, twice, once for either side, so
-// that each is the next product's operand as it is.
+// Half of the waves own 32 tokens each as j, for gu and gB, against the blocks
+// of 32 behind them, the other half as i, for gC, against those before; the two
+// waves of a SIMD have L / 32 + 1 blocks together.  Either forms S and G with
+// its own tokens as the columns of the products' results, so that E S and E G
+// are the next products' operands as they are.  Between blocks, E is a product of a decay to (or from) the block's border that
+// belongs to the row and one that belongs to the own token.  What h, gh, x and
+// gy of the next head (and the second half of this one's h and gh) need from
+// memory is asked for while this one is computed.  The token sums row, col,
+// ... go to memory, where tokens_kernel closes them.
 //
 // Rounding with bfloat16 streams: S and G are exact products of the streams in
 // float32.  What feeds the float32 results (ga, gd and their sums) is float32
@@ -37,42 +43,235 @@ hipError_t launch_adjoints(const SelectArgs& a, hipStream_t stream);  // bssm_se
 
 namespace {
 
-constexpr int kTileP = 64;
 constexpr int kHalf = 32;  // rows of h and gh in LDS at a time
 
-__device__ __forceinline__ bool pieces16(const void* p, int64_t b, int64_t r, int64_t g, int64_t n, int bf16) {
-  const int k = bf16 ? 8 : 4;
-  return n % k == 0 && b % k == 0 && r % k == 0 && g % k == 0 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
-}
-
-// 4 values of a [P, N] record; zeros outside.
-__device__ __forceinline__ v4f record_piece(const float* src, int64_t p, int64_t c, int64_t np, int64_t n) {
-  v4f o = {0.f, 0.f, 0.f, 0.f};
-  if (p >= np || c >= n) return o;
-  if (n % 4 == 0) return *reinterpret_cast<const v4f*>(src + p * n + c);
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (c + r < n) o[r] = src[p * n + c + r];
-  return o;
-}
+static_assert(kTileP == 2 * kHalf, "two halves");
 
 template <typename T>
 struct Sizes {
   static constexpr int kL = sizeof(T) == 2 ? 128 : 64;      // tokens of a record
-  static constexpr int kThreads = kL * 4;                   // a wave for 16 tokens
-  static constexpr int kPlanes = sizeof(T) == 2 ? 3 : 1;    // parts of h and gh
-  static constexpr int kPerLane = kL / kWave;               // tokens a lane of wave 0
+  static constexpr int kBlocks = kL / kTile;                // of 32 tokens
+  static constexpr int kThreads = 2 * kBlocks * kWave;
 };
 
+// The token sums in memory, each [B, H, padded T]: row + C . gC', B . gB' / d, col and the diagonal; then, a wave each,
+// <gh, h> and gy . x of a record: [2, B, H, records, waves].
+struct TokenSums {
+  float *later, *earlier, *direct, *diagonal, *whole, *skip;
+  __device__ __forceinline__ TokenSums(const SelectArgs& a, int64_t b, int64_t h, int64_t records, int waves) {
+    const int64_t tp = (a.t + kSpan - 1) / kSpan * kSpan, all = a.b * a.h, at = b * a.h + h;
+    later = a.token_sums + at * tp;
+    earlier = later + all * tp;
+    direct = earlier + all * tp;
+    diagonal = direct + all * tp;
+    whole = a.token_sums + 4 * all * tp + at * records * waves;
+    skip = whole + all * records * waves;
+  }
+};
+
+// A half (32 values of P) of a [P, N] record in registers.
 template <typename T, int NP>
-__global__ __launch_bounds__(Sizes<T>::kThreads) void backward_kernel(SelectArgs a, int64_t parts) {
+struct HalfRecord {
+  static constexpr int kThreads = Sizes<T>::kThreads, kAll = kHalf * NP / 4, kPieces = (kAll + kThreads - 1) / kThreads;
+  static_assert(kAll % kThreads == 0 || kAll < kThreads, "whole pieces a thread, or one for some");
+  v4f v[kPieces];
+  template <bool FAST>
+  __device__ __forceinline__ void load(const float* src, int64_t p_first, int64_t np, int64_t n) {
+    src += p_first * n;
+    const int64_t rows = np - p_first < kHalf ? np - p_first : kHalf;
+    const Window w = window(src, rows * n * 4);
+    const int thread = anew(threadIdx.x);
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      const int at = (k * kThreads + thread) * 4, c = at % NP, p = at / NP;
+      if constexpr (FAST) {
+        v[k] = load16(w, c < n ? static_cast<uint32_t>(p * n + c) * 4u : kPast);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[k][r] = p < rows && c + r < n ? src[p * n + c + r] : 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ float dot(const HalfRecord& o) const {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s = fmaf(v[k][r], o.v[k][r], s);
+    return s;
+  }
+  __device__ __forceinline__ void store(T (*planes)[kHalf * NP]) const {
+    const int thread = anew(threadIdx.x);
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      const int at = (k * kThreads + thread) * 4;
+      if (at >= kHalf * NP) break;
+      v4f rest = v[k];
+#pragma unroll
+      for (int s = 0; s < kParts<T>; ++s) {
+        Pack<T, 4> o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          o.v[r] = lane::narrow<T>(rest[r]);
+          rest[r] -= lane::widen(o.v[r]);
+        }
+        lane::store_pack<T, 4>(planes[s] + Lds<T, NP>::at(at / NP, at % NP), o);
+      }
+    }
+  }
+};
+
+// What a workgroup holds in LDS.
+template <typename T, int NP>
+struct Tiles {
+  static constexpr int L = Sizes<T>::kL;
+  alignas(16) T xs[L * kTileP], gs[L * kTileP], ks[L * NP], qs[L * NP];
+  alignas(16) T hs[kParts<T>][kHalf * NP], ghs[kParts<T>][kHalf * NP];
+  // since: decay from the start of the token's 32 to it; until: its step times the decay from it to their end.
+  alignas(16) float step[L], near[L], since[L], until[L];
+  double base[L / kNear];
+  __device__ __forceinline__ double at(int t) const { return base[t / kNear] + near[t]; }
+};
+
+// A lane's sums for its own token.
+struct Own {
+  float row, col, diagonal, dot_x;  // inside the record: as i, as j, of the diagonal, gy . x
+  float from_h, from_gh;            // with what comes from h and gh
+};
+
+// The record's tokens with each other, the wave's own as i (AS_I: gC) or as j (gB and gu).
+template <typename T, int NP, bool AS_I>
+__device__ __forceinline__ void inside(const Tiles<T, NP>& t, int block, v16f (&acc)[NP / kTile],
+                                       v16f (&gu)[kTileP / kTile], Own& sum) {
+  constexpr int kBlocks = Sizes<T>::kBlocks;
+  const int ln = anew(threadIdx.x % kWave), g = ln / 32, own = block * kTile + ln % 32;
+  // The streams of the own tokens, and of the other side.
+  const T *own_n = AS_I ? t.qs : t.ks, *own_p = AS_I ? t.gs : t.xs, *other_n = AS_I ? t.ks : t.qs,
+          *other_p = AS_I ? t.xs : t.gs;
+  const float d_own = t.step[own], near_own = t.near[own];
+  const double base_own = t.base[own / kNear];
+  Operand<T> n_own[NP / kDepth];
+#pragma unroll
+  for (int k = 0; k < NP / kDepth; ++k) n_own[k] = along<NP>(own_n, own, k * kDepth, g);
+#pragma unroll 1
+  for (int blk = AS_I ? 0 : block; blk <= (AS_I ? block : kBlocks - 1); ++blk) {
+    v16f s = zeros(), gx = zeros();
+#pragma unroll
+    for (int k = 0; k < NP / kDepth; ++k) mma(s, along<NP>(other_n, blk * kTile + ln % 32, k * kDepth, g), n_own[k]);
+#pragma unroll
+    for (int k = 0; k < kTileP / kDepth; ++k)
+      mma(gx, along<kTileP>(other_p, blk * kTile + ln % 32, k * kDepth, g), along<kTileP>(own_p, own, k * kDepth, g));
+    Operand<T> es[2], eg[2];
+    if (blk != block) {
+      // Border between the blocks: the end of the rows' block (AS_I) or its start.
+      const int first = blk * kTile, last = first + kTile - 1;
+      const float border = lane::exp2_(AS_I ? static_cast<float>(base_own + near_own - t.at(last))
+                                            : static_cast<float>(t.base[first / kNear] - base_own - near_own));
+      const float border_d = border * d_own;
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const v4f decay = *reinterpret_cast<const v4f*>((AS_I ? t.until : t.since) + first + 8 * q4 + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int el = 4 * q4 + e;
+          if (AS_I) {
+            const float egv = decay[e] * border * gx[el];
+            eg[q4 / 2].set(el % 8, egv);
+            sum.row = fmaf(egv, s[el], sum.row);
+          } else {
+            const float esv = decay[e] * border * s[el];
+            es[q4 / 2].set(el % 8, esv);
+            eg[q4 / 2].set(el % 8, decay[e] * border_d * gx[el]);
+            sum.col = fmaf(esv, gx[el], sum.col);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const int row = blk * kTile + 8 * q4 + 4 * g;
+        const float gap = static_cast<float>(t.base[(blk * kTile + 8 * q4) / kNear] - base_own) - near_own;
+        const v4f nr = *reinterpret_cast<const v4f*>(t.near + row), dr = *reinterpret_cast<const v4f*>(t.step + row);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = row + e, el = 4 * q4 + e;
+          const float diff = nr[e] + gap;  // s_row - s_own
+          const bool in = AS_I ? at <= own : at >= own;
+          // Selected after the exponential, which is as good outside as in, so that no lane branches.
+          const float ex = lane::exp2_(AS_I ? -diff : diff), ev = in ? ex : 0.f;
+          const float sv = in ? s[el] : 0.f, gv = in ? gx[el] : 0.f, esv = ev * sv, w = esv * gv;
+          if (!AS_I) es[q4 / 2].set(el % 8, esv);
+          eg[q4 / 2].set(el % 8, ev * gv * (AS_I ? dr[e] : d_own));
+          if (AS_I) {
+            sum.row = fmaf(at == own ? 0.f : w, dr[e], sum.row);
+          } else {
+            const float dw = at == own ? w : 0.f;
+            sum.col += w - dw;
+            sum.diagonal += dw;
+            sum.dot_x += at == own ? gx[el] : 0.f;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r0 = blk * kTile + half * kDepth;
+      if (!AS_I)
+#pragma unroll
+        for (int m = 0; m < kTileP / kTile; ++m) mma(gu[m], across<true, kTileP>(t.gs, r0, m * kTile, ln), es[half]);
+#pragma unroll
+      for (int n = 0; n < NP / kTile; ++n) mma(acc[n], across<true, NP>(other_n, r0, n * kTile, ln), eg[half]);
+    }
+  }
+}
+
+// What comes from 32 values of P of the state before the record, gC: exp(s_i) h^T gy_i (AS_I), or of the adjoint
+// behind it, gu and gB.  h C_i (gh B_j) is formed in full, for its dot product with gy_i (x_j) and for gu; gC (gB)
+// takes the first part of h (gh).
+template <typename T, int NP, bool AS_I>
+__device__ __forceinline__ void outside(const Tiles<T, NP>& t, int block, int half, v16f (&acc)[NP / kTile], v16f& gu,
+                                        Own& sum) {
+  constexpr int L = Sizes<T>::kL;
+  const int ln = anew(threadIdx.x % kWave), g = ln / 32, own = block * kTile + ln % 32;
+  const T *own_n = AS_I ? t.qs : t.ks, *own_p = AS_I ? t.gs : t.xs;
+  const float fade = lane::exp2_(static_cast<float>(AS_I ? t.at(own) - t.base[0] : t.at(L - 1) - t.at(own)));
+  const float into = AS_I ? fade : fade * t.step[own];
+  v16f z = zeros();
+#pragma unroll
+  for (int k = 0; k < NP / kDepth; ++k) {
+    const Operand<T> n_own = along<NP>(own_n, own, k * kDepth, g);
+#pragma unroll
+    for (int s = 0; s < kParts<T>; ++s) mma(z, along<NP>(AS_I ? t.hs[s] : t.ghs[s], ln % 32, k * kDepth, g), n_own);
+  }
+  float dot = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; r += 4) {
+    const Pack<T, 4> v = lane::load_pack<T, 4>(own_p + Lds<T, kTileP>::at(own, half * kHalf + result_row(r, g)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      dot = fmaf(z[r + e], lane::widen(v.v[e]), dot);
+      if (!AS_I) gu[r + e] = fmaf(z[r + e], fade, gu[r + e]);
+    }
+  }
+  if (AS_I) sum.from_h = fmaf(dot, fade, sum.from_h);
+  else sum.from_gh = fmaf(dot, fade, sum.from_gh);
+#pragma unroll
+  for (int k = 0; k < kHalf / kDepth; ++k) {
+    Operand<T> p_own = along<kTileP>(own_p, own, half * kHalf + k * kDepth, g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p_own.set(e, p_own.get(e) * into);
+#pragma unroll
+    for (int n = 0; n < NP / kTile; ++n)
+      mma(acc[n], across<false, NP>(AS_I ? t.hs[0] : t.ghs[0], k * kDepth, n * kTile, ln), p_own);
+  }
+}
+
+// The whole of a wave that owns tokens as i (AS_I) or as j; both kinds pass the same barriers.
+template <typename T, int NP, bool FAST, bool AS_I>
+__device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts, Tiles<T, NP>& t) {
   using Z = Sizes<T>;
-  constexpr int L = Z::kL, kThreads = Z::kThreads, kWaves = kThreads / kWave, kPl = pitch<T>(kTileP), nPl = pitch<T>(NP);
-  constexpr int kPieces = (kHalf * NP / 4 + kThreads - 1) / kThreads;
-  __shared__ __align__(16) T xs[L * kPl], gs[L * kPl], ks[L * nPl], qs[L * nPl], hs[Z::kPlanes][kHalf * nPl], ghs[Z::kPlanes][kHalf * nPl];
-  __shared__ __align__(16) float step[L], tok_f[L], tok_b[L], tok_d[L], red[kWaves][2];
-  __shared__ Sums<L> sums;
-  const int wave = threadIdx.x / kWave, ln = threadIdx.x % kWave, g = ln / 16, own = wave * 16 + ln % 16;
+  constexpr int L = Z::kL, kThreads = Z::kThreads, kWaves = kThreads / kWave;
+  const int wave = wave_index(), block = wave % Z::kBlocks;
   // Sequences vary fastest, so that a part's neighbours on an XCD share B, C.
   int64_t i = blockIdx.x;
   const int64_t b = i % a.b;
@@ -84,283 +283,217 @@ __global__ __launch_bounds__(Sizes<T>::kThreads) void backward_kernel(SelectArgs
                 h_last = grp * per_group + (part + 1) * per_group / parts;
   const int64_t t0 = rec * L, live = row_length(a, b) - t0, pn = a.p * a.n;
   {
-    const bool vb = pieces16(a.bk, a.bk_batch, a.bk_row, a.bk_group, a.n, a.bf16),
-               vc = pieces16(a.cq, a.cq_batch, a.cq_row, a.cq_group, a.n, a.bf16);
-    stage<L, NP, kThreads>(ks, static_cast<const T*>(a.bk) + b * a.bk_batch + grp * a.bk_group + t0 * a.bk_row,
-                           a.bk_row, live, 0, a.n, vb);
-    stage<L, NP, kThreads>(qs, static_cast<const T*>(a.cq) + b * a.cq_batch + grp * a.cq_group + t0 * a.cq_row,
-                           a.cq_row, live, 0, a.n, vc);
+    Rows<T, L, NP, kThreads> rows;
+    rows.template load<FAST>(static_cast<const T*>(a.bk) + b * a.bk_batch + grp * a.bk_group + t0 * a.bk_row, a.bk_row,
+                             live, 0, a.n);
+    rows.store(t.ks);
+    rows.template load<FAST>(static_cast<const T*>(a.cq) + b * a.cq_batch + grp * a.cq_group + t0 * a.cq_row, a.cq_row,
+                             live, 0, a.n);
+    rows.store(t.qs);
   }
-  const bool vx = pieces16(a.x, a.x_batch, a.x_row, a.x_head, a.p, a.bf16), vg = pieces16(a.gy, a.p, a.p, a.p, a.p, a.bf16);
-  v4f gk[NP / 16], gq[NP / 16];  // gradients of B and C, transposed: rows n, column own
+  v16f acc[NP / kTile];  // gradient of C (as i) or B (as j), transposed: rows n, column own
 #pragma unroll
-  for (int n = 0; n < NP / 16; ++n) gk[n] = gq[n] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int n = 0; n < NP / kTile; ++n) acc[n] = zeros();
 
+  Rows<T, L, kTileP, kThreads> rx, rg;
+  HalfRecord<T, NP> rh, rgh;
+  float r_step = 0.f, r_near = 0.f, r_near_end = 0.f;  // of token threadIdx.x
+  double r_base = 0., r_start = 0., r_end = 0.;
+  auto load_half = [&](int64_t h, int64_t p_first) {
+    rh.template load<FAST>(a.states + ((b * a.h + h) * records + rec) * pn, p_first, a.p, a.n);
+    rgh.template load<FAST>(a.adjoints + ((b * a.h + h) * records + rec) * pn, p_first, a.p, a.n);
+  };
+  auto load = [&](int64_t h, int64_t p0) {
+    rx.template load<FAST>(static_cast<const T*>(a.x) + b * a.x_batch + t0 * a.x_row + h * a.x_head, a.x_row, live, p0,
+                           a.p);
+    rg.template load<FAST>(static_cast<const T*>(a.gy) + ((b * a.t + t0) * a.h + h) * a.p, a.h * a.p, live, p0, a.p);
+    load_half(h, p0);
+    const int at = anew(threadIdx.x);
+    if (at < L) {
+      const Steps s(a, b, h);
+      const int first = at / kTile * kTile;
+      r_step = s.step[t0 + at];
+      r_near = s.near[t0 + at];
+      r_near_end = s.near[t0 + first + kTile - 1];
+      r_base = s.base[(t0 + at) / kNear];
+      r_start = s.base[(t0 + first) / kNear];
+      r_end = s.base[(t0 + first) / kNear + kTile / kNear - 1];
+    }
+  };
+  load(h_first, 0);
   for (int64_t h = h_first; h < h_last; ++h) {
-    const float rate = a.rate[h], rate2 = rate * lane::kLog2e, skip = a.skip == nullptr ? 0.f : a.skip[h];
-    float row = 0.f, col = 0.f, diagonal = 0.f, from_h = 0.f, from_gh = 0.f, dot_h = 0.f, dot_x = 0.f;
-    float d_lane[Z::kPerLane], slope[Z::kPerLane];  // wave 0
+    const float skip = a.skip == nullptr ? 0.f : a.skip[h];
+    Own sum{0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    float dot_h = 0.f;
     for (int64_t p0 = 0; p0 < a.p; p0 += kTileP) {
       __syncthreads();
-      stage<L, kTileP, kThreads>(xs, static_cast<const T*>(a.x) + b * a.x_batch + t0 * a.x_row + h * a.x_head, a.x_row,
-                                 live, p0, a.p, vx);
-      stage<L, kTileP, kThreads>(gs, static_cast<const T*>(a.gy) + ((b * a.t + t0) * a.h + h) * a.p, a.h * a.p, live,
-                                 p0, a.p, vg);
-      const float* h_rec = a.states + ((b * a.h + h) * records + rec) * pn;
-      const float* gh_rec = a.adjoints + ((b * a.h + h) * records + rec) * pn;
-      auto stage_half = [&](int64_t from) {
-#pragma unroll
-        for (int k = 0; k < kPieces; ++k) {
-          const int at = (k * kThreads + threadIdx.x) * 4, p = at / NP, c = at % NP;
-          if (p >= kHalf) break;
-          v4f hv = record_piece(h_rec, from + p, c, a.p, a.n), gv = record_piece(gh_rec, from + p, c, a.p, a.n);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) dot_h = fmaf(hv[r], gv[r], dot_h);
-#pragma unroll
-          for (int s = 0; s < Z::kPlanes; ++s) {
-            Pack<T, 4> o, go;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              o.v[r] = lane::narrow<T>(hv[r]);
-              go.v[r] = lane::narrow<T>(gv[r]);
-              hv[r] -= lane::widen(o.v[r]);
-              gv[r] -= lane::widen(go.v[r]);
-            }
-            lane::store_pack<T, 4>(hs[s] + p * nPl + c, o);
-            lane::store_pack<T, 4>(ghs[s] + p * nPl + c, go);
-          }
-        }
-      };
-      stage_half(p0);
-      if (wave == 0 && p0 == 0) {
-        float log2_fade[Z::kPerLane];
-#pragma unroll
-        for (int e = 0; e < Z::kPerLane; ++e) {  // lane: tokens kPerLane * ln + e
-          const int64_t t = Z::kPerLane * ln + e;
-          d_lane[e] = slope[e] = 0.f;
-          if (t < live) d_lane[e] = time_step(a, b, t0 + t, h, slope[e]);
-          step[t] = d_lane[e];
-          log2_fade[e] = d_lane[e] * rate2;
-        }
-        sums.template fill<Z::kPerLane>(log2_fade);
+      rx.store(t.xs);
+      rg.store(t.gs);
+      dot_h += rh.dot(rgh);
+      rh.store(t.hs);
+      rgh.store(t.ghs);
+      if (const int at = anew(threadIdx.x); at < L) {
+        t.step[at] = r_step;
+        t.near[at] = r_near;
+        t.since[at] = lane::exp2_(static_cast<float>(r_base - r_start + r_near));
+        t.until[at] = r_step * lane::exp2_(static_cast<float>(r_end + r_near_end - r_base - r_near));
+        if (at % kNear == 0) t.base[at / kNear] = r_base;
       }
       __syncthreads();
-      const float s_own = sums.near[own], d_own = step[own];
-      Operand<T> x_own[2], g_own[2];
+      const bool second = p0 + kHalf < a.p;
+      if (second) load_half(h, p0 + kHalf);
+      v16f gu[kTileP / kTile];  // rows p, column own (as j)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        x_own[k] = along(xs + own * kPl + 32 * k, g);
-        g_own[k] = along(gs + own * kPl + 32 * k, g);
-      }
-      v4f gu[kTileP / 16];  // rows p, column own
+      for (int m = 0; m < kTileP / kTile; ++m) gu[m] = zeros();
+      inside<T, NP, AS_I>(t, block, acc, gu, sum);
 #pragma unroll
-      for (int k = 0; k < kTileP / 16; ++k) gu[k] = v4f{0.f, 0.f, 0.f, 0.f};
-      {  // own = j: rows i
-        Operand<T> k_own[NP / 32];
-#pragma unroll
-        for (int k = 0; k < NP / 32; ++k) k_own[k] = along(ks + own * nPl + 32 * k, g);
-        for (int kk = wave / 2; kk < L / 32; ++kk) {
-          Computed<T, 1> es, eg;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int i0 = kk * 32 + half * 16;
-            v4f s = {0.f, 0.f, 0.f, 0.f}, gx = {0.f, 0.f, 0.f, 0.f};
-            if (i0 >= wave * 16) {
-#pragma unroll
-              for (int k = 0; k < NP / 32; ++k) mma(s, along(qs + (i0 + ln % 16) * nPl + 32 * k, g), k_own[k]);
-#pragma unroll
-              for (int k = 0; k < 2; ++k) mma(gx, along(gs + (i0 + ln % 16) * kPl + 32 * k, g), x_own[k]);
-            }
-            const float to = sums.between(i0 / 16, wave) - s_own;
-            const v4f si = *reinterpret_cast<const v4f*>(sums.near + i0 + 4 * g);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int at = i0 + 4 * g + r;
-              const float e = at >= own ? lane::exp2_(si[r] + to) : 0.f;
-              const float esr = e * s[r];
-              es.set(half * 4 + r, esr);
-              eg.set(half * 4 + r, e * gx[r] * d_own);
-              if (at == own) {
-                diagonal = fmaf(esr, gx[r], diagonal);
-                dot_x += gx[r];
-              } else {
-                col = fmaf(esr, gx[r], col);
-              }
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < kTileP / 16; ++k) mma(gu[k], across<true>(gs + kk * 32 * kPl + 16 * k, kPl, ln), es);
-#pragma unroll
-          for (int n = 0; n < NP / 16; ++n) mma(gk[n], across<true>(qs + kk * 32 * nPl + 16 * n, nPl, ln), eg);
-        }
-      }
-      {  // own = i: rows j
-        Operand<T> q_own[NP / 32];
-#pragma unroll
-        for (int k = 0; k < NP / 32; ++k) q_own[k] = along(qs + own * nPl + 32 * k, g);
-        for (int kk = 0; kk <= wave / 2; ++kk) {
-          Computed<T, 1> eg;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int j0 = kk * 32 + half * 16;
-            v4f s = {0.f, 0.f, 0.f, 0.f}, gx = {0.f, 0.f, 0.f, 0.f};
-            if (j0 <= wave * 16) {
-#pragma unroll
-              for (int k = 0; k < NP / 32; ++k) mma(s, along(ks + (j0 + ln % 16) * nPl + 32 * k, g), q_own[k]);
-#pragma unroll
-              for (int k = 0; k < 2; ++k) mma(gx, along(xs + (j0 + ln % 16) * kPl + 32 * k, g), g_own[k]);
-            }
-            const float from = s_own + sums.between(wave, j0 / 16);
-            const v4f sj = *reinterpret_cast<const v4f*>(sums.near + j0 + 4 * g), dj = *reinterpret_cast<const v4f*>(step + j0 + 4 * g);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int at = j0 + 4 * g + r;
-              const float e = at <= own ? lane::exp2_(from - sj[r]) * dj[r] * gx[r] : 0.f;
-              eg.set(half * 4 + r, e);
-              if (at != own) row = fmaf(e, s[r], row);
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NP / 16; ++n) mma(gq[n], across<true>(ks + kk * 32 * nPl + 16 * n, nPl, ln), eg);
-        }
-      }
-      // From the state before the record, gC: exp(s_i) h^T gy_i; from the adjoint behind it, gu and gB.
-      const float before = lane::exp2_(static_cast<float>(sums.at(own))),
-                  behind = lane::exp2_(static_cast<float>(sums.at(L - 1) - sums.at(own)));
-#pragma unroll
-      for (int half = 0; half < kTileP / kHalf; ++half) {
-        if (half > 0) {
-          if (p0 + half * kHalf >= a.p) break;  // uniform
+      for (int half = 0; half < 2; ++half) {
+        if (half == 1) {
+          if (!second) break;
           __syncthreads();
-          stage_half(p0 + half * kHalf);
+          dot_h += rh.dot(rgh);
+          rh.store(t.hs);
+          rgh.store(t.ghs);
           __syncthreads();
         }
-#pragma unroll
-        for (int m = 0; m < kHalf / 16; ++m) {
-          v4f o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int k = 0; k < NP / 32; ++k)
-            mma(o, along(ghs[0] + (16 * m + ln % 16) * nPl + 32 * k, g), along(ks + own * nPl + 32 * k, g));
-          gu[half * (kHalf / 16) + m] += o * behind;
+        if (half == (second ? 1 : 0)) {
+          const bool more = p0 + kTileP < a.p;
+          if (more || h + 1 < h_last) load(more ? h : h + 1, more ? p0 + kTileP : 0);
         }
-#pragma unroll
-        for (int n = 0; n < NP / 16; ++n) {
-          v4f o = {0.f, 0.f, 0.f, 0.f}, go = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = 0; s < Z::kPlanes; ++s) {
-            mma(o, across<false>(hs[s] + 16 * n, nPl, ln), g_own[half]);
-            mma(go, across<false>(ghs[s] + 16 * n, nPl, ln), x_own[half]);
-          }
-          const Pack<T, 4> q = lane::load_pack<T, 4>(qs + own * nPl + 16 * n + 4 * g),
-                           kb = lane::load_pack<T, 4>(ks + own * nPl + 16 * n + 4 * g);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            o[r] *= before;
-            go[r] *= behind;
-            from_h = fmaf(o[r], lane::widen(q.v[r]), from_h);
-            from_gh = fmaf(go[r], lane::widen(kb.v[r]), from_gh);
-          }
-          gq[n] += o;
-          gk[n] += go * d_own;
-        }
+        outside<T, NP, AS_I>(t, block, half, acc, gu[half], sum);
       }
-      if (t0 + own < a.t) {
-        T* out = static_cast<T*>(a.gx) + ((b * a.t + t0 + own) * a.h + h) * a.p + p0;
+      if (!AS_I) {
+        const int ln = anew(threadIdx.x % kWave), g = ln / 32, own = block * kTile + ln % 32;
+        const float d_own = t.step[own];
+        const int64_t row = a.h * a.p, rows = a.t - t0 < L ? a.t - t0 : L, cols = a.p - p0;
+        T* out = static_cast<T*>(a.gx) + (b * a.t + t0) * row + h * a.p + p0;
+        const Window w = window(out, ((rows - 1) * row + cols) * sizeof(T));
 #pragma unroll
-        for (int k = 0; k < kTileP / 16; ++k) {
-          const int c0 = 16 * k + 4 * g;
-          const Pack<T, 4> gi = lane::load_pack<T, 4>(gs + own * kPl + c0);
-          Pack<T, 4> o;
+        for (int m = 0; m < kTileP / kTile; ++m)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o.v[r] = lane::narrow<T>(fmaf(d_own, gu[k][r], skip * lane::widen(gi.v[r])));
-          if (p0 + c0 + 4 <= a.p && a.p % 4 == 0) {
-            lane::store_pack<T, 4>(out + c0, o);
-          } else {
+          for (int r = 0; r < 16; r += 4) {
+            const int c0 = m * kTile + result_row(r, g);
+            const Pack<T, 4> gi = lane::load_pack<T, 4>(t.gs + Lds<T, kTileP>::at(own, c0));
+            Pack<T, 4> o;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (p0 + c0 + r < a.p) out[c0 + r] = o.v[r];
+            for (int e = 0; e < 4; ++e) o.v[e] = lane::narrow<T>(fmaf(d_own, gu[m][r + e], skip * lane::widen(gi.v[e])));
+            put4<FAST>(w, out, own, row, c0, cols, own < rows, o);
           }
-        }
       }
     }
-    // The head's token sums: lanes g = 0..3 of a column hold parts of them.
-    auto over_groups = [](float v) {
-      v += __shfl_xor(v, 16, kWave);
-      return v + __shfl_xor(v, 32, kWave);
-    };
-    row = over_groups(row);
-    col = over_groups(col);
-    diagonal = over_groups(diagonal);
-    from_h = over_groups(from_h);
-    from_gh = over_groups(from_gh);
-    const float d_own = step[own];
-    if (g == 0) {
-      tok_f[own] = row - d_own * col + from_h;
-      tok_b[own] = d_own * from_gh;
-      tok_d[own] = diagonal + col + from_gh;
+    // The head's token sums: the two halves of a column hold parts of them.
+    const int ln = anew(threadIdx.x % kWave), g = ln / 32, own = block * kTile + ln % 32;
+    const TokenSums to(a, b, h, records, kWaves);
+    auto both = [](float v) { return v + __shfl_xor(v, 32, kWave); };
+    if (AS_I) {
+      const float later = both(sum.row + sum.from_h);
+      if (g == 0) to.later[t0 + own] = later;
+    } else {
+      const float earlier = both(sum.from_gh), direct = both(sum.col), diagonal = both(sum.diagonal);
+      if (g == 0) {
+        to.earlier[t0 + own] = earlier;
+        to.direct[t0 + own] = direct;
+      } else {
+        to.diagonal[t0 + own] = diagonal;
+      }
     }
-    dot_h = lane::lanes_sum(dot_h);
-    dot_x = lane::lanes_sum(dot_x);
+    const float whole = lane::lanes_sum(dot_h), gx = lane::lanes_sum(sum.dot_x);
     if (ln == 0) {
-      red[wave][0] = dot_h;
-      red[wave][1] = dot_x;
-    }
-    __syncthreads();
-    if (wave == 0) {
-      float whole = 0.f, skip_sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        whole += red[w][0];
-        skip_sum += red[w][1];
-      }
-      whole *= lane::exp2_(static_cast<float>(sums.at(L - 1)));
-      float f = 0.f, bsum = 0.f;
-#pragma unroll
-      for (int e = 0; e < Z::kPerLane; ++e) {
-        f += tok_f[Z::kPerLane * ln + e];
-        bsum += tok_b[Z::kPerLane * ln + e];
-      }
-      // f of this lane's tokens and later, b of earlier ones
-      const float f_up = lanes_prefix(f);
-      float later = __shfl(f_up, kWave - 1, kWave) - f_up + f, earlier = lanes_prefix(bsum) - bsum;
-      float g_rate = 0.f, g_bias = 0.f;
-#pragma unroll
-      for (int e = 0; e < Z::kPerLane; ++e) {
-        const int t = Z::kPerLane * ln + e;
-        const float ga = later + earlier + whole;
-        later -= tok_f[t];
-        earlier += tok_b[t];
-        const float gd = fmaf(rate, ga, tok_d[t]) * slope[e];
-        g_rate = fmaf(d_lane[e], ga, g_rate);
-        g_bias += gd;
-        if (t0 + t < a.t) lane::put_param(a.gdt, (b * a.t + t0 + t) * a.h + h, t < live ? gd : 0.f, a.dt_bf16);
-      }
-      g_rate = lane::lanes_sum(g_rate);
-      g_bias = lane::lanes_sum(g_bias);
-      if (ln == 0) {
-        float* out = a.rows + (rec * a.b + b) * 3 * a.h + h;
-        out[0] = g_rate;
-        out[a.h] = skip_sum;
-        out[2 * a.h] = g_bias;
-      }
+      to.whole[rec * kWaves + wave] = whole;
+      to.skip[rec * kWaves + wave] = gx;
     }
   }
+  const int ln = threadIdx.x % kWave, g = ln / 32, own = block * kTile + ln % 32;
   if (t0 + own >= a.t) return;
   const int64_t at = ((b * a.t + t0 + own) * a.g + grp) * a.n, all = a.b * a.t * a.g * a.n;
+  float* partial = a.gparts + (2 * part + AS_I) * all + at;
+  T* whole = static_cast<T*>(AS_I ? a.gcq : a.gbk) + at;
 #pragma unroll
-  for (int n = 0; n < NP / 16; ++n)
+  for (int n = 0; n < NP / kTile; ++n)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t c = 16 * n + 4 * g + r;
+    for (int r = 0; r < 16; r += 4) {
+      const int c = n * kTile + result_row(r, g);
       if (c >= a.n) continue;
-      if (parts == 1) {
-        static_cast<T*>(a.gbk)[at + c] = lane::narrow<T>(gk[n][r]);
-        static_cast<T*>(a.gcq)[at + c] = lane::narrow<T>(gq[n][r]);
-      } else {
-        a.gparts[(2 * part) * all + at + c] = gk[n][r];
-        a.gparts[(2 * part + 1) * all + at + c] = gq[n][r];
+      if (parts > 1 && a.n % 4 == 0) {
+        *reinterpret_cast<v4f*>(partial + c) = v4f{acc[n][r], acc[n][r + 1], acc[n][r + 2], acc[n][r + 3]};
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (c + e >= a.n) break;
+        if (parts > 1) partial[c + e] = acc[n][r + e];
+        else whole[c + e] = lane::narrow<T>(acc[n][r + e]);
       }
     }
+}
+
+template <typename T, int NP, bool FAST>
+__global__ __launch_bounds__(Sizes<T>::kThreads) void backward_kernel(SelectArgs a, int64_t parts) {
+  __shared__ Tiles<T, NP> t;
+  if (wave_index() >= Sizes<T>::kBlocks) backward_wave<T, NP, FAST, true>(a, parts, t);
+  else backward_wave<T, NP, FAST, false>(a, parts, t);
+}
+
+// A wave closes the token sums of a record and head: gradients of dt, and the
+// record's part of those of A, D and dt_bias.
+__global__ __launch_bounds__(256) void tokens_kernel(SelectArgs a, int record, int waves) {
+  const int ln = threadIdx.x % kWave;
+  const int64_t records = (a.t + record - 1) / record;
+  int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+  if (i >= a.b * records * a.h) return;
+  const int64_t h = i % a.h, rec = i / a.h % records, b = i / a.h / records, t0 = rec * record;
+  const int64_t live = row_length(a, b) - t0;
+  const float rate = a.rate[h], bias = a.dt_bias == nullptr ? 0.f : a.dt_bias[h];
+  const Steps s(a, b, h);
+  const TokenSums from(a, b, h, records, waves);
+  const int per = record / kWave;  // tokens a lane, 1 or 2
+  float f[2], e[2], direct[2], diagonal[2], d[2], slope[2];
+  float f_sum = 0.f, e_sum = 0.f;
+  for (int k = 0; k < per; ++k) {
+    const int64_t t = t0 + per * ln + k;
+    d[k] = s.step[t];
+    direct[k] = from.direct[t];
+    diagonal[k] = from.diagonal[t];
+    const float c = from.earlier[t];
+    f[k] = from.later[t] - d[k] * direct[k];
+    e[k] = d[k] * c;
+    direct[k] += diagonal[k] + c;
+    slope[k] = 1.f;
+    if (per * ln + k < live && a.softplus)
+      slope[k] = lane::softplus_slope_(lane::param(a.dt, b * a.dt_batch + t * a.dt_row + h, a.dt_bf16) + bias);
+    f_sum += f[k];
+    e_sum += e[k];
+  }
+  float whole = 0.f, skip = 0.f;
+  if (ln < waves) {
+    whole = from.whole[rec * waves + ln];
+    skip = from.skip[rec * waves + ln];
+  }
+  const int64_t last = (t0 + record - 1) / kNear;
+  whole = lane::lanes_sum(whole) *
+          lane::exp2_(static_cast<float>(s.base[last] - s.base[t0 / kNear] + s.near[t0 + record - 1]));
+  skip = lane::lanes_sum(skip);
+  const float f_up = lanes_prefix(f_sum);
+  float later = __shfl(f_up, kWave - 1, kWave) - f_up + f_sum, earlier = lanes_prefix(e_sum) - e_sum;
+  float g_rate = 0.f, g_bias = 0.f;
+  for (int k = 0; k < per; ++k) {
+    const int64_t t = t0 + per * ln + k;
+    const float ga = later + earlier + whole;
+    later -= f[k];
+    earlier += e[k];
+    const float gd = per * ln + k < live ? fmaf(rate, ga, direct[k]) * slope[k] : 0.f;
+    g_rate = fmaf(d[k], ga, g_rate);
+    g_bias += gd;
+    if (t < a.t) lane::put_param(a.gdt, (b * a.t + t) * a.h + h, gd, a.dt_bf16);
+  }
+  g_rate = lane::lanes_sum(g_rate);
+  g_bias = lane::lanes_sum(g_bias);
+  if (ln == 0) {
+    float* out = a.rows + (rec * a.b + b) * 3 * a.h + h;
+    out[0] = g_rate;
+    out[a.h] = skip;
+    out[2 * a.h] = g_bias;
+  }
 }
 
 // Gradients of B and C: their sums over the parts of a group's heads.
@@ -381,17 +514,19 @@ __global__ __launch_bounds__(256) void heads_kernel(SelectArgs a, int64_t rows) 
   });
 }
 
-template <typename T>
-hipError_t sizes(const SelectArgs& a, hipStream_t stream) {
-  constexpr int L = Sizes<T>::kL;
-  const int64_t records = (a.t + L - 1) / L, parts = select_parts(a);
-  const dim3 grid(static_cast<unsigned>(a.b * a.g * records * parts)), block(Sizes<T>::kThreads);
+template <typename T, bool FAST>
+hipError_t launch(const SelectArgs& a, hipStream_t stream) {
+  using Z = Sizes<T>;
+  const int64_t records = (a.t + Z::kL - 1) / Z::kL, parts = select_parts(a);
+  const dim3 grid(static_cast<unsigned>(a.b * a.g * records * parts)), block(Z::kThreads);
   if (records > 0 && a.b > 0) {
     if (hipError_t e = launch_adjoints(a, stream); e != hipSuccess) return e;
-    if (a.n <= 32) hipLaunchKernelGGL((backward_kernel<T, 32>), grid, block, 0, stream, a, parts);
-    else if (a.n <= 64) hipLaunchKernelGGL((backward_kernel<T, 64>), grid, block, 0, stream, a, parts);
-    else hipLaunchKernelGGL((backward_kernel<T, 128>), grid, block, 0, stream, a, parts);
+    if (a.n <= 32) hipLaunchKernelGGL((backward_kernel<T, 32, FAST>), grid, block, 0, stream, a, parts);
+    else if (a.n <= 64) hipLaunchKernelGGL((backward_kernel<T, 64, FAST>), grid, block, 0, stream, a, parts);
+    else hipLaunchKernelGGL((backward_kernel<T, 128, FAST>), grid, block, 0, stream, a, parts);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    hipLaunchKernelGGL(tokens_kernel, dim3(static_cast<unsigned>((a.b * a.h * records + 3) / 4)), dim3(256), 0, stream, a,
+                       Z::kL, Z::kThreads / kWave);
     if (parts > 1) {
       const int64_t all = 2 * a.b * a.t * a.g * a.n;
       hipLaunchKernelGGL(parts_kernel<T>, dim3(static_cast<unsigned>((all + 255) / 256)), dim3(256), 0, stream, a, parts);
@@ -413,9 +548,16 @@ int64_t select_parts(const SelectArgs& a) {
   return want < most ? want : most;
 }
 
+// Four sums a token, two of a record's waves (at most 8 of them).
+int64_t select_token_floats(const SelectArgs& a) {
+  const int64_t tp = (a.t + select_scan::kSpan - 1) / select_scan::kSpan * select_scan::kSpan, record = select_record(a.bf16);
+  return a.b * a.h * (4 * tp + 2 * 8 * ((a.t + record - 1) / record));
+}
+
 hipError_t launch_select_backward(const SelectArgs& a, hipStream_t stream) {
   if (a.h == 0) return hipSuccess;
-  return a.bf16 ? select_scan::sizes<__bf16>(a, stream) : select_scan::sizes<float>(a, stream);
+  if (select_fast(a)) return a.bf16 ? select_scan::launch<__bf16, true>(a, stream) : select_scan::launch<float, true>(a, stream);
+  return a.bf16 ? select_scan::launch<__bf16, false>(a, stream) : select_scan::launch<float, false>(a, stream);
 }
 
 }  // namespace bssm

@@ -12,118 +12,202 @@
 // differences inside a chunk, never products of exponentials that leave the
 // range.
 //
-// A workgroup (4 waves) owns one (sequence, head, 64 values of P) and walks
-// its chunks with the state in registers: x, B, C are read once and y is
-// written once.  Where there are too few of those for the chip the time axis
-// is split into segments: a pass without outputs gives each segment's state
-// from zero, and the full pass of a segment starts from the earlier ones'.
-// A wave's part: 16 tokens of the outputs, 16 values of P of the state.
+// A workgroup (8 waves) owns one (sequence, head, 64 values of P) and walks
+// its chunks with the state in registers: x, B, C are read once (the next
+// chunk's while this one is computed) and y is written once.  Four waves form
+// the outputs, 32 tokens x 32 values each, and four move the state on, 32
+// values x half of N each: both need only the chunk's tiles and the state
+// before it, so a SIMD has one of either kind.  Where there are too few
+// workgroups for the chip the time axis is split into segments: a pass without
+// outputs gives each segment's state from zero, and the full pass of a segment
+// starts from the earlier ones'.
 //
 // Rounding with bfloat16 streams: the chunk's weights exp(s_i - s_j) (C.B) d
 // and h0 enter y's products as bfloat16 (y is rounded to it anyway, and their
-// errors are of that size); the state, which is a float32 result, takes its
-// weighted values in three bfloat16 parts, which is all of their bits (two left
-// errors of 2e-6 in the state).  Sums are float32.
+// errors are of that size); the state, which is a float32 result, takes the
+// weighted values exp(s_64 - s_j) d_j x_j in three bfloat16 parts, which is all
+// of their bits; they are made once, on x's way into LDS.  Sums are float32.
 #include "bssm_select.h"
+
+#include <initializer_list>
 
 namespace bssm {
 namespace select_scan {
 namespace {
 
 constexpr int kChunk = kSelectChunk;
-constexpr int kThreads = 256;
-constexpr int kTileP = 64;
+constexpr int kThreads = 512;       // of the full pass
+constexpr int kCarryThreads = 256;  // of the state's passes
 constexpr int kRecordsB16 = 128, kRecordsF32 = 64;  // tokens between two kept states
 
-__device__ __forceinline__ bool pieces16(const SelectArgs& a) {
-  const int n = a.bf16 ? 8 : 4;
-  return a.p % n == 0 && a.x_batch % n == 0 && a.x_row % n == 0 && a.x_head % n == 0 &&
-         (reinterpret_cast<uintptr_t>(a.x) & 15u) == 0;
-}
-__device__ __forceinline__ bool pieces16(const void* p, int64_t b, int64_t r, int64_t g, int64_t n, int bf16) {
-  const int k = bf16 ? 8 : 4;
-  return n % k == 0 && b % k == 0 && r % k == 0 && g % k == 0 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
+// Steps and running sums of every token: a wave takes kSpan tokens of a head, two a lane.
+__global__ __launch_bounds__(256) void steps_kernel(SelectArgs a) {
+  const int ln = threadIdx.x % kWave;
+  const int64_t spans = (a.t + kSpan - 1) / kSpan;
+  int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+  if (i >= a.b * spans * a.h) return;
+  const int64_t h = i % a.h, b = i / a.h / spans, t0 = i / a.h % spans * kSpan, n = row_length(a, b);
+  const float rate2 = a.rate[h] * lane::kLog2e, bias = a.dt_bias == nullptr ? 0.f : a.dt_bias[h];
+  float d[2];
+  double log2_fade[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int64_t t = t0 + 2 * ln + e;
+    d[e] = 0.f;
+    if (t < n) {
+      const float v = lane::param(a.dt, b * a.dt_batch + t * a.dt_row + h, a.dt_bf16) + bias;
+      d[e] = a.softplus ? lane::softplus_(v) : v;
+    }
+    log2_fade[e] = d[e] * rate2;
+  }
+  const double before = lanes_prefix(log2_fade[0] + log2_fade[1]) - (log2_fade[0] + log2_fade[1]);
+  const double start = __shfl(before, ln / 8 * 8, kWave);
+  const Steps s(a, b, h);
+  const int64_t at = t0 + 2 * ln;
+  if (ln % 8 == 0) const_cast<double*>(s.base)[at / kNear] = before;
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  const float n0 = static_cast<float>(before - start + log2_fade[0]);
+  *reinterpret_cast<v2f*>(const_cast<float*>(s.step) + at) = v2f{d[0], d[1]};
+  *reinterpret_cast<v2f*>(const_cast<float*>(s.near) + at) =
+      v2f{n0, static_cast<float>(before - start + log2_fade[0] + log2_fade[1])};
 }
 
-// A wave's 16 values of P of a state, transposed: tile i holds n = 16 i + 4 g + r, p = first + l % 16.
+// The part of the state that one of four waves carries, transposed: tile m holds, of the
+// wave's 32 values of P (column l % 32), the states 32 (wave % 2 + 2 m) on.
 template <int NP>
 struct State {
-  v4f v[NP / 16];
-  __device__ __forceinline__ void clear() {
+  static constexpr int kTiles = NP <= kTile ? 1 : NP / kTile / 2;
+  v16f v[kTiles];
+  int n_first, p, g;
+  bool any;  // with 32 states the odd waves carry none
+  __device__ __forceinline__ explicit State(int wave) {
+    const int ln = threadIdx.x % kWave;
+    n_first = wave % 2 * kTile;
+    p = wave / 2 * kTile + ln % 32;
+    g = ln / 32;
+    any = n_first < NP;
 #pragma unroll
-    for (int i = 0; i < NP / 16; ++i) v[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int m = 0; m < kTiles; ++m) v[m] = zeros();
   }
-  // fn(element of the tile, pointer to 4 of memory, how many of the 4 exist)
+  static constexpr int kStride = 2 * kTile;  // between a wave's tiles
+  // fn(tile, first element, state of that): 4 consecutive states each.
   template <typename Fn>
-  __device__ __forceinline__ void each(int64_t p, int64_t np, int64_t n, int g, Fn fn) {
-    if (p >= np) return;
+  __device__ __forceinline__ void each(Fn fn) {
+    if (!any) return;
 #pragma unroll
-    for (int i = 0; i < NP / 16; ++i) {
-      const int64_t c = 16 * i + 4 * g;
-      if (c < n) fn(v[i], p * n + c, n - c < 4 ? static_cast<int>(n - c) : 4);
-    }
+    for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) fn(v[m], r, n_first + m * kStride + result_row(r, g));
   }
-  __device__ __forceinline__ void add(const float* src, float scale, int64_t p, int64_t np, int64_t n, int g) {
+  __device__ __forceinline__ void scale(float x) {
 #pragma unroll
-    for (int i = 0; i < NP / 16; ++i) v[i] *= scale;
+    for (int m = 0; m < kTiles; ++m) v[m] *= x;
+  }
+  // One [P, N] state of memory, P from p0 on.
+  template <bool FAST>
+  __device__ __forceinline__ void add(const float* src, int64_t p0, int64_t np, int64_t n) {
     if (src == nullptr) return;
-    each(p, np, n, g, [&](v4f& t, int64_t at, int k) {
-      if (k == 4 && n % 4 == 0) {
-        t += *reinterpret_cast<const v4f*>(src + at);
+    src += p0 * n;
+    const Window w = window(src, (np - p0 < kTileP ? np - p0 : kTileP) * n * 4);
+    each([&](v16f& t, int r, int c) {
+      if constexpr (FAST) {
+        const v4f o = load16(w, c < n ? static_cast<uint32_t>(p * n + c) * 4u : kPast);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[r + e] += o[e];
       } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (r < k) t[r] += src[at + r];
+        for (int e = 0; e < 4; ++e)
+          if (p0 + p < np && c + e < n) t[r + e] += src[p * n + c + e];
       }
     });
   }
-  __device__ __forceinline__ void store(float* dst, int64_t p, int64_t np, int64_t n, int g) {
-    each(p, np, n, g, [&](v4f& t, int64_t at, int k) {
-      if (k == 4 && n % 4 == 0) {
-        *reinterpret_cast<v4f*>(dst + at) = t;
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (r < k) dst[at + r] = t[r];
-      }
+  template <bool FAST>
+  __device__ __forceinline__ void store(float* dst, int64_t p0, int64_t np, int64_t n) {
+    dst += p0 * n;
+    const Window w = window(dst, (np - p0 < kTileP ? np - p0 : kTileP) * n * 4);
+    each([&](v16f& t, int r, int c) {
+      put4<FAST>(w, dst, p, n, c, n, p0 + p < np, Pack<float, 4>{{t[r], t[r + 1], t[r + 2], t[r + 3]}});
     });
+  }
+  template <typename T>
+  __device__ __forceinline__ void to_lds(T* lds) {
+    each([&](v16f& t, int r, int c) {
+      Pack<T, 4> o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o.v[e] = lane::narrow<T>(t[r + e]);
+      lane::store_pack<T, 4>(lds + Lds<T, NP>::at(p, c), o);
+    });
+  }
+  // state = fade * state + sum_j k_j (w_j u_j)^T over the chunk's tokens j, w_j u_j in parts.
+  template <typename T>
+  __device__ __forceinline__ void advance(const T (*wu)[kChunk * kTileP], const T* ks, float fade, int wave) {
+    if (!any) return;
+    const int ln = anew(threadIdx.x % kWave), p_first = wave / 2 * kTile;
+    scale(fade);
+#pragma unroll
+    for (int k0 = 0; k0 < kChunk; k0 += kDepth) {
+      Operand<T> u[kParts<T>];
+#pragma unroll
+      for (int i = 0; i < kParts<T>; ++i) u[i] = across<true, kTileP>(wu[i], k0, p_first, ln);
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) {
+        const Operand<T> k = across<true, NP>(ks, k0, n_first + m * kStride, ln);
+#pragma unroll
+        for (int i = 0; i < kParts<T>; ++i) mma(v[m], k, u[i]);
+      }
+    }
   }
 };
 
-// Wave 0: step d and running sums of d A (base 2) of a chunk's tokens, and the weight that a token has in the state
-// that the chunk leaves (BACK: in the adjoint before it).  Tokens from `live` on have d = 0.
-template <bool BACK>
-__device__ __forceinline__ void chunk_steps(const SelectArgs& a, int64_t b, int64_t t0, int64_t h, int64_t live,
-                                            float rate2, float* step, Sums<kChunk>& sums, float* weight, float* fade) {
-  const int ln = threadIdx.x;
-  float slope, d = 0.f;
-  if (ln < live) d = time_step(a, b, t0 + ln, h, slope);
-  const float log2_fade[1] = {d * rate2};
-  sums.fill<1>(log2_fade);
-  if (step != nullptr) step[ln] = d;
-  const double own = sums.at(ln), all = __shfl(own, kChunk - 1, kWave);
-  weight[ln] = BACK ? lane::exp2_(static_cast<float>(own)) : d * lane::exp2_(static_cast<float>(all - own));
-  if (ln == 0) *fade = static_cast<float>(all);
-}
-
-// state = fade * state + sum_j k_j (w_j u_j)^T over the chunk's tokens j.
-template <typename T, int NP>
-__device__ __forceinline__ void advance(State<NP>& st, const T* us, const T* ks, const float* weight, float fade,
-                                        int p_first, int ln) {
-  const int g = ln / 16;
+// The steps and sums of one chunk.  until[j]: step times the decay from token j to the end of its 32 tokens.
+struct ChunkSteps {
+  float step[kChunk], near[kChunk], until[kChunk];
+  double base[kChunk / kNear];
+};
+// A thread's share of them between memory and LDS: the tokens that are its rows of the stream.
+template <typename ROWS>
+struct ChunkLoad {
+  static constexpr int kPieces = ROWS::kPieces;
+  float step[kPieces], near[kPieces], near_end, near_half;
+  double base[kPieces], first, half, last;
+  __device__ __forceinline__ void load(const Steps& s, int64_t t0) {
+    const int thread = anew(threadIdx.x);
 #pragma unroll
-  for (int i = 0; i < NP / 16; ++i) st.v[i] *= fade;
-#pragma unroll
-  for (int kk = 0; kk < kChunk / 32; ++kk) {
-    const Operand<T> u = across<true>(us + kk * 32 * pitch<T>(kTileP) + p_first, pitch<T>(kTileP), ln);
-    Computed<T, 3> wu;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) wu.set(e, u.get(e) * weight[kk * 32 + (e < 4 ? 4 * g + e : 12 + 4 * g + e)]);
-#pragma unroll
-    for (int i = 0; i < NP / 16; ++i)
-      mma(st.v[i], across<true>(ks + kk * 32 * pitch<T>(NP) + 16 * i, pitch<T>(NP), ln), wu);
+    for (int i = 0; i < kPieces; ++i) {
+      const int r = ROWS::row(i, thread);
+      step[i] = s.step[t0 + r];
+      near[i] = s.near[t0 + r];
+      base[i] = s.base[t0 / kNear + r / kNear];
+    }
+    first = s.base[t0 / kNear];
+    half = s.base[t0 / kNear + kTile / kNear - 1];
+    last = s.base[t0 / kNear + kChunk / kNear - 1];
+    near_half = s.near[t0 + kTile - 1];
+    near_end = s.near[t0 + kChunk - 1];
   }
-}
+  // log2 of the whole chunk's decay
+  __device__ __forceinline__ float fade() const { return static_cast<float>(last - first + near_end); }
+  // Weight of the rows in the state that the chunk leaves (BACK: in the adjoint before it).
+  template <bool BACK>
+  __device__ __forceinline__ void weights(float (&w)[kPieces]) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      w[i] = BACK ? lane::exp2_(static_cast<float>(base[i] - first + near[i]))
+                  : step[i] * lane::exp2_(static_cast<float>(last + near_end - base[i] - near[i]));
+  }
+  __device__ __forceinline__ void store(ChunkSteps& o) const {
+    const int thread = anew(threadIdx.x);
+    if (thread % ROWS::kCols != 0) return;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int r = ROWS::row(i, thread);
+      o.step[r] = step[i];
+      o.near[r] = near[i];
+      o.until[r] = step[i] * lane::exp2_(static_cast<float>((r < kTile ? half + near_half : last + near_end) - base[i] - near[i]));
+      if (r % kNear == 0) o.base[r / kNear] = base[i];
+    }
+  }
+};
 
 struct Block {
   int64_t b, h, p0, seg, first, last;  // chunks [first, last)
@@ -152,101 +236,132 @@ __device__ __forceinline__ float* segment_fade(const SelectArgs& a, int64_t segs
   return a.segments + segs * a.b * a.h * a.p * a.n + (seg * a.b + b) * a.h + h;
 }
 
-template <typename T, int NP>
+template <typename T, int NP, bool FAST>
 __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t segs) {
-  __shared__ __align__(16) T xs[kChunk * pitch<T>(kTileP)], ks[kChunk * pitch<T>(NP)], qs[kChunk * pitch<T>(NP)],
-      hs[kTileP * pitch<T>(NP)];
-  __shared__ __align__(16) float step[kChunk], left[kChunk];
-  __shared__ Sums<kChunk> sums;
-  __shared__ float log2_fade;
+  __shared__ __align__(16) T xs[kChunk * kTileP], wx[kParts<T>][kChunk * kTileP], ks[kChunk * NP], qs[kChunk * NP],
+      hs[kTileP * NP];
+  __shared__ __align__(16) ChunkSteps cs;
   const Block at(a, segs);
-  const int wave = threadIdx.x / kWave, ln = threadIdx.x % kWave, g = ln / 16, own = wave * 16 + ln % 16;
+  const int wave = wave_index() % 4, ib = wave % 2, pb = wave / 2;
+  const bool carries = wave_index() >= 4;
   const int64_t grp = at.h / (a.h / a.g), n_live = row_length(a, at.b), bh = at.b * a.h + at.h;
   const T* x = static_cast<const T*>(a.x) + at.b * a.x_batch + at.h * a.x_head;
   const T* bk = static_cast<const T*>(a.bk) + at.b * a.bk_batch + grp * a.bk_group;
   const T* cq = static_cast<const T*>(a.cq) + at.b * a.cq_batch + grp * a.cq_group;
-  const bool vx = pieces16(a), vb = pieces16(a.bk, a.bk_batch, a.bk_row, a.bk_group, a.n, a.bf16),
-             vc = pieces16(a.cq, a.cq_batch, a.cq_row, a.cq_group, a.n, a.bf16);
-  const float rate2 = a.rate[at.h] * lane::kLog2e, skip = a.skip == nullptr ? 0.f : a.skip[at.h];
-  const int64_t p = at.p0 + own, pn = a.p * a.n;
+  const float skip = a.skip == nullptr ? 0.f : a.skip[at.h];
+  const int64_t pn = a.p * a.n;
   const int64_t record = sizeof(T) == 2 ? kRecordsB16 : kRecordsF32, ratio = record / kChunk,
                 records = (a.t + record - 1) / record;
-  State<NP> st;
-  st.clear();
-  st.add(a.state0 == nullptr ? nullptr : a.state0 + bh * pn, 1.f, p, a.p, a.n, g);
-  for (int64_t s = 0; s < at.seg; ++s)
-    st.add(segment_state(a, s, at.b, at.h), *segment_fade(a, segs, s, at.b, at.h), p, a.p, a.n, g);
+  const Steps steps(a, at.b, at.h);
+  State<NP> st(wave);
+  if (carries) {
+    st.template add<FAST>(a.state0 == nullptr ? nullptr : a.state0 + bh * pn, at.p0, a.p, a.n);
+    for (int64_t s = 0; s < at.seg; ++s) {
+      st.scale(*segment_fade(a, segs, s, at.b, at.h));
+      st.template add<FAST>(segment_state(a, s, at.b, at.h), at.p0, a.p, a.n);
+    }
+  }
+  typedef Rows<T, kChunk, kTileP, kThreads> RowsX;
+  RowsX rx;
+  Rows<T, kChunk, NP, kThreads> rk, rq;
+  ChunkLoad<RowsX> rs;
+  auto load = [&](int64_t c) {
+    const int64_t t0 = c * kChunk, live = n_live - t0;
+    rx.template load<FAST>(x + t0 * a.x_row, a.x_row, live, at.p0, a.p);
+    rk.template load<FAST>(bk + t0 * a.bk_row, a.bk_row, live, 0, a.n);
+    rq.template load<FAST>(cq + t0 * a.cq_row, a.cq_row, live, 0, a.n);
+    rs.load(steps, t0);
+  };
+  if (at.first < at.last) load(at.first);
   for (int64_t c = at.first; c < at.last; ++c) {
     const int64_t t0 = c * kChunk, live = n_live - t0;
-    if (a.states != nullptr && c % ratio == 0)
-      st.store(a.states + (bh * records + c / ratio) * pn, p, a.p, a.n, g);
+    if (carries && a.states != nullptr && c % ratio == 0)
+      st.template store<FAST>(a.states + (bh * records + c / ratio) * pn, at.p0, a.p, a.n);
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NP / 16; ++i) {
-      Pack<T, 4> o;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o.v[r] = lane::narrow<T>(st.v[i][r]);
-      lane::store_pack<T, 4>(hs + own * pitch<T>(NP) + 16 * i + 4 * g, o);
-    }
-    stage<kChunk, kTileP, kThreads>(xs, x + t0 * a.x_row, a.x_row, live, at.p0, a.p, vx);
-    stage<kChunk, NP, kThreads>(ks, bk + t0 * a.bk_row, a.bk_row, live, 0, a.n, vb);
-    stage<kChunk, NP, kThreads>(qs, cq + t0 * a.cq_row, a.cq_row, live, 0, a.n, vc);
-    if (wave == 0) chunk_steps<false>(a, at.b, t0, at.h, live, rate2, step, sums, left, &log2_fade);
+    if (carries) st.to_lds(hs);
+    float weight[RowsX::kPieces];
+    rs.template weights<false>(weight);
+    rx.store(xs);
+    rx.store_weighted(wx, weight);
+    rk.store(ks);
+    rq.store(qs);
+    rs.store(cs);
+    const float fade = rs.fade();
     __syncthreads();
-    // Outputs of the wave's 16 tokens, transposed: rows p, column own.
-    Operand<T> q[NP / 32];
-#pragma unroll
-    for (int k = 0; k < NP / 32; ++k) q[k] = along(qs + own * pitch<T>(NP) + 32 * k, g);
-    const float s_own = sums.near[own], since = lane::exp2_(static_cast<float>(sums.at(own)));
-    v4f y[kTileP / 16];
-#pragma unroll
-    for (int i = 0; i < kTileP / 16; ++i) {
-      y[i] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < NP / 32; ++k) mma(y[i], along(hs + (16 * i + ln % 16) * pitch<T>(NP) + 32 * k, g), q[k]);
-      y[i] *= since;
+    if (c + 1 < at.last) load(c + 1);
+    if (carries) {
+      st.advance(wx, ks, lane::exp2_(fade), wave);
+      continue;
     }
-    for (int kk = 0; kk <= wave / 2; ++kk) {
-      Computed<T, 1> m;
+    const int ln = anew(threadIdx.x % kWave), g = ln / 32, own = ib * kTile + ln % 32;
+    // Outputs, transposed: rows p, column own.
+    Operand<T> q[NP / kDepth];
+#pragma unroll
+    for (int k = 0; k < NP / kDepth; ++k) q[k] = along<NP>(qs, own, k * kDepth, g);
+    v16f y = zeros();
+#pragma unroll
+    for (int k = 0; k < NP / kDepth; ++k) mma(y, along<NP>(hs, pb * kTile + ln % 32, k * kDepth, g), q[k]);
+    const double base_own = cs.base[own / kNear];
+    const float near_own = cs.near[own];
+    y *= lane::exp2_(static_cast<float>(base_own - cs.base[0] + near_own));
+    if (ib == 1) {  // the tokens of the block before: the decay is one to that block's end and one from there
+      v16f dot = zeros();
+#pragma unroll
+      for (int k = 0; k < NP / kDepth; ++k) mma(dot, along<NP>(ks, ln % 32, k * kDepth, g), q[k]);
+      const float from = lane::exp2_(static_cast<float>(base_own - cs.base[kTile / kNear - 1]) + (near_own - cs.near[kTile - 1]));
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int j0 = kk * 32 + half * 16;
-        v4f dot = {0.f, 0.f, 0.f, 0.f};
-        if (j0 <= wave * 16)
+        Operand<T> m;
 #pragma unroll
-          for (int k = 0; k < NP / 32; ++k) mma(dot, along(ks + (j0 + ln % 16) * pitch<T>(NP) + 32 * k, g), q[k]);
-        const float from = s_own + sums.between(wave, j0 / 16);
-        const v4f sj = *reinterpret_cast<const v4f*>(sums.near + j0 + 4 * g), dj = *reinterpret_cast<const v4f*>(step + j0 + 4 * g);
+        for (int q4 = 0; q4 < 2; ++q4) {
+          const v4f uj = *reinterpret_cast<const v4f*>(cs.until + half * kDepth + 8 * q4 + 4 * g);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          m.set(half * 4 + r, j0 + 4 * g + r <= own ? dot[r] * lane::exp2_(from - sj[r]) * dj[r] : 0.f);
-      }
-#pragma unroll
-      for (int i = 0; i < kTileP / 16; ++i)
-        mma(y[i], across<true>(xs + kk * 32 * pitch<T>(kTileP) + 16 * i, pitch<T>(kTileP), ln), m);
-    }
-    const int64_t t = t0 + own;
-    if (t < a.t) {
-      T* out = static_cast<T*>(a.y) + ((at.b * a.t + t) * a.h + at.h) * a.p + at.p0;
-#pragma unroll
-      for (int i = 0; i < kTileP / 16; ++i) {
-        const int c0 = 16 * i + 4 * g;
-        const Pack<T, 4> xi = lane::load_pack<T, 4>(xs + own * pitch<T>(kTileP) + c0);
-        Pack<T, 4> o;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o.v[r] = lane::narrow<T>(own < live ? fmaf(skip, lane::widen(xi.v[r]), y[i][r]) : 0.f);
-        if (at.p0 + c0 + 4 <= a.p && a.p % 4 == 0) {
-          lane::store_pack<T, 4>(out + c0, o);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (at.p0 + c0 + r < a.p) out[c0 + r] = o.v[r];
+          for (int e = 0; e < 4; ++e) m.set(4 * q4 + e, dot[8 * half + 4 * q4 + e] * (from * uj[e]));
         }
+        mma(y, across<true, kTileP>(xs, half * kDepth, pb * kTile, ln), m);
       }
     }
-    advance<T, NP>(st, xs, ks, left, lane::exp2_(log2_fade), wave * 16, ln);
+    {
+      v16f dot = zeros();
+#pragma unroll
+      for (int k = 0; k < NP / kDepth; ++k) mma(dot, along<NP>(ks, ib * kTile + ln % 32, k * kDepth, g), q[k]);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int j0 = ib * kTile + half * kDepth;
+        const float from = near_own + static_cast<float>(base_own - cs.base[j0 / kNear]);
+        Operand<T> m;
+#pragma unroll
+        for (int q4 = 0; q4 < 2; ++q4) {
+          const int j = j0 + 8 * q4 + 4 * g;
+          const v4f sj = *reinterpret_cast<const v4f*>(cs.near + j), dj = *reinterpret_cast<const v4f*>(cs.step + j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // formed for all, then selected: no lane branches
+            const float v = dot[8 * half + 4 * q4 + e] * lane::exp2_(from - sj[e]) * dj[e];
+            m.set(4 * q4 + e, j + e <= own ? v : 0.f);
+          }
+        }
+        mma(y, across<true, kTileP>(xs, j0, pb * kTile, ln), m);
+      }
+    }
+    const int64_t y_row = a.h * a.p, y_rows = a.t - t0 < kChunk ? a.t - t0 : kChunk;
+    T* out = static_cast<T*>(a.y) + (at.b * a.t + t0) * y_row + at.h * a.p + at.p0;
+    const int64_t cols = a.p - at.p0;
+    const Window w = window(out, ((y_rows - 1) * y_row + cols) * sizeof(T));
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int c0 = pb * kTile + result_row(r, g);
+      const Pack<T, 4> xi = lane::load_pack<T, 4>(xs + Lds<T, kTileP>::at(own, c0));
+      Pack<T, 4> o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = fmaf(skip, lane::widen(xi.v[e]), y[r + e]);
+        o.v[e] = lane::narrow<T>(own < live ? v : 0.f);
+      }
+      put4<FAST>(w, out, own, y_row, c0, cols, own < y_rows, o);
+    }
   }
-  if (at.seg == segs - 1 && a.state_out != nullptr) st.store(a.state_out + bh * pn, p, a.p, a.n, g);
+  if (carries && at.seg == segs - 1 && a.state_out != nullptr)
+    st.template store<FAST>(a.state_out + bh * pn, at.p0, a.p, a.n);
 }
 
 // The state alone, along a segment.  Forward (BACK false): from zero, into the
@@ -254,14 +369,11 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t
 //   gh0 = exp(s_64) gh0' + sum_i exp(s_i) C_i gy_i^T;
 // LOCAL: from zero, into the workspace; else from the later segments', keeping
 // the adjoint behind every record's last token and the one before the first.
-template <typename T, int NP, bool BACK, bool LOCAL>
-__global__ __launch_bounds__(kThreads) void carry_kernel(SelectArgs a, int64_t segs) {
-  __shared__ __align__(16) T us[kChunk * pitch<T>(kTileP)], ks[kChunk * pitch<T>(NP)];
-  __shared__ __align__(16) float weight[kChunk];
-  __shared__ Sums<kChunk> sums;
-  __shared__ float log2_fade;
+template <typename T, int NP, bool FAST, bool BACK, bool LOCAL>
+__global__ __launch_bounds__(kCarryThreads, sizeof(T) == 2 ? 2 : 1) void carry_kernel(SelectArgs a, int64_t segs) {
+  __shared__ __align__(16) T wu[kParts<T>][kChunk * kTileP], ks[kChunk * NP];
   const Block at(a, segs);
-  const int wave = threadIdx.x / kWave, ln = threadIdx.x % kWave, g = ln / 16, own = wave * 16 + ln % 16;
+  const int wave = wave_index();
   const int64_t grp = at.h / (a.h / a.g), n_live = row_length(a, at.b), bh = at.b * a.h + at.h;
   const T* u = BACK ? static_cast<const T*>(a.gy) + (at.b * a.t * a.h + at.h) * a.p
                     : static_cast<const T*>(a.x) + at.b * a.x_batch + at.h * a.x_head;
@@ -269,39 +381,52 @@ __global__ __launch_bounds__(kThreads) void carry_kernel(SelectArgs a, int64_t s
   const T* k = BACK ? static_cast<const T*>(a.cq) + at.b * a.cq_batch + grp * a.cq_group
                     : static_cast<const T*>(a.bk) + at.b * a.bk_batch + grp * a.bk_group;
   const int64_t k_row = BACK ? a.cq_row : a.bk_row;
-  const bool vu = BACK ? pieces16(a.gy, a.p, a.p, a.p, a.p, a.bf16) : pieces16(a);
-  const bool vk = BACK ? pieces16(a.cq, a.cq_batch, a.cq_row, a.cq_group, a.n, a.bf16)
-                       : pieces16(a.bk, a.bk_batch, a.bk_row, a.bk_group, a.n, a.bf16);
-  const float rate2 = a.rate[at.h] * lane::kLog2e;
-  const int64_t p = at.p0 + own, pn = a.p * a.n;
+  const int64_t pn = a.p * a.n;
   const int64_t record = sizeof(T) == 2 ? kRecordsB16 : kRecordsF32, ratio = record / kChunk,
                 records = (a.t + record - 1) / record, chunks = (a.t + kChunk - 1) / kChunk;
-  State<NP> st;
-  st.clear();
+  const Steps steps(a, at.b, at.h);
+  State<NP> st(wave);
   float total = 0.f;
   if constexpr (!LOCAL) {
-    st.add(a.gstate_out == nullptr ? nullptr : a.gstate_out + bh * pn, 1.f, p, a.p, a.n, g);
-    for (int64_t s = segs - 1; s > at.seg; --s)
-      st.add(segment_state(a, s, at.b, at.h), *segment_fade(a, segs, s, at.b, at.h), p, a.p, a.n, g);
+    st.template add<FAST>(a.gstate_out == nullptr ? nullptr : a.gstate_out + bh * pn, at.p0, a.p, a.n);
+    for (int64_t s = segs - 1; s > at.seg; --s) {
+      st.scale(*segment_fade(a, segs, s, at.b, at.h));
+      st.template add<FAST>(segment_state(a, s, at.b, at.h), at.p0, a.p, a.n);
+    }
   }
-  for (int64_t i = 0; i < at.last - at.first; ++i) {
-    const int64_t c = BACK ? at.last - 1 - i : at.first + i, t0 = c * kChunk, live = n_live - t0;
+  typedef Rows<T, kChunk, kTileP, kCarryThreads> RowsU;
+  RowsU ru;
+  Rows<T, kChunk, NP, kCarryThreads> rk;
+  ChunkLoad<RowsU> rs;
+  const int64_t count = at.last - at.first;
+  auto chunk = [&](int64_t i) { return BACK ? at.last - 1 - i : at.first + i; };
+  auto load = [&](int64_t c) {
+    const int64_t t0 = c * kChunk, live = n_live - t0;
+    ru.template load<FAST>(u + t0 * u_row, u_row, live, at.p0, a.p);
+    rk.template load<FAST>(k + t0 * k_row, k_row, live, 0, a.n);
+    rs.load(steps, t0);
+  };
+  if (count > 0) load(chunk(0));
+  for (int64_t i = 0; i < count; ++i) {
+    const int64_t c = chunk(i);
     if (!LOCAL && (c % ratio == ratio - 1 || c == chunks - 1))
-      st.store(a.adjoints + (bh * records + c / ratio) * pn, p, a.p, a.n, g);
-    if (live <= 0) continue;  // uniform: the workgroup has one sequence
+      st.template store<FAST>(a.adjoints + (bh * records + c / ratio) * pn, at.p0, a.p, a.n);
     __syncthreads();
-    stage<kChunk, kTileP, kThreads>(us, u + t0 * u_row, u_row, live, at.p0, a.p, vu);
-    stage<kChunk, NP, kThreads>(ks, k + t0 * k_row, k_row, live, 0, a.n, vk);
-    if (wave == 0) chunk_steps<BACK>(a, at.b, t0, at.h, live, rate2, nullptr, sums, weight, &log2_fade);
+    float weight[RowsU::kPieces];
+    rs.template weights<BACK>(weight);
+    ru.store_weighted(wu, weight);
+    rk.store(ks);
+    const float fade = rs.fade();
     __syncthreads();
-    total += log2_fade;
-    advance<T, NP>(st, us, ks, weight, lane::exp2_(log2_fade), wave * 16, ln);
+    if (i + 1 < count) load(chunk(i + 1));
+    total += fade;
+    st.advance(wu, ks, lane::exp2_(fade), wave);
   }
   if constexpr (LOCAL) {
-    st.store(segment_state(a, at.seg, at.b, at.h), p, a.p, a.n, g);
+    st.template store<FAST>(segment_state(a, at.seg, at.b, at.h), at.p0, a.p, a.n);
     if (threadIdx.x == 0 && at.p0 == 0) *segment_fade(a, segs, at.seg, at.b, at.h) = lane::exp2_(total);
   } else if (at.seg == 0 && a.gstate0 != nullptr) {
-    st.store(a.gstate0 + bh * pn, p, a.p, a.n, g);
+    st.template store<FAST>(a.gstate0 + bh * pn, at.p0, a.p, a.n);
   }
 }
 
@@ -309,38 +434,67 @@ unsigned blocks(const SelectArgs& a, int64_t segs) {
   return static_cast<unsigned>(a.b * a.h * ((a.p + kTileP - 1) / kTileP) * segs);
 }
 
-template <typename T, int NP>
-hipError_t forward(const SelectArgs& a, hipStream_t stream) {
+template <typename T, int NP, bool FAST>
+hipError_t launch(const SelectArgs& a, bool back, hipStream_t stream) {
   const int64_t segs = select_segments(a);
-  if (segs > 1) hipLaunchKernelGGL((carry_kernel<T, NP, false, true>), dim3(blocks(a, segs)), dim3(kThreads), 0, stream, a, segs);
-  hipLaunchKernelGGL((forward_kernel<T, NP>), dim3(blocks(a, segs)), dim3(kThreads), 0, stream, a, segs);
-  return hipGetLastError();
-}
-template <typename T, int NP>
-hipError_t reverse(const SelectArgs& a, hipStream_t stream) {
-  const int64_t segs = select_segments(a);
-  if (segs > 1) hipLaunchKernelGGL((carry_kernel<T, NP, true, true>), dim3(blocks(a, segs)), dim3(kThreads), 0, stream, a, segs);
-  hipLaunchKernelGGL((carry_kernel<T, NP, true, false>), dim3(blocks(a, segs)), dim3(kThreads), 0, stream, a, segs);
+  const dim3 grid(blocks(a, segs)), block(kCarryThreads);
+  if (back) {
+    if (segs > 1) hipLaunchKernelGGL((carry_kernel<T, NP, FAST, true, true>), grid, block, 0, stream, a, segs);
+    hipLaunchKernelGGL((carry_kernel<T, NP, FAST, true, false>), grid, block, 0, stream, a, segs);
+    return hipGetLastError();
+  }
+  const int64_t waves = a.b * a.h * ((a.t + kSpan - 1) / kSpan);
+  if (waves > 0) hipLaunchKernelGGL(steps_kernel, dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, stream, a);
+  if (segs > 1) hipLaunchKernelGGL((carry_kernel<T, NP, FAST, false, true>), grid, block, 0, stream, a, segs);
+  hipLaunchKernelGGL((forward_kernel<T, NP, FAST>), grid, dim3(kThreads), 0, stream, a, segs);
   return hipGetLastError();
 }
 
-template <typename T>
+template <typename T, bool FAST>
 hipError_t sizes(const SelectArgs& a, bool back, hipStream_t stream) {
-  if (a.n <= 32) return back ? reverse<T, 32>(a, stream) : forward<T, 32>(a, stream);
-  if (a.n <= 64) return back ? reverse<T, 64>(a, stream) : forward<T, 64>(a, stream);
-  return back ? reverse<T, 128>(a, stream) : forward<T, 128>(a, stream);
+  if (a.n <= 32) return launch<T, 32, FAST>(a, back, stream);
+  if (a.n <= 64) return launch<T, 64, FAST>(a, back, stream);
+  return launch<T, 128, FAST>(a, back, stream);
+}
+hipError_t types(const SelectArgs& a, bool back, hipStream_t stream) {
+  if (select_fast(a)) return a.bf16 ? sizes<__bf16, true>(a, back, stream) : sizes<float, true>(a, back, stream);
+  return a.bf16 ? sizes<__bf16, false>(a, back, stream) : sizes<float, false>(a, back, stream);
 }
 
 }  // namespace
 
 // The reverse pass of the state (called by the backward, bssm_select_bwd.hip).
 hipError_t launch_adjoints(const SelectArgs& a, hipStream_t stream) {
-  return a.bf16 ? sizes<__bf16>(a, true, stream) : sizes<float>(a, true, stream);
+  return types(a, true, stream);
 }
 
 }  // namespace select_scan
 
+// The kernels' fast form moves every stream in 16-byte units through 32-bit
+// offsets of a chunk's or record's rows: P and N whole units, every row on a
+// 16-byte boundary, rows that do not overlap and 128 of them below 2^31 bytes.
+// The other form moves single elements.
+bool select_fast(const SelectArgs& a) {
+  const int64_t unit = a.bf16 ? 8 : 4, size = a.bf16 ? 2 : 4, most = ((int64_t)1 << 31) / (128 * size);
+  if (a.p % unit != 0 || a.n % unit != 0 || a.h * a.p >= most) return false;
+  const int64_t rows[] = {a.x_row, a.bk_row, a.cq_row}, least[] = {a.p, a.n, a.n};
+  for (int i = 0; i < 3; ++i)
+    if (rows[i] < least[i] || rows[i] >= most) return false;
+  for (int64_t s : {a.x_batch, a.x_row, a.x_head, a.bk_batch, a.bk_row, a.bk_group, a.cq_batch, a.cq_row, a.cq_group})
+    if (s % unit != 0) return false;
+  for (const void* p : {a.x, a.bk, a.cq, static_cast<const void*>(a.y), a.gy, static_cast<const void*>(a.gx)})
+    if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) return false;
+  for (const float* p : {a.state0, static_cast<const float*>(a.state_out), a.gstate_out, static_cast<const float*>(a.gstate0)})
+    if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) return false;
+  return a.p * a.n < ((int64_t)1 << 28);
+}
+
 int64_t select_record(int bf16) { return bf16 ? select_scan::kRecordsB16 : select_scan::kRecordsF32; }
+
+int64_t select_step_floats(const SelectArgs& a) {
+  const int64_t tp = (a.t + select_scan::kSpan - 1) / select_scan::kSpan * select_scan::kSpan;
+  return a.b * a.h * (2 * tp + 2 * (tp / select_scan::kNear));
+}
 
 // One segment where the sequences, heads and P tiles alone give every compute
 // unit a workgroup; else two a unit, each of 8 chunks or more: a segment costs
@@ -358,7 +512,7 @@ int64_t select_segment_floats(const SelectArgs& a) {
 
 hipError_t launch_select_forward(const SelectArgs& a, hipStream_t stream) {
   if (a.b * a.h * a.p == 0) return hipSuccess;
-  return a.bf16 ? select_scan::sizes<__bf16>(a, false, stream) : select_scan::sizes<float>(a, false, stream);
+  return select_scan::types(a, false, stream);
 }
 
 }  // namespace bssm

@@ -86,6 +86,7 @@ struct SelectArgs {
   float* state_out;                    // [B, H, P, N] or null
   float* states;                       // [B, H, records, P, N]: state before every record'th token, or null
   float* segments;                     // workspace, see select_segments
+  float* steps;                        // the tokens' steps and their sums: written by the forward, read by the backward
   int64_t b, t, h, p, n, g;
   int bf16, dt_bf16, softplus;
   // Backward.
@@ -96,16 +97,20 @@ struct SelectArgs {
   void *gx, *gdt;                      // contiguous
   void *gbk, *gcq;                     // [B, T, G, N] contiguous
   float* gparts;                       // [parts, 2, B, T, G, N]: gradients of B and C by parts of a group's heads
+  float* token_sums;                   // workspace of select_token_floats
   float* rows;                         // [B * records, 3, H]: gradients of A, D, dt_bias by records
   float *grate, *gskip, *gdt_bias;     // [H]
 };
 // Tokens between two kept states; parts that a group's heads are split into by
 // the backward; segments that the time axis is split into by the passes that
 // carry a state (1: no workspace), and the workspace's floats.
+bool select_fast(const SelectArgs& a);
 int64_t select_record(int bf16);
 int64_t select_parts(const SelectArgs& a);
 int64_t select_segments(const SelectArgs& a);
 int64_t select_segment_floats(const SelectArgs& a);
+int64_t select_step_floats(const SelectArgs& a);
+int64_t select_token_floats(const SelectArgs& a);
 hipError_t launch_select_forward(const SelectArgs& a, hipStream_t stream);
 hipError_t launch_select_backward(const SelectArgs& a, hipStream_t stream);
 

@@ -737,34 +737,38 @@ int bssm_distill_backward(int bf16, int teacher_bf16, const void* logits, int64_
  * Tokens from a row's length on give y = 0 and leave the state.  state_out
  * (NULL: not wanted) receives the last state.  For a backward, states [batch,
  * heads, bssm_select_sizes(0, ...), values, n] keeps states along the way
- * (NULL: none).  segments: workspace of bssm_select_sizes(1, ...) floats (may
- * be NULL for 0). */
+ * (NULL: none).  steps, bssm_select_sizes(3, ...) floats, receives the tokens'
+ * steps and their sums, which a backward reads.  segments: workspace of
+ * bssm_select_sizes(1, ...) floats (may be NULL for 0).  Both on 16-byte
+ * boundaries. */
 int bssm_select_forward(int bf16, const void* x, int64_t x_batch, int64_t x_row, int64_t x_head, int dt_bf16,
                         const void* dt, int64_t dt_batch, int64_t dt_row, const float* rate, const void* b,
                         int64_t b_batch, int64_t b_row, int64_t b_group, const void* c, int64_t c_batch,
                         int64_t c_row, int64_t c_group, const float* skip, const float* dt_bias, int softplus,
                         const int64_t* lengths, const float* state0, void* y, float* state_out, float* states,
-                        float* segments, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t n,
-                        int64_t groups, void* stream);
+                        float* steps, float* segments, int64_t batch, int64_t t, int64_t heads, int64_t values,
+                        int64_t n, int64_t groups, void* stream);
 
-/* Gradients of the above, contiguous, of the inputs' types.  grad_y
- * [batch, t, heads, values] contiguous; grad_state_out may be NULL (zero).
- * Workspaces (float32): adjoints of the size of states; segments as in the
- * forward; parts [bssm_select_sizes(2, ...), 2, batch, t, groups, n] (may be
+/* Gradients of the above, contiguous, of the inputs' types; states and steps
+ * as the forward left them.  grad_y [batch, t, heads, values] contiguous;
+ * grad_state_out may be NULL (zero).  Workspaces (float32): adjoints of the
+ * size of states; segments as in the forward; token_sums of
+ * bssm_select_sizes(4, ...) floats; parts [bssm_select_sizes(2, ...), 2, batch, t, groups, n] (may be
  * NULL where that is 1); rows [batch * bssm_select_sizes(0, ...), 3, heads].
  * grad_rate, grad_skip, grad_dt_bias [heads] and grad_state0 may be NULL. */
 int bssm_select_backward(int bf16, const void* x, int64_t x_batch, int64_t x_row, int64_t x_head, int dt_bf16,
                          const void* dt, int64_t dt_batch, int64_t dt_row, const float* rate, const void* b,
                          int64_t b_batch, int64_t b_row, int64_t b_group, const void* c, int64_t c_batch,
                          int64_t c_row, int64_t c_group, const float* skip, const float* dt_bias, int softplus,
-                         const int64_t* lengths, const float* states, const void* grad_y, const float* grad_state_out,
-                         float* adjoints, float* segments, float* parts, float* rows, void* grad_x, void* grad_dt,
-                         float* grad_rate, void* grad_b, void* grad_c, float* grad_skip, float* grad_dt_bias,
+                         const int64_t* lengths, const float* states, const float* steps, const void* grad_y,
+                         const float* grad_state_out, float* adjoints, float* segments, float* token_sums,
+                         float* parts, float* rows, void* grad_x, void* grad_dt, float* grad_rate, void* grad_b, void* grad_c, float* grad_skip, float* grad_dt_bias,
                          float* grad_state0, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t n,
                          int64_t groups, void* stream);
 
 /* Sizes of the scan's buffers: what = 0 kept states a sequence and head, 1
- * floats of the segments' workspace, 2 parts of the gradients of b and c. */
+ * floats of the segments' workspace, 2 parts of the gradients of b and c, 3
+ * floats of the tokens' steps, 4 floats of the backward's token sums. */
 int64_t bssm_select_sizes(int what, int bf16, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t n,
                           int64_t groups);
 

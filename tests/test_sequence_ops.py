@@ -221,7 +221,7 @@ def test_c_entry_points_refuse():
 
     def scan(h=4, n=8, g=2, b=1):
         return lib.bssm_select_forward(0, None, 0, 0, 0, 0, None, 0, 0, None, None, 0, 0, 0, None, 0, 0, 0, None, None, 1,
-                                       None, None, None, None, None, None, b, 4, h, 8, n, g, None)
+                                       None, None, None, None, None, None, None, b, 4, h, 8, n, g, None)
 
     assert scan(n=129) == 2 and scan(g=3) == 1 and scan(b=-1) == 1 and scan() == 1 and scan(b=0) == 0
     assert b"null" in (scan(), lib.bssm_last_error())[1]
