@@ -78,12 +78,13 @@ _SIGNATURES = {
                                  + [_P] * 2 + [_L, _L, _L, _L, _F, _P],
     "bssm_short_conv_forward": [_I] * 4 + [_P, _L, _L] + [_P] * 6 + [_L] * 3 + [_P],
     "bssm_short_conv_backward": [_I] * 4 + [_P, _L, _L] + [_P] * 11 + [_L] * 3 + [_P],
-    "bssm_short_conv_partial_rows": [_I, _L, _L, _L],
+    "bssm_short_conv_partial_rows": [_L, _L, _L],
     "bssm_layer_norm_forward": [_I, _I, _P, _L, _P, _P, _F] + [_P] * 3 + [_L, _L, _P],
     "bssm_layer_norm_backward": [_I, _I, _P, _L] + [_P] * 8 + [_L, _L, _P],
     "bssm_layer_norm_partial_rows": [_I, _L, _L],
-    "bssm_distill_forward": [_I, _I, _P, _L, _P, _P, _F] + [_P] * 3 + [_L] * 3 + [_P],
-    "bssm_distill_backward": [_I, _I, _P, _L, _P, _P, _F] + [_P] * 3 + [_I, _P] + [_L] * 3 + [_P],
+    "bssm_distill_forward": [_I, _I, _P, _L, _P, _P, _F] + [_P] * 4 + [_I, _P] + [_L] * 3 + [_P],
+    "bssm_distill_count_floats": [],
+    "bssm_distill_backward": [_I, _I, _P, _L, _P, _P, _F] + [_P] * 3 + [_I, _I, _P] + [_L] * 3 + [_P],
     "bssm_select_forward": _SELECT_HEAD + [_P] * 6 + [_L] * 6 + [_P],
     "bssm_select_backward": _SELECT_HEAD + [_P] * 17 + [_L] * 6 + [_P],
     "bssm_select_sizes": [_I, _I] + [_L] * 6,
@@ -127,7 +128,8 @@ def load() -> ctypes.CDLL:
                 fn.restype = ctypes.c_int
             lib.bssm_value_stats_workspace.restype = ctypes.c_int64
             lib.bssm_small_batch_limit.restype = ctypes.c_int64
-            for name in ("bssm_short_conv_partial_rows", "bssm_layer_norm_partial_rows", "bssm_select_sizes"):
+            for name in ("bssm_short_conv_partial_rows", "bssm_layer_norm_partial_rows",
+                         "bssm_distill_count_floats", "bssm_select_sizes"):
                 getattr(lib, name).restype = ctypes.c_int64
             lib.bssm_last_error.argtypes = []
             lib.bssm_last_error.restype = ctypes.c_char_p

@@ -41,33 +41,45 @@ def _formula(logits: Tensor, teacher: Tensor, index: Tensor, tau: float) -> tupl
 
 
 class _DistillFunction(torch.autograd.Function):
+    """Autograd boundary: the forward that holds a row writes its gradient too (for an upstream gradient of 1)."""
+
     @staticmethod
     def forward(ctx, logits, teacher, index, tau, reduction):
         r, v = logits.shape
         k = index.shape[1]
         dev = logits.device
-        loss = torch.empty(r, device=dev, dtype=torch.float32)
-        stats = torch.empty(r, 3, device=dev, dtype=torch.float32)
-        mean = None if reduction == "none" else torch.empty(3, device=dev, dtype=torch.float32)
+
+        def f32(*shape):
+            return torch.empty(*shape, device=dev, dtype=torch.float32)
+
+        loss, stats = f32(r), f32(r, 3)
+        mean = None if reduction == "none" else f32(3)
+        grad = torch.empty(r, v, device=dev, dtype=logits.dtype) if ctx.needs_input_grad[0] else None
+        of_rows = reduction == "mean"
+        counts = f32(_hip.function("bssm_distill_count_floats")()) if of_rows and grad is not None else None
         P = _hip.ptr
         kinds = int(logits.dtype == torch.bfloat16), int(teacher.dtype == torch.bfloat16)
         _hip.launch(dev, "bssm_distill_forward", *kinds, P(logits), logits.stride(0), P(teacher), P(index), tau,
-                    P(loss), P(stats), P(mean), r, v, k, _hip.stream_of(dev))
-        ctx.save_for_backward(logits, teacher, index, stats, mean if reduction == "mean" else None)
-        ctx.tau, ctx.kinds, ctx.scalar = tau, kinds, reduction != "none"
-        return loss if mean is None else mean[0 if reduction == "mean" else 2].clone()
+                    P(loss), P(stats), P(mean), P(grad), int(of_rows), P(counts), r, v, k, _hip.stream_of(dev))
+        if grad is not None:
+            ctx.save_for_backward(logits, teacher, index, stats, mean if of_rows else None)
+            ctx.tau, ctx.kinds, ctx.scalar, ctx.grad = tau, kinds, reduction != "none", grad
+        return loss if mean is None else mean[0 if of_rows else 2].clone()
 
     @staticmethod
-    def backward(ctx, grad):
+    def backward(ctx, upstream):
         logits, teacher, index, stats, mean = ctx.saved_tensors
         r, v = logits.shape
         dev = logits.device
-        out = torch.empty(r, v, device=dev, dtype=logits.dtype)
-        grad = grad.contiguous()
+        upstream = upstream.contiguous()
         P = _hip.ptr
+        out, ctx.grad = ctx.grad, None  # handed out once: a second backward of the same graph computes its own
+        ready = out is not None
+        if not ready:
+            out = torch.empty(r, v, device=dev, dtype=logits.dtype)
         _hip.launch(dev, "bssm_distill_backward", *ctx.kinds, P(logits), logits.stride(0), P(teacher), P(index),
-                    ctx.tau, P(stats), P(mean), P(grad), int(ctx.scalar), P(out), r, v, index.shape[1],
-                    _hip.stream_of(dev))
+                    ctx.tau, P(stats), P(mean), P(upstream), int(ctx.scalar), int(ready), P(out), r, v,
+                    index.shape[1], _hip.stream_of(dev))
         return out, None, None, None, None
 
 

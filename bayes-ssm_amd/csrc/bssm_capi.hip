@@ -1231,6 +1231,7 @@ int short_conv_check(const char* fn, const bssm::ShortConvArgs& a) {
   if (a.w < 2 || a.w > 4) return fail(BSSM_ERR_UNSUPPORTED, "%s: width must be 2, 3 or 4, got %d", fn, a.w);
   if (a.b < 0 || a.t < 0 || a.c < 0) return fail(BSSM_ERR_ARGUMENT, "%s: negative size", fn);
   if (a.t > 1 && a.x_row < a.c) return fail(BSSM_ERR_ARGUMENT, "%s: x rows overlap", fn);
+  if (a.t > (int64_t)1 << 30) return fail(BSSM_ERR_ARGUMENT, "%s: t must be at most 2^30", fn);
   if (int rc = check_size(fn, a.b * (a.t + 1) * a.c)) return rc;
   return check_grid(fn, a.b * a.c * (a.t / 4 + 1) / 64);
 }
@@ -1249,6 +1250,7 @@ int distill_check(const char* fn, const bssm::DistillArgs& a) {
     return fail(BSSM_ERR_UNSUPPORTED, "%s: at most %d teacher entries a row, got %lld", fn, bssm::kDistillMaxTeacher,
                 (long long)a.k);
   if (a.r > 1 && a.logits_row < a.v) return fail(BSSM_ERR_ARGUMENT, "%s: logits rows overlap", fn);
+  if (a.v > (int64_t)1 << 28) return fail(BSSM_ERR_ARGUMENT, "%s: at most 2^28 vocabulary entries", fn);
   if (!(a.tau > 0.f) || !(a.tau < INFINITY)) return fail(BSSM_ERR_ARGUMENT, "%s: temperature must be positive and finite", fn);
   if (int rc = check_size(fn, a.r * a.v)) return rc;
   return check_grid(fn, a.r);
@@ -1285,8 +1287,8 @@ bssm::SelectArgs select_args(int bf16, const void* x, int64_t x_batch, int64_t x
 
 extern "C" {
 
-int64_t bssm_short_conv_partial_rows(int bf16, int64_t batch, int64_t t, int64_t channels) {
-  return bssm::short_conv_partial_rows(batch, t, channels, bf16 != 0);
+int64_t bssm_short_conv_partial_rows(int64_t batch, int64_t t, int64_t channels) {
+  return bssm::short_conv_partial_rows(batch, t, channels);
 }
 
 int bssm_short_conv_forward(int bf16, int param_bf16, int width, int silu, const void* x, int64_t x_batch,
@@ -1364,30 +1366,36 @@ int bssm_layer_norm_backward(int bf16, int param_bf16, const void* x, int64_t x_
 
 int bssm_distill_forward(int bf16, int teacher_bf16, const void* logits, int64_t logits_row, const void* teacher,
                          const int64_t* index, float temperature, float* loss, float* stats, float* mean,
-                         int64_t rows, int64_t vocabulary, int64_t entries, void* stream) {
+                         void* grad_logits, int mean_of_rows, float* counts, int64_t rows, int64_t vocabulary,
+                         int64_t entries, void* stream) {
   const char* fn = "bssm_distill_forward";
   bssm::DistillArgs a{};
   a.logits = logits; a.logits_row = logits_row; a.teacher = teacher; a.index = index; a.tau = temperature;
-  a.loss = loss; a.lse = stats; a.mean = mean; a.r = rows; a.v = vocabulary; a.k = entries;
+  a.loss = loss; a.stats = stats; a.mean = mean; a.grad = grad_logits; a.counts = counts;
+  a.mean_of_rows = mean_of_rows != 0; a.r = rows; a.v = vocabulary; a.k = entries;
   a.bf16 = bf16 != 0; a.teacher_bf16 = teacher_bf16 != 0;
   if (int rc = distill_check(fn, a)) return rc;
   if (rows > 0) {
     if (int rc = need(fn, {{logits, "logits"}, {loss, "loss"}, {stats, "stats"}})) return rc;
+    if (grad_logits != nullptr && mean_of_rows && counts == nullptr)
+      return fail(BSSM_ERR_ARGUMENT, "%s: the mean's gradient needs counts", fn);
     if (entries > 0)
       if (int rc = need(fn, {{teacher, "teacher"}, {index, "index"}})) return rc;
   }
   return launched(fn, bssm::launch_distill_forward(a, static_cast<hipStream_t>(stream)));
 }
 
+int64_t bssm_distill_count_floats(void) { return bssm::distill_count_floats(); }
+
 int bssm_distill_backward(int bf16, int teacher_bf16, const void* logits, int64_t logits_row, const void* teacher,
                           const int64_t* index, float temperature, const float* stats, const float* mean,
-                          const float* upstream, int upstream_scalar, void* grad_logits, int64_t rows,
+                          const float* upstream, int upstream_scalar, int ready, void* grad_logits, int64_t rows,
                           int64_t vocabulary, int64_t entries, void* stream) {
   const char* fn = "bssm_distill_backward";
   bssm::DistillArgs a{};
   a.logits = logits; a.logits_row = logits_row; a.teacher = teacher; a.index = index; a.tau = temperature;
-  a.lse = const_cast<float*>(stats); a.mean = const_cast<float*>(mean); a.upstream = upstream;
-  a.upstream_scalar = upstream_scalar != 0; a.grad = grad_logits; a.r = rows; a.v = vocabulary; a.k = entries;
+  a.stats = const_cast<float*>(stats); a.mean = const_cast<float*>(mean); a.upstream = upstream;
+  a.upstream_scalar = upstream_scalar != 0; a.ready = ready != 0; a.grad = grad_logits; a.r = rows; a.v = vocabulary; a.k = entries;
   a.bf16 = bf16 != 0; a.teacher_bf16 = teacher_bf16 != 0;
   if (int rc = distill_check(fn, a)) return rc;
   if (rows == 0) return ok();

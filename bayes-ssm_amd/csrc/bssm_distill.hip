@@ -9,9 +9,18 @@
 // Exponents are taken of (x - max) / tau: a row of the type's lowest value
 // stays finite for tau < 1, and a vocabulary entry at -infinity has q = 0.
 //
-// Bound by memory: the forward reads the logits once (a running maximum and a
-// sum that is rescaled when the maximum moves), the backward reads them again
-// and writes the gradient.
+// Bound by memory, so a training step reads the logits once: a workgroup holds
+// a row in registers (up to 16 pieces of 16 bytes a thread), and the forward
+// writes the gradient for an upstream gradient of 1 (with the mean's division
+// in it) from there.  The backward leaves a row whose upstream gradient is 1,
+// which is what a plain loss.backward() gives, as it is, and forms the others
+// from the logits again (multiplied, the gradient would be rounded twice).
+// Longer rows are read a second time by the forward.
+//
+// Rows lie where they lie: pieces start at the row's first 4-byte boundary at
+// or before its start (an odd bfloat16 row shares its first 4 bytes with the
+// one before), a buffer's range ends with the row, and elements outside are
+// masked.
 #include "bssm_lane.h"
 #include "bssm_sequence.h"
 
@@ -22,9 +31,12 @@ namespace {
 using lane::Pack;
 using lane::kWave;
 
-constexpr int kThreads = 512;
-constexpr int kWaves = kThreads / kWave;
+typedef __amdgpu_buffer_rsrc_t Window;
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
+constexpr int kCountBlocks = 64;  // partial counts of rows with a teacher
+
+template <int THREADS>
 __device__ __forceinline__ float block_sum(float x, float* red) {
   x = lane::lanes_sum(x);
   __syncthreads();
@@ -32,9 +44,10 @@ __device__ __forceinline__ float block_sum(float x, float* red) {
   __syncthreads();
   x = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) x += red[w];
+  for (int w = 0; w < THREADS / kWave; ++w) x += red[w];
   return x;
 }
+template <int THREADS>
 __device__ __forceinline__ float block_max(float x, float* red) {
   x = lane::lanes_max(x);
   __syncthreads();
@@ -42,105 +55,249 @@ __device__ __forceinline__ float block_max(float x, float* red) {
   __syncthreads();
   x = red[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) x = fmaxf(x, red[w]);
+  for (int w = 1; w < THREADS / kWave; ++w) x = fmaxf(x, red[w]);
   return x;
 }
 
+// One row's logits as pieces of 16 bytes; element e of piece k is vocabulary entry k * kN + e - shift.
+template <typename T>
+struct RowOf {
+  static constexpr int kN = 16 / static_cast<int>(sizeof(T));
+  Window w;
+  int shift, end;  // valid elements are [shift, end)
+  __device__ __forceinline__ RowOf(const T* row, int v) {
+    shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) / sizeof(T)) & (4 / static_cast<int>(sizeof(T)) - 1);
+    end = v + shift;
+    const uint32_t bytes = (static_cast<uint32_t>(end) * sizeof(T) + 3u) & ~3u;
+    w = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(row - shift), 0, static_cast<int>(bytes), 0x00020000);
+  }
+  __device__ __forceinline__ Pack<T, kN> load(int piece) const {
+    return __builtin_bit_cast(Pack<T, kN>, __builtin_amdgcn_raw_buffer_load_b128(w, piece * 16, 0, 0));
+  }
+  __device__ __forceinline__ bool whole(int piece) const { return piece * kN >= shift && piece * kN + kN <= end; }
+  __device__ __forceinline__ bool has(int piece, int e) const { return piece * kN + e >= shift && piece * kN + e < end; }
+  // A gradient row of the same shift, elements outside left alone.
+  __device__ __forceinline__ void store(T* row, int piece, const Pack<T, kN>& p) const {
+    if (whole(piece)) {
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, p), w, piece * 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kN; ++e)
+        if (has(piece, e)) row[piece * kN + e - shift] = p.v[e];
+    }
+  }
+};
+
 struct Teacher {
-  int64_t at[kDistillMaxTeacher];  // vocabulary index, -1: does not count
+  int at[kDistillMaxTeacher];  // vocabulary index, -1: does not count
   float p[kDistillMaxTeacher];
 };
 
-// The row's teacher distribution into LDS; log p_k = (l_k - max) / tau - log sum.
+__device__ __forceinline__ bool counts(const DistillArgs& a, int64_t at, float& l, int64_t& i) {
+  l = lane::param(a.teacher, at, a.teacher_bf16);
+  i = a.index[at];
+  return i >= 0 && i < a.v && !(l == -INFINITY);
+}
+
+// The row's teacher distribution into LDS, not yet divided by its sum; log p_k = (l_k - top) / tau - log sum.
+template <int THREADS>
 __device__ __forceinline__ bool teacher_row(const DistillArgs& a, int64_t r, Teacher& t, float* red, float& top,
                                             float& sum) {
   const float c = lane::kLog2e / a.tau;
-  float m = -INFINITY;
-  bool any = false;
-  for (int64_t k = threadIdx.x; k < a.k; k += kThreads) {
-    const float l = lane::param(a.teacher, r * a.k + k, a.teacher_bf16);
-    const int64_t i = a.index[r * a.k + k];
-    const bool there = i >= 0 && i < a.v && !(l == -INFINITY);
-    t.at[k] = there ? i : -1;
+  const int entries = static_cast<int>(a.k);
+  float m = -INFINITY, any = 0.f;
+  for (int k = threadIdx.x; k < entries; k += THREADS) {
+    float l;
+    int64_t i;
+    const bool there = counts(a, r * a.k + k, l, i);
+    t.at[k] = there ? static_cast<int>(i) : -1;
     t.p[k] = l;
-    if (there) m = fmaxf(m, l);
-    any |= there;
+    if (there) {
+      m = fmaxf(m, l);
+      any = 1.f;
+    }
   }
-  top = block_max(m, red);
-  any = block_max(any ? 1.f : 0.f, red) > 0.f;
+  top = block_max<THREADS>(m, red);
+  any = block_max<THREADS>(any, red);
   if (top == -INFINITY) top = 0.f;  // every entry that counts is NaN
   float s = 0.f;
-  for (int64_t k = threadIdx.x; k < a.k; k += kThreads) {
+  for (int k = threadIdx.x; k < entries; k += THREADS) {
     const float e = t.at[k] >= 0 ? lane::exp2_((t.p[k] - top) * c) : 0.f;
     t.p[k] = e;
     s += e;
   }
-  sum = block_sum(s, red);
-  return any;
+  sum = block_sum<THREADS>(s, red);
+  return any > 0.f;
 }
 
-template <typename T>
-__device__ __forceinline__ float logit(const DistillArgs& a, int64_t r, int64_t v) {
-  return lane::widen(static_cast<const T*>(a.logits)[r * a.logits_row + v]);
+// The listed entries' gradient once more, from float32: an index that is
+// listed twice is written by its first place, with the sum of its p.
+template <typename T, int THREADS>
+__device__ __forceinline__ void listed(const DistillArgs& a, const Teacher& t, const T* x, T* g, float top, float inv_s,
+                                       float inv_t, float u) {
+  const float c = lane::kLog2e / a.tau;
+  const int entries = static_cast<int>(a.k);
+  for (int k = threadIdx.x; k < entries; k += THREADS) {
+    const int at = t.at[k];
+    if (at < 0) continue;
+    float p = 0.f;
+    bool first = true;
+    for (int j = 0; j < entries; ++j) {
+      if (t.at[j] != at) continue;
+      if (j < k) first = false;
+      p += t.p[j];
+    }
+    if (first) g[at] = lane::narrow<T>(u * (lane::exp2_((lane::widen(x[at]) - top) * c) * inv_s - p * inv_t));
+  }
 }
 
-// lse[r] = (maximum, sum of exponentials, 1 if the row has a teacher).
-template <typename T, int N>
-__global__ __launch_bounds__(kThreads) void forward_kernel(DistillArgs a) {
+// Rows with a teacher, by a block's share of the rows, a wave a row at a time.
+__global__ __launch_bounds__(256) void count_kernel(DistillArgs a) {
+  __shared__ float red[4];
+  float n = 0.f;
+  for (int64_t r = blockIdx.x * 4 + threadIdx.x / kWave; r < a.r; r += kCountBlocks * 4) {
+    bool any = false;
+    for (int64_t k = threadIdx.x % kWave; k < a.k; k += kWave) {
+      float l;
+      int64_t i;
+      any |= counts(a, r * a.k + k, l, i);
+    }
+    if (__any(any)) n += 1.f;
+  }
+  n = block_sum<256>(threadIdx.x % kWave == 0 ? n : 0.f, red);
+  if (threadIdx.x == 0) a.counts[blockIdx.x] = n;
+}
+__device__ __forceinline__ float rows_with_teacher(const DistillArgs& a) {
+  float n = 0.f;
+  for (int i = 0; i < kCountBlocks; ++i) n += a.counts[i];
+  return fmaxf(n, 1.f);
+}
+
+// PIECES > 0: the row is held, that many pieces a thread; 0: it is read again.
+// a.grad: the gradient for an upstream gradient of 1 is wanted.
+// stats[r] = (maximum, sum of exponentials, 1 if the row has a teacher).
+template <typename T, int THREADS, int PIECES>
+__global__ __launch_bounds__(THREADS) void forward_kernel(DistillArgs a) {
+  constexpr int N = RowOf<T>::kN, kHold = PIECES > 0 ? PIECES : 1;
   __shared__ Teacher t;
-  __shared__ float red[kWaves];
+  __shared__ float red[THREADS / kWave];
   const int64_t r = blockIdx.x;
   const float c = lane::kLog2e / a.tau;
   const T* x = static_cast<const T*>(a.logits) + r * a.logits_row;
+  const RowOf<T> row(x, static_cast<int>(a.v));
+  const int pieces = (row.end + N - 1) / N;
+  Pack<T, N> held[kHold];
   float m = -INFINITY, s = 0.f;
-  for (int64_t v = threadIdx.x * N; v < a.v; v += kThreads * N) {
-    const Pack<T, N> p = lane::load_pack<T, N>(x + v);
-    float best = m;
+  auto top_of = [&](const Pack<T, N>& p, int piece) {
+    float best = -INFINITY;
+    if (row.whole(piece)) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) best = fmaxf(best, lane::widen(p.v[i]));
-    if (best > m) {
-      s = m == -INFINITY ? s : s * lane::exp2_((m - best) * c);
-      m = best;
+      for (int e = 0; e < N; ++e) best = fmaxf(best, lane::widen(p.v[e]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (row.has(piece, e)) best = fmaxf(best, lane::widen(p.v[e]));
     }
-    const float base = m == -INFINITY ? 0.f : m;
+    return best;
+  };
+  auto sum_of = [&](const Pack<T, N>& p, int piece, float base) {
+    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += lane::exp2_((lane::widen(p.v[i]) - base) * c);
+    for (int e = 0; e < N; ++e) {
+      const float v = lane::exp2_((lane::widen(p.v[e]) - base) * c);
+      sum += row.whole(piece) || row.has(piece, e) ? v : 0.f;
+    }
+    return sum;
+  };
+  float top, total;
+  if constexpr (PIECES > 0) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) held[i] = row.load(i * THREADS + threadIdx.x);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+      if (const int piece = i * THREADS + threadIdx.x; piece < pieces) m = fmaxf(m, top_of(held[i], piece));
+    top = block_max<THREADS>(m, red);
+    if (top == -INFINITY) top = 0.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+      if (const int piece = i * THREADS + threadIdx.x; piece < pieces) s += sum_of(held[i], piece, top);
+    total = block_sum<THREADS>(s, red);
+  } else {
+    for (int piece = threadIdx.x; piece < pieces; piece += THREADS) {
+      const Pack<T, N> p = row.load(piece);
+      const float best = fmaxf(m, top_of(p, piece));
+      if (best > m) {
+        s = m == -INFINITY ? s : s * lane::exp2_((m - best) * c);
+        m = best;
+      }
+      s += sum_of(p, piece, m == -INFINITY ? 0.f : m);
+    }
+    top = block_max<THREADS>(m, red);
+    if (top == -INFINITY) top = 0.f;
+    total = block_sum<THREADS>(m == -INFINITY ? s : s * lane::exp2_((m - top) * c), red);
   }
-  float top = block_max(m, red);
-  if (top == -INFINITY) top = 0.f;
-  const float total = block_sum(m == -INFINITY ? s : s * lane::exp2_((m - top) * c), red);
   float t_top, t_sum;
-  const bool any = teacher_row(a, r, t, red, t_top, t_sum);
+  const bool any = teacher_row<THREADS>(a, r, t, red, t_top, t_sum);
+  const float inv_t = 1.f / t_sum;
   float loss = 0.f;
-  const float log_t = logf(t_sum), log_s = logf(total), inv_tau = 1.f / a.tau, inv_t = 1.f / t_sum;
-  for (int64_t k = threadIdx.x; k < a.k; k += kThreads) {
+  const float log_t = logf(t_sum), log_s = logf(total), inv_tau = 1.f / a.tau;
+  for (int k = threadIdx.x; k < a.k; k += THREADS) {
     if (t.at[k] < 0) continue;
     const float p = t.p[k] * inv_t;
     if (p == 0.f) continue;
     const float l = lane::param(a.teacher, r * a.k + k, a.teacher_bf16);
     const float log_p = (l - t_top) * inv_tau - log_t;
-    const float log_q = (logit<T>(a, r, t.at[k]) - top) * inv_tau - log_s;
+    const float log_q = (lane::widen(x[t.at[k]]) - top) * inv_tau - log_s;
     loss = fmaf(p, log_p - log_q, loss);
   }
-  loss = block_sum(loss, red);
+  loss = block_sum<THREADS>(loss, red);
   if (threadIdx.x == 0) {
     a.loss[r] = any ? a.tau * a.tau * loss : 0.f;
-    a.lse[3 * r] = top;
-    a.lse[3 * r + 1] = total;
-    a.lse[3 * r + 2] = any ? 1.f : 0.f;
+    a.stats[3 * r] = top;
+    a.stats[3 * r + 1] = total;
+    a.stats[3 * r + 2] = any ? 1.f : 0.f;
   }
+  if (a.grad == nullptr) return;
+  const float u = a.tau / (a.mean_of_rows ? rows_with_teacher(a) : 1.f), inv_s = 1.f / total;
+  T* g = static_cast<T*>(a.grad) + r * a.v;
+  const RowOf<T> to(g, static_cast<int>(a.v));
+  auto gradient = [&](const Pack<T, N>& p, int piece) {
+    Pack<T, N> o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float v = u * (lane::exp2_((lane::widen(p.v[e]) - top) * c) * inv_s);
+      o.v[e] = lane::narrow<T>(any ? v : 0.f);
+    }
+    if (to.shift == row.shift) {
+      to.store(g, piece, o);
+    } else {  // bfloat16 rows of which one is odd
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (row.has(piece, e)) g[piece * N + e - row.shift] = o.v[e];
+    }
+  };
+  if constexpr (PIECES > 0) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+      if (const int piece = i * THREADS + threadIdx.x; piece < pieces) gradient(held[i], piece);
+  } else {
+    for (int piece = threadIdx.x; piece < pieces; piece += THREADS) gradient(row.load(piece), piece);
+  }
+  if (!any) return;
+  __syncthreads();
+  listed<T, THREADS>(a, t, x, g, top, inv_s, inv_t, u);
 }
 
 // mean[] = (sum / rows with a teacher, 1 / rows, sum), in a fixed order.
-__global__ __launch_bounds__(kThreads) void mean_kernel(DistillArgs a) {
-  __shared__ float red[kWaves];
+__global__ __launch_bounds__(1024) void mean_kernel(DistillArgs a) {
+  __shared__ float red[16];
   float s = 0.f, n = 0.f;
-  for (int64_t r = threadIdx.x; r < a.r; r += kThreads) {
+  for (int64_t r = threadIdx.x; r < a.r; r += 1024) {
     s += a.loss[r];
-    n += a.lse[3 * r + 2];
+    n += a.stats[3 * r + 2];
   }
-  s = block_sum(s, red);
-  n = fmaxf(block_sum(n, red), 1.f);
+  s = block_sum<1024>(s, red);
+  n = fmaxf(block_sum<1024>(n, red), 1.f);
   if (threadIdx.x == 0) {
     a.mean[0] = s / n;
     a.mean[1] = 1.f / n;
@@ -148,82 +305,87 @@ __global__ __launch_bounds__(kThreads) void mean_kernel(DistillArgs a) {
   }
 }
 
-template <typename T, int N>
-__global__ __launch_bounds__(kThreads) void backward_kernel(DistillArgs a) {
+// The gradient from the logits and the forward's statistics; with `ready`, of the rows that the forward's does not fit.
+template <typename T>
+__global__ __launch_bounds__(512) void backward_kernel(DistillArgs a) {
+  constexpr int THREADS = 512, N = RowOf<T>::kN;
   __shared__ Teacher t;
-  __shared__ float red[kWaves];
+  __shared__ float red[THREADS / kWave];
   const int64_t r = blockIdx.x;
   const float c = lane::kLog2e / a.tau;
   const T* x = static_cast<const T*>(a.logits) + r * a.logits_row;
   T* g = static_cast<T*>(a.grad) + r * a.v;
-  const float top = a.lse[3 * r], inv_s = 1.f / a.lse[3 * r + 1];
-  const bool any = a.lse[3 * r + 2] > 0.f;
-  const float u = a.tau * a.upstream[a.upstream_scalar ? 0 : r] * (a.mean == nullptr ? 1.f : a.mean[1]);
+  const RowOf<T> row(x, static_cast<int>(a.v)), to(g, static_cast<int>(a.v));
+  const int pieces = (row.end + N - 1) / N;
+  const float top = a.stats[3 * r], inv_s = 1.f / a.stats[3 * r + 1];
+  const bool any = a.stats[3 * r + 2] > 0.f;
+  const float up = a.upstream[a.upstream_scalar ? 0 : r];
+  if (a.ready && up == 1.f) return;
+  const float u = a.tau * up * (a.mean == nullptr ? 1.f : a.mean[1]);
   float t_top, t_sum;
-  teacher_row(a, r, t, red, t_top, t_sum);
-  for (int64_t v = threadIdx.x * N; v < a.v; v += kThreads * N) {
-    Pack<T, N> p;
-    if (any) {
-      p = lane::load_pack<T, N>(x + v);
+  teacher_row<THREADS>(a, r, t, red, t_top, t_sum);
+  for (int piece = threadIdx.x; piece < pieces; piece += THREADS) {
+    const Pack<T, N> p = row.load(piece);
+    Pack<T, N> o;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        p.v[i] = lane::narrow<T>(u * (lane::exp2_((lane::widen(p.v[i]) - top) * c) * inv_s));
+    for (int e = 0; e < N; ++e) {
+      const float v = u * (lane::exp2_((lane::widen(p.v[e]) - top) * c) * inv_s);
+      o.v[e] = lane::narrow<T>(any ? v : 0.f);
+    }
+    if (to.shift == row.shift) {
+      to.store(g, piece, o);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) p.v[i] = lane::narrow<T>(0.f);
+      for (int e = 0; e < N; ++e)
+        if (row.has(piece, e)) g[piece * N + e - row.shift] = o.v[e];
     }
-    lane::store_pack<T, N>(g + v, p);
   }
   if (!any) return;
-  // The listed entries once more, from float32: an index that is listed twice
-  // is written by its first place, with the sum of its p.
   __syncthreads();
-  const float inv_t = 1.f / t_sum;
-  for (int64_t k = threadIdx.x; k < a.k; k += kThreads) {
-    const int64_t at = t.at[k];
-    if (at < 0) continue;
-    float p = 0.f;
-    bool first = true;
-    for (int64_t j = 0; j < a.k; ++j) {
-      if (t.at[j] != at) continue;
-      if (j < k) first = false;
-      p += t.p[j];
-    }
-    if (first) g[at] = lane::narrow<T>(u * (lane::exp2_((logit<T>(a, r, at) - top) * c) * inv_s - p * inv_t));
-  }
+  listed<T, THREADS>(a, t, x, g, top, inv_s, 1.f / t_sum, u);
 }
 
-bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-bool vectors(const DistillArgs& a) {
-  const int n = a.bf16 ? 8 : 4;
-  return a.v % n == 0 && a.logits_row % n == 0 && aligned(a.logits) && aligned(a.grad);
-}
-
-template <typename T, int N>
-hipError_t launch(const DistillArgs& a, bool back, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(a.r)), block(kThreads);
-  if (back) hipLaunchKernelGGL((backward_kernel<T, N>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((forward_kernel<T, N>), grid, block, 0, stream, a);
+// The fewest threads that hold the row in 8 pieces each, and 1024 with 16 for
+// twice the longest of those: with 8 (60 registers) a compute unit has four
+// rows of 64 KB in flight.
+template <typename T>
+hipError_t forward(const DistillArgs& a, hipStream_t stream) {
+  const int64_t pieces = a.v / RowOf<T>::kN + 2;
+  const dim3 grid(static_cast<unsigned>(a.r));
+  if (pieces <= 256 * 2) hipLaunchKernelGGL((forward_kernel<T, 256, 2>), grid, dim3(256), 0, stream, a);
+  else if (pieces <= 256 * 8) hipLaunchKernelGGL((forward_kernel<T, 256, 8>), grid, dim3(256), 0, stream, a);
+  else if (pieces <= 512 * 8) hipLaunchKernelGGL((forward_kernel<T, 512, 8>), grid, dim3(512), 0, stream, a);
+  else if (pieces <= 1024 * 8) hipLaunchKernelGGL((forward_kernel<T, 1024, 8>), grid, dim3(1024), 0, stream, a);
+  else if (pieces <= 1024 * 16) hipLaunchKernelGGL((forward_kernel<T, 1024, 16>), grid, dim3(1024), 0, stream, a);
+  else hipLaunchKernelGGL((forward_kernel<T, 1024, 0>), grid, dim3(1024), 0, stream, a);
   return hipGetLastError();
-}
-hipError_t types(const DistillArgs& a, bool back, hipStream_t stream) {
-  if (a.r == 0) return hipSuccess;
-  if (vectors(a)) return a.bf16 ? launch<__bf16, 8>(a, back, stream) : launch<float, 4>(a, back, stream);
-  return a.bf16 ? launch<__bf16, 1>(a, back, stream) : launch<float, 1>(a, back, stream);
 }
 
 }  // namespace
 }  // namespace distill
 
+int64_t distill_count_floats() { return distill::kCountBlocks; }
+
 hipError_t launch_distill_forward(const DistillArgs& a, hipStream_t stream) {
-  if (hipError_t e = distill::types(a, false, stream); e != hipSuccess) return e;
+  if (a.r > 0) {
+    if (a.grad != nullptr && a.mean_of_rows) {
+      hipLaunchKernelGGL(distill::count_kernel, dim3(distill::kCountBlocks), dim3(256), 0, stream, a);
+      if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    if (hipError_t e = a.bf16 ? distill::forward<__bf16>(a, stream) : distill::forward<float>(a, stream); e != hipSuccess)
+      return e;
+  }
   if (a.mean == nullptr) return hipSuccess;
-  hipLaunchKernelGGL(distill::mean_kernel, dim3(1), dim3(distill::kThreads), 0, stream, a);
+  hipLaunchKernelGGL(distill::mean_kernel, dim3(1), dim3(1024), 0, stream, a);
   return hipGetLastError();
 }
 
 hipError_t launch_distill_backward(const DistillArgs& a, hipStream_t stream) {
-  return distill::types(a, true, stream);
+  if (a.r == 0) return hipSuccess;
+  const dim3 grid(static_cast<unsigned>(a.r)), block(512);
+  if (a.bf16) hipLaunchKernelGGL(distill::backward_kernel<__bf16>, grid, block, 0, stream, a);
+  else hipLaunchKernelGGL(distill::backward_kernel<float>, grid, block, 0, stream, a);
+  return hipGetLastError();
 }
 
 }  // namespace bssm

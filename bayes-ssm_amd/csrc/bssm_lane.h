@@ -56,6 +56,20 @@ __device__ __forceinline__ float sigmoid_(float x) { return rcp_(1.f + exp_(-x))
 __device__ __forceinline__ float softplus_(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
 __device__ __forceinline__ float softplus_slope_(float x) { return 1.f / (1.f + expf(-x)); }
 
+// N consecutive parameters of either type from one access (aligned to N elements).
+template <int N>
+__device__ __forceinline__ void params(const void* p, int64_t i, int bf16, float (&out)[N]) {
+  if (bf16) {
+    const Pack<__bf16, N> v = load_pack<__bf16, N>(static_cast<const __bf16*>(p) + i);
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = widen(v.v[e]);
+  } else {
+    const Pack<float, N> v = *reinterpret_cast<const Pack<float, N>*>(static_cast<const float*>(p) + i);
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = v.v[e];
+  }
+}
+
 template <int WIDTH = kWave>
 __device__ __forceinline__ float lanes_sum(float x) {
 #pragma unroll
@@ -69,15 +83,15 @@ __device__ __forceinline__ float lanes_max(float x) {
   return x;
 }
 
-// Column sums of partials [rows, cols] (float32): a block of 256 threads takes
-// 32 columns, its 8 row groups every 8th row with four loads in flight, and
+// Column sums of partials [rows, cols] (float32): a block of 1024 threads takes
+// 32 columns, its 32 row groups every 32nd row with four loads in flight, and
 // they meet in LDS in a fixed order.  put(column, sum).
-constexpr int kFoldColumns = 32;
+constexpr int kFoldColumns = 32, kFoldThreads = 1024;
 template <typename Put>
 __device__ __forceinline__ void fold_columns(const float* __restrict__ part, int64_t rows, int64_t cols, int64_t block,
                                              Put put) {
-  constexpr int kGroups = 256 / kFoldColumns;
-  __shared__ float red[256];
+  constexpr int kGroups = kFoldThreads / kFoldColumns;
+  __shared__ float red[kFoldThreads];
   const int cl = threadIdx.x % kFoldColumns, g = threadIdx.x / kFoldColumns;
   const int64_t c = block * kFoldColumns + cl;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -97,6 +111,7 @@ __device__ __forceinline__ void fold_columns(const float* __restrict__ part, int
     put(c, sum);
   }
 }
+inline unsigned fold_blocks(int64_t cols) { return static_cast<unsigned>((cols + kFoldColumns - 1) / kFoldColumns); }
 
 }  // namespace lane
 }  // namespace bssm

@@ -5,12 +5,15 @@
 //
 // Bound by memory: the forward reads and writes a stream once, the backward
 // reads two and writes one.  A row belongs to one wave, to 4 or to 16 waves
-// (the fewest that hold it in kVectors vectors a lane), stays in registers
+// (the fewest that hold it in kHeld vectors a lane), stays in registers
 // between the mean, the centred sum of squares and the output, and is read
-// once.  Longer rows (see `fits`) are read again from the caches for each of the three.
-// The backward's blocks walk rows a grid apart and keep the column sums of
-// their rows in registers: the weight's and the bias's gradient leave a block
-// as one row of partials and are folded in a fixed order.
+// once.  Longer rows are read again from the caches for each of the three.
+// Blocks walk rows a grid apart, so that weight and bias are read once a wave
+// and stay in registers (read for every row by single elements they cost three
+// times the row), and ask for the next row before they reduce this one.  The
+// backward keeps the column sums of its rows in registers: the weight's and the
+// bias's gradient leave a block as one row of partials and are folded in a
+// fixed order.
 #include "bssm_lane.h"
 #include "bssm_sequence.h"
 
@@ -21,8 +24,12 @@ namespace {
 using lane::Pack;
 using lane::kWave;
 
-constexpr int kVectors = 4;       // vectors of a row that a lane holds
-constexpr int kMaxBlocks = 1024;  // blocks of the backward: 4 a compute unit
+// Vectors of a row that a lane holds: two sets of four beside the sums fill the registers that 4 waves leave, 16 waves
+// leave half of those.
+template <int WAVES>
+constexpr int kHeld = WAVES == 16 ? 2 : 4;
+constexpr int kMaxBlocks = 512;         // blocks of the backward: 2 a compute unit, each adds a row of partials
+constexpr int kMaxForwardBlocks = 1536;  // 6 a compute unit
 
 // Sum over the WAVES waves of a row (all of the block when WAVES > 1).
 template <int WAVES>
@@ -72,69 +79,103 @@ struct Place {
   }
 };
 
-template <typename T, int N, int WAVES, bool HELD>
+// This thread's vectors of a row.
+template <typename T, int N, int WAVES>
+struct Held {
+  Pack<T, N> v[kHeld<WAVES>];
+  __device__ __forceinline__ void load(const T* row, int c_first, int d) {
+#pragma unroll
+    for (int k = 0; k < kHeld<WAVES>; ++k)
+      if (c_first + k * Place<WAVES>::kLanes * N < d) v[k] = lane::load_pack<T, N>(row + c_first + k * Place<WAVES>::kLanes * N);
+  }
+};
+// This thread's parameters; `none` where there are none.
+template <int N, int WAVES>
+struct Params {
+  float v[kHeld<WAVES>][N];
+  __device__ __forceinline__ Params(const void* p, int bf16, int c_first, int d, float none) {
+#pragma unroll
+    for (int k = 0; k < kHeld<WAVES>; ++k) {
+      const int c = c_first + k * Place<WAVES>::kLanes * N;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[k][i] = none;
+      if (p != nullptr && c < d) lane::params<N>(p, c, bf16, v[k]);
+    }
+  }
+};
+
+template <typename T, int N, int WAVES>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void forward_kernel(LayerNormArgs a) {
   __shared__ float red[2 * WAVES];
   const Place<WAVES> at;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * Place<WAVES>::kRows + at.row;
+  constexpr int kRows = Place<WAVES>::kRows, kStep = Place<WAVES>::kLanes * N;
+  const int d = static_cast<int>(a.d), c_first = at.ln * N;
+  const float inv_d = 1.f / static_cast<float>(a.d);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + at.row;
   if (r >= a.r) return;  // whole waves, and whole blocks where a row is a block's
+  const Params<N, WAVES> w(a.weight, a.param_bf16, c_first, d, 1.f), b(a.bias, a.param_bf16, c_first, d, 0.f);
+  Held<T, N, WAVES> x, next;
+  next.load(static_cast<const T*>(a.x) + r * a.x_row, c_first, d);
+  for (; r < a.r; r += step) {
+    x = next;
+    if (r + step < a.r) next.load(static_cast<const T*>(a.x) + (r + step) * a.x_row, c_first, d);
+    float sum = 0.f, sq = 0.f;
+#pragma unroll
+    for (int v = 0; v < kHeld<WAVES>; ++v)
+      if (c_first + v * kStep < d)
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum += lane::widen(x.v[v].v[i]);
+    const float mean = row_sum<WAVES>(sum, red) * inv_d;
+#pragma unroll
+    for (int v = 0; v < kHeld<WAVES>; ++v)
+      if (c_first + v * kStep < d)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float o = lane::widen(x.v[v].v[i]) - mean;
+          sq = fmaf(o, o, sq);
+        }
+    const float rstd = rsqrtf(fmaf(row_sum<WAVES>(sq, red), inv_d, a.eps));
+    T* y = static_cast<T*>(a.y) + r * a.d;
+#pragma unroll
+    for (int v = 0; v < kHeld<WAVES>; ++v)
+      if (c_first + v * kStep < d) {
+        Pack<T, N> out;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          out.v[i] = lane::narrow<T>(fmaf((lane::widen(x.v[v].v[i]) - mean) * rstd, w.v[v][i], b.v[v][i]));
+        lane::store_pack<T, N>(y + c_first + v * kStep, out);
+      }
+    if (at.ln == 0 && a.mean != nullptr) {
+      a.mean[r] = mean;
+      a.rstd[r] = rstd;
+    }
+  }
+}
+
+// Rows too long to be held: each of the three passes reads the row, one element a lane.
+template <typename T>
+__global__ __launch_bounds__(1024) void forward_long_kernel(LayerNormArgs a) {
+  constexpr int WAVES = 16;
+  __shared__ float red[2 * WAVES];
+  const int64_t r = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + r * a.x_row;
   T* y = static_cast<T*>(a.y) + r * a.d;
-  const int64_t step = Place<WAVES>::kLanes * N, c_first = at.ln * N;
   const float inv_d = 1.f / static_cast<float>(a.d);
-  Pack<T, N> held[kVectors];
   float sum = 0.f, sq = 0.f;
-  if constexpr (HELD) {
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v)
-      if (c_first + v * step < a.d) held[v] = lane::load_pack<T, N>(x + c_first + v * step);
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v)
-      if (c_first + v * step < a.d)
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum += lane::widen(held[v].v[i]);
-  } else {
-    for (int64_t c = c_first; c < a.d; c += step) {
-      const Pack<T, N> p = lane::load_pack<T, N>(x + c);
-#pragma unroll
-      for (int i = 0; i < N; ++i) sum += lane::widen(p.v[i]);
-    }
-  }
+  for (int64_t c = threadIdx.x; c < a.d; c += 1024) sum += lane::widen(x[c]);
   const float mean = row_sum<WAVES>(sum, red) * inv_d;
-  auto centred = [&](const Pack<T, N>& p) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float o = lane::widen(p.v[i]) - mean;
-      sq = fmaf(o, o, sq);
-    }
-  };
-  if constexpr (HELD) {
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v)
-      if (c_first + v * step < a.d) centred(held[v]);
-  } else {
-    for (int64_t c = c_first; c < a.d; c += step) centred(lane::load_pack<T, N>(x + c));
+  for (int64_t c = threadIdx.x; c < a.d; c += 1024) {
+    const float o = lane::widen(x[c]) - mean;
+    sq = fmaf(o, o, sq);
   }
   const float rstd = rsqrtf(fmaf(row_sum<WAVES>(sq, red), inv_d, a.eps));
-  auto write = [&](const Pack<T, N>& p, int64_t c) {
-    Pack<T, N> out;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float o = (lane::widen(p.v[i]) - mean) * rstd;
-      if (a.weight != nullptr) o *= lane::param(a.weight, c + i, a.param_bf16);
-      if (a.bias != nullptr) o += lane::param(a.bias, c + i, a.param_bf16);
-      out.v[i] = lane::narrow<T>(o);
-    }
-    lane::store_pack<T, N>(y + c, out);
-  };
-  if constexpr (HELD) {
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v)
-      if (c_first + v * step < a.d) write(held[v], c_first + v * step);
-  } else {
-    for (int64_t c = c_first; c < a.d; c += step) write(lane::load_pack<T, N>(x + c), c);
+  for (int64_t c = threadIdx.x; c < a.d; c += 1024) {
+    const float w = a.weight == nullptr ? 1.f : lane::param(a.weight, c, a.param_bf16);
+    const float b = a.bias == nullptr ? 0.f : lane::param(a.bias, c, a.param_bf16);
+    y[c] = lane::narrow<T>(fmaf((lane::widen(x[c]) - mean) * rstd, w, b));
   }
-  if (at.ln == 0 && a.mean != nullptr) {
+  if (threadIdx.x == 0 && a.mean != nullptr) {
     a.mean[r] = mean;
     a.rstd[r] = rstd;
   }
@@ -143,41 +184,45 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void forward_kern
 // Gradient of the input and, where a.partials is given, the column sums.
 template <typename T, int N, int WAVES>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void backward_kernel(LayerNormArgs a) {
-  constexpr int kRows = Place<WAVES>::kRows;
+  constexpr int kRows = Place<WAVES>::kRows, kStep = Place<WAVES>::kLanes * N;
   __shared__ float red[2 * WAVES];
   __shared__ float cols[WAVES == 1 ? kRows - 1 : 1][WAVES == 1 ? kWave * N : 1];
   const Place<WAVES> at;
-  const int64_t step = Place<WAVES>::kLanes * N, c_first = at.ln * N;
+  const int d = static_cast<int>(a.d), c_first = at.ln * N;
   const float inv_d = 1.f / static_cast<float>(a.d);
-  float gw[kVectors][N], gb[kVectors][N];
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  float gw[kHeld<WAVES>][N], gb[kHeld<WAVES>][N];
 #pragma unroll
-  for (int v = 0; v < kVectors; ++v)
+  for (int v = 0; v < kHeld<WAVES>; ++v)
 #pragma unroll
     for (int i = 0; i < N; ++i) gw[v][i] = gb[v][i] = 0.f;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + at.row; r < a.r;
-       r += static_cast<int64_t>(gridDim.x) * kRows) {
-    const T* x = static_cast<const T*>(a.x) + r * a.x_row;
-    const T* gy = static_cast<const T*>(a.gy) + r * a.d;
-    const float mean = a.mean[r], rstd = a.rstd[r];
-    Pack<T, N> px[kVectors], pg[kVectors];
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v)
-      if (c_first + v * step < a.d) {
-        px[v] = lane::load_pack<T, N>(x + c_first + v * step);
-        pg[v] = lane::load_pack<T, N>(gy + c_first + v * step);
-      }
+  int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + at.row;
+  const Params<N, WAVES> w(a.weight, a.param_bf16, c_first, d, 1.f);
+  Held<T, N, WAVES> x, g, next_x, next_g;
+  float next_mean = 0.f, next_rstd = 0.f;
+  auto load = [&](int64_t row) {
+    next_x.load(static_cast<const T*>(a.x) + row * a.x_row, c_first, d);
+    next_g.load(static_cast<const T*>(a.gy) + row * a.d, c_first, d);
+    next_mean = a.mean[row];
+    next_rstd = a.rstd[row];
+  };
+  if (r < a.r) load(r);
+  for (; r < a.r; r += step) {
+    x = next_x;
+    g = next_g;
+    const float mean = next_mean, rstd = next_rstd;
+    if (r + step < a.r) load(r + step);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int v = 0; v < kVectors; ++v)
-      if (c_first + v * step < a.d)
+    for (int v = 0; v < kHeld<WAVES>; ++v)
+      if (c_first + v * kStep < d)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const float xh = (lane::widen(px[v].v[i]) - mean) * rstd, g = lane::widen(pg[v].v[i]);
-          const float w = a.weight == nullptr ? 1.f : lane::param(a.weight, c_first + v * step + i, a.param_bf16);
-          gw[v][i] = fmaf(g, xh, gw[v][i]);
-          gb[v][i] += g;
-          s1 = fmaf(g, w, s1);
-          s2 = fmaf(g * w, xh, s2);
+          const float xh = (lane::widen(x.v[v].v[i]) - mean) * rstd, gi = lane::widen(g.v[v].v[i]), gu = gi * w.v[v][i];
+          gw[v][i] = fmaf(gi, xh, gw[v][i]);
+          gb[v][i] += gi;
+          s1 += gu;
+          s2 = fmaf(gu, xh, s2);
         }
     if (a.gx == nullptr) continue;
     row_sums<WAVES>(s1, s2, red);
@@ -185,47 +230,46 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void backward_ker
     s2 *= inv_d;
     T* gx = static_cast<T*>(a.gx) + r * a.d;
 #pragma unroll
-    for (int v = 0; v < kVectors; ++v)
-      if (c_first + v * step < a.d) {
+    for (int v = 0; v < kHeld<WAVES>; ++v)
+      if (c_first + v * kStep < d) {
         Pack<T, N> out;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const float xh = (lane::widen(px[v].v[i]) - mean) * rstd, g = lane::widen(pg[v].v[i]);
-          const float w = a.weight == nullptr ? 1.f : lane::param(a.weight, c_first + v * step + i, a.param_bf16);
-          out.v[i] = lane::narrow<T>(rstd * (fmaf(g, w, -s1) - xh * s2));
+          const float xh = (lane::widen(x.v[v].v[i]) - mean) * rstd, gu = lane::widen(g.v[v].v[i]) * w.v[v][i];
+          out.v[i] = lane::narrow<T>(rstd * (gu - s1 - xh * s2));
         }
-        lane::store_pack<T, N>(gx + c_first + v * step, out);
+        lane::store_pack<T, N>(gx + c_first + v * kStep, out);
       }
   }
   if (a.partials == nullptr) return;
   float* part = a.partials + static_cast<int64_t>(blockIdx.x) * 2 * a.d;
 #pragma unroll
-  for (int v = 0; v < kVectors; ++v)
+  for (int v = 0; v < kHeld<WAVES>; ++v)
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      float s[N];
+      Pack<float, N> s;
 #pragma unroll
-      for (int i = 0; i < N; ++i) s[i] = k == 0 ? gw[v][i] : gb[v][i];
+      for (int i = 0; i < N; ++i) s.v[i] = k == 0 ? gw[v][i] : gb[v][i];
       if constexpr (WAVES == 1) {  // the block's 4 rows at a time meet here
         __syncthreads();
         if (at.row > 0)
 #pragma unroll
-          for (int i = 0; i < N; ++i) cols[at.row - 1][i * kWave + at.ln] = s[i];
+          for (int i = 0; i < N; ++i) cols[at.row - 1][i * kWave + at.ln] = s.v[i];
         __syncthreads();
         if (at.row == 0)
 #pragma unroll
-          for (int w = 0; w < kRows - 1; ++w)
+          for (int o = 0; o < kRows - 1; ++o)
 #pragma unroll
-            for (int i = 0; i < N; ++i) s[i] += cols[w][i * kWave + at.ln];
+            for (int i = 0; i < N; ++i) s.v[i] += cols[o][i * kWave + at.ln];
       }
-      if (at.row == 0 && c_first + v * step < a.d)
+      if (at.row == 0 && c_first + v * kStep < d)
 #pragma unroll
-        for (int i = 0; i < N; ++i) part[k * a.d + c_first + v * step + i] = s[i];
+        for (int i = 0; i < N; ++i) part[k * a.d + c_first + v * kStep + i] = s.v[i];
     }
 }
 
-// Rows too long to be held: three passes over a row, and the column sums by
-// blocks of their own (256 columns x a share of the rows).
+// The same for rows too long to be held; the column sums are taken by blocks of
+// their own (256 columns x a share of the rows).
 template <typename T>
 __global__ __launch_bounds__(1024) void backward_long_kernel(LayerNormArgs a) {
   constexpr int WAVES = 16;
@@ -262,7 +306,7 @@ __global__ __launch_bounds__(256) void columns_kernel(LayerNormArgs a, int64_t r
   a.partials[(blockIdx.y * 2 + 1) * a.d + c] = gb;
 }
 
-__global__ __launch_bounds__(256) void fold_kernel(LayerNormArgs a, int64_t rows) {
+__global__ __launch_bounds__(lane::kFoldThreads) void fold_kernel(LayerNormArgs a, int64_t rows) {
   lane::fold_columns(a.partials, rows, 2 * a.d, blockIdx.x, [&](int64_t c, float sum) {
     if (c < a.d) {
       if (a.gweight != nullptr) lane::put_param(a.gweight, c, sum, a.param_bf16);
@@ -275,36 +319,38 @@ __global__ __launch_bounds__(256) void fold_kernel(LayerNormArgs a, int64_t rows
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool vectors(const LayerNormArgs& a) {
   const int n = a.bf16 ? 8 : 4;
-  return a.d % n == 0 && a.x_row % n == 0 && aligned(a.x) && aligned(a.y) && aligned(a.gy) && aligned(a.gx);
+  return a.d % n == 0 && a.x_row % n == 0 && aligned(a.x) && aligned(a.y) && aligned(a.gy) && aligned(a.gx) &&
+         aligned(a.weight) && aligned(a.bias);
 }
 // Waves of a row with N values a vector: 1, 4 or 16; 0 where 16 do not hold it.
 int row_waves(int64_t d, int n) {
-  const int64_t one = (int64_t)kVectors * kWave * n;
-  return d <= one ? 1 : d <= 4 * one ? 4 : d <= 16 * one ? 16 : 0;
+  const int64_t lanes = (int64_t)kWave * n;
+  return d <= kHeld<1> * lanes ? 1 : d <= kHeld<4> * 4 * lanes ? 4 : d <= kHeld<16> * 16 * lanes ? 16 : 0;
 }
 // Blocks of the backward, from the sizes alone: each adds a row of partials.
 int64_t backward_blocks(int64_t r, int64_t d, int bf16) {
   const int waves = row_waves(d, bf16 ? 8 : 4), rows = waves == 1 ? 4 : 1;
-  const int64_t most = waves == 16 ? kMaxBlocks / 4 : waves == 0 ? 64 : kMaxBlocks, want = (r + rows - 1) / rows;
+  const int64_t most = waves == 16 ? kMaxBlocks / 2 : waves == 0 ? 64 : kMaxBlocks, want = (r + rows - 1) / rows;
   return want < most ? want : most;
 }
 
 hipError_t fold(const LayerNormArgs& a, int64_t rows, hipStream_t s) {
   if (a.gweight == nullptr && a.gbias == nullptr) return hipSuccess;
-  const int64_t cols = 2 * a.d;
-  hipLaunchKernelGGL(fold_kernel, dim3(static_cast<unsigned>((cols + lane::kFoldColumns - 1) / lane::kFoldColumns)),
-                     dim3(256), 0, s, a, rows);
+  hipLaunchKernelGGL(fold_kernel, dim3(lane::fold_blocks(2 * a.d)), dim3(lane::kFoldThreads), 0, s, a, rows);
   return hipGetLastError();
 }
 
 template <typename T, int N>
 hipError_t forward(const LayerNormArgs& a, hipStream_t s) {
-  const auto grid = [&](int rows) { return dim3(static_cast<unsigned>((a.r + rows - 1) / rows)); };
+  const auto grid = [&](int rows, int64_t most) {
+    const int64_t want = (a.r + rows - 1) / rows;
+    return dim3(static_cast<unsigned>(want < most ? want : most));
+  };
   switch (row_waves(a.d, N)) {
-    case 1: hipLaunchKernelGGL((forward_kernel<T, N, 1, true>), grid(4), dim3(256), 0, s, a); break;
-    case 4: hipLaunchKernelGGL((forward_kernel<T, N, 4, true>), grid(1), dim3(256), 0, s, a); break;
-    case 16: hipLaunchKernelGGL((forward_kernel<T, N, 16, true>), grid(1), dim3(1024), 0, s, a); break;
-    default: hipLaunchKernelGGL((forward_kernel<T, N, 16, false>), grid(1), dim3(1024), 0, s, a); break;
+    case 1: hipLaunchKernelGGL((forward_kernel<T, N, 1>), grid(4, kMaxForwardBlocks), dim3(256), 0, s, a); break;
+    case 4: hipLaunchKernelGGL((forward_kernel<T, N, 4>), grid(1, kMaxForwardBlocks), dim3(256), 0, s, a); break;
+    case 16: hipLaunchKernelGGL((forward_kernel<T, N, 16>), grid(1, kMaxForwardBlocks / 3), dim3(1024), 0, s, a); break;
+    default: hipLaunchKernelGGL(forward_long_kernel<T>, dim3(static_cast<unsigned>(a.r)), dim3(1024), 0, s, a); break;
   }
   return hipGetLastError();
 }

@@ -94,9 +94,9 @@ struct Lds {
     else if constexpr (kUnits == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
     else return row >> 2 & 3;
   }
-  static __device__ __forceinline__ int at(int row, int col) {
-    return row * W + ((col / kUnit ^ turn(row)) * kUnit + col % kUnit);
-  }
+  // Element of column c0 + c, which have no bits in common: with a constant c0
+  // one exclusive or of what the lane alone decides.
+  static __device__ __forceinline__ int at(int row, int c0, int c) { return (row * W + (c ^ turn(row) * kUnit)) ^ c0; }
 };
 
 // The operand whose row is the LDS row `row` (of lane l % 32) and whose k are the columns from c0 on, plain order.
@@ -104,10 +104,10 @@ template <int W, typename T>
 __device__ __forceinline__ Operand<T> along(const T* tile, int row, int c0, int g) {
   Operand<T> o;
   if constexpr (sizeof(T) == 2) {
-    o.v = *reinterpret_cast<const v8b*>(tile + Lds<T, W>::at(row, c0 + 8 * g));
+    o.v = *reinterpret_cast<const v8b*>(tile + Lds<T, W>::at(row, c0, 8 * g));
   } else {
-    const v4f a = *reinterpret_cast<const v4f*>(tile + Lds<T, W>::at(row, c0 + 8 * g)),
-              b = *reinterpret_cast<const v4f*>(tile + Lds<T, W>::at(row, c0 + 8 * g + 4));
+    const v4f a = *reinterpret_cast<const v4f*>(tile + Lds<T, W>::at(row, c0, 8 * g)),
+              b = *reinterpret_cast<const v4f*>(tile + Lds<T, W>::at(row, c0 + 4, 8 * g));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       o.v[e] = a[e];
@@ -130,7 +130,7 @@ __device__ __forceinline__ Operand<T> across(const T* tile, int k0, int c0, int 
     typedef __attribute__((address_space(3))) v4s* At;
     const int dr = ln % 16 / 4, dc = ln / 16 % 2 * 16 + ln % 4 * 4;
     // k0 is a multiple of 16, the rows' permutation repeats with 16.
-    const T *p0 = tile + k0 * W + Lds<T, W>::at(r0 + dr, c0 + dc), *p1 = tile + k0 * W + Lds<T, W>::at(r1 + dr, c0 + dc);
+    const T *p0 = tile + k0 * W + Lds<T, W>::at(r0 + dr, c0, dc), *p1 = tile + k0 * W + Lds<T, W>::at(r1 + dr, c0, dc);
     const v4b a = __builtin_bit_cast(v4b, __builtin_amdgcn_ds_read_tr16_b64_v4i16((At)p0));
     const v4b b = __builtin_bit_cast(v4b, __builtin_amdgcn_ds_read_tr16_b64_v4i16((At)p1));
 #pragma unroll
@@ -141,8 +141,8 @@ __device__ __forceinline__ Operand<T> across(const T* tile, int k0, int c0, int 
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      o.v[e] = tile[k0 * W + Lds<T, W>::at(r0 + e, c0 + ln % 32)];
-      o.v[e + 4] = tile[k0 * W + Lds<T, W>::at(r1 + e, c0 + ln % 32)];
+      o.v[e] = tile[k0 * W + Lds<T, W>::at(r0 + e, c0, ln % 32)];
+      o.v[e + 4] = tile[k0 * W + Lds<T, W>::at(r1 + e, c0, ln % 32)];
     }
   }
   return o;
@@ -158,8 +158,8 @@ typedef __amdgpu_buffer_rsrc_t Window;
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 constexpr uint32_t kPast = 0x80000000u;
-__device__ __forceinline__ Window window(const void* base, int64_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes < 0 ? 0 : bytes), 0x00020000);
+__device__ __forceinline__ Window window(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes), 0x00020000);
 }
 __device__ __forceinline__ v4f load16(Window w, uint32_t at) {
   return __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(w, static_cast<int>(at), 0, 0));
@@ -185,15 +185,15 @@ struct Rows {
   // Row r at src + r * st; rows from `rows` on and columns from n on are 0.
   // FAST (see fast_streams): 16-byte units on their boundaries, the window's 32-bit offsets.
   template <bool FAST>
-  __device__ __forceinline__ void load(const T* src, int64_t st, int64_t rows, int64_t c0, int64_t n) {
+  __device__ __forceinline__ void load(const T* src, int64_t st, int64_t rows, int c0, int n) {
     const int thread = anew(threadIdx.x), c = thread % kCols * 8, r = thread / kCols;
     if constexpr (FAST) {
-      const int64_t here = rows < ROWS ? rows : ROWS;
+      const int here = rows < ROWS ? static_cast<int>(rows < 0 ? 0 : rows) : ROWS;
       const uint32_t size = sizeof(T), row = static_cast<uint32_t>(st) * size;
-      const Window w = window(src, here > 0 ? (here - 1) * static_cast<int64_t>(row) + n * size : 0);
+      const Window w = window(src, here > 0 ? (here - 1) * row + n * size : 0u);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
-        const int col = static_cast<int>(c0) + c + u * 8 / kUnits;
+        const int col = c0 + c + u * 8 / kUnits;
         const uint32_t at = col < n && !idle(thread) ? r * row + col * size : kPast;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) v[i][u] = load16(w, at + i * kStep * row);
@@ -219,7 +219,7 @@ struct Rows {
     for (int i = 0; i < kPieces; ++i)
 #pragma unroll
       for (int u = 0; u < kUnits; ++u)
-        *reinterpret_cast<v4f*>(lds + Lds<T, W>::at(row(i, thread), c + u * Lds<T, W>::kUnit)) = v[i][u];
+        *reinterpret_cast<v4f*>(lds + Lds<T, W>::at(row(i, thread), u * Lds<T, W>::kUnit, c)) = v[i][u];
   }
   // Each row times its weight (of piece i: weight[i]), as the parts of a Computed operand.
   __device__ __forceinline__ void store_weighted(T (*planes)[ROWS * W], const float (&weight)[kPieces]) const {
@@ -241,7 +241,7 @@ struct Rows {
         }
 #pragma unroll
         for (int u = 0; u < kUnits; ++u)
-          *reinterpret_cast<v4f*>(planes[s] + Lds<T, W>::at(row(i, thread), c + u * Lds<T, W>::kUnit)) =
+          *reinterpret_cast<v4f*>(planes[s] + Lds<T, W>::at(row(i, thread), u * Lds<T, W>::kUnit, c)) =
               reinterpret_cast<const v4f*>(&o)[u];
       }
     }
@@ -250,10 +250,10 @@ struct Rows {
 
 // The same 4 consecutive columns from c on of row `row` of an output [.., n] whose rows are st apart.
 template <bool FAST, typename T>
-__device__ __forceinline__ void put4(Window w, T* base, int64_t row, int64_t st, int c, int64_t n, bool row_there,
+__device__ __forceinline__ void put4(Window w, T* base, int row, int64_t st, int c, int n, bool row_there,
                                      const Pack<T, 4>& x) {
   if constexpr (FAST) {
-    store4(w, c < n ? static_cast<uint32_t>((row * st + c) * sizeof(T)) : kPast, x);
+    store4(w, c < n ? (static_cast<uint32_t>(row) * static_cast<uint32_t>(st) + c) * static_cast<uint32_t>(sizeof(T)) : kPast, x);
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)

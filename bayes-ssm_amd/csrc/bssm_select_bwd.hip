@@ -76,10 +76,10 @@ struct HalfRecord {
   static_assert(kAll % kThreads == 0 || kAll < kThreads, "whole pieces a thread, or one for some");
   v4f v[kPieces];
   template <bool FAST>
-  __device__ __forceinline__ void load(const float* src, int64_t p_first, int64_t np, int64_t n) {
+  __device__ __forceinline__ void load(const float* src, int p_first, int np, int n) {
     src += p_first * n;
-    const int64_t rows = np - p_first < kHalf ? np - p_first : kHalf;
-    const Window w = window(src, rows * n * 4);
+    const int rows = np - p_first < kHalf ? np - p_first : kHalf;
+    const Window w = window(src, static_cast<uint32_t>(rows * n) * 4u);
     const int thread = anew(threadIdx.x);
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) {
@@ -115,7 +115,7 @@ struct HalfRecord {
           o.v[r] = lane::narrow<T>(rest[r]);
           rest[r] -= lane::widen(o.v[r]);
         }
-        lane::store_pack<T, 4>(planes[s] + Lds<T, NP>::at(at / NP, at % NP), o);
+        lane::store_pack<T, 4>(planes[s] + Lds<T, NP>::at(at / NP, 0, at % NP), o);
       }
     }
   }
@@ -155,12 +155,13 @@ __device__ __forceinline__ void inside(const Tiles<T, NP>& t, int block, v16f (&
   for (int k = 0; k < NP / kDepth; ++k) n_own[k] = along<NP>(own_n, own, k * kDepth, g);
 #pragma unroll 1
   for (int blk = AS_I ? 0 : block; blk <= (AS_I ? block : kBlocks - 1); ++blk) {
+    const int here = anew(own);  // 16 registers less than kept operands would take
     v16f s = zeros(), gx = zeros();
 #pragma unroll
     for (int k = 0; k < NP / kDepth; ++k) mma(s, along<NP>(other_n, blk * kTile + ln % 32, k * kDepth, g), n_own[k]);
 #pragma unroll
     for (int k = 0; k < kTileP / kDepth; ++k)
-      mma(gx, along<kTileP>(other_p, blk * kTile + ln % 32, k * kDepth, g), along<kTileP>(own_p, own, k * kDepth, g));
+      mma(gx, along<kTileP>(other_p, blk * kTile + ln % 32, k * kDepth, g), along<kTileP>(own_p, here, k * kDepth, g));
     Operand<T> es[2], eg[2];
     if (blk != block) {
       // Border between the blocks: the end of the rows' block (AS_I) or its start.
@@ -246,7 +247,7 @@ __device__ __forceinline__ void outside(const Tiles<T, NP>& t, int block, int ha
   float dot = 0.f;
 #pragma unroll
   for (int r = 0; r < 16; r += 4) {
-    const Pack<T, 4> v = lane::load_pack<T, 4>(own_p + Lds<T, kTileP>::at(own, half * kHalf + result_row(r, g)));
+    const Pack<T, 4> v = lane::load_pack<T, 4>(own_p + Lds<T, kTileP>::at(own, half * kHalf + result_row(r, 0), 4 * g));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       dot = fmaf(z[r + e], lane::widen(v.v[e]), dot);
@@ -285,47 +286,58 @@ __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts
   {
     Rows<T, L, NP, kThreads> rows;
     rows.template load<FAST>(static_cast<const T*>(a.bk) + b * a.bk_batch + grp * a.bk_group + t0 * a.bk_row, a.bk_row,
-                             live, 0, a.n);
+                             live, 0, static_cast<int>(a.n));
     rows.store(t.ks);
     rows.template load<FAST>(static_cast<const T*>(a.cq) + b * a.cq_batch + grp * a.cq_group + t0 * a.cq_row, a.cq_row,
-                             live, 0, a.n);
+                             live, 0, static_cast<int>(a.n));
     rows.store(t.qs);
   }
   v16f acc[NP / kTile];  // gradient of C (as i) or B (as j), transposed: rows n, column own
 #pragma unroll
   for (int n = 0; n < NP / kTile; ++n) acc[n] = zeros();
 
+  // The head's streams; the loops move them on by a head.
+  const int np = static_cast<int>(a.p), nn = static_cast<int>(a.n);
+  const T *x = static_cast<const T*>(a.x) + b * a.x_batch + t0 * a.x_row + h_first * a.x_head,
+          *gy = static_cast<const T*>(a.gy) + ((b * a.t + t0) * a.h + h_first) * a.p;
+  const int64_t gy_row = a.h * a.p, rec_step = records * pn;
+  const float *h_rec = a.states + ((b * a.h + h_first) * records + rec) * pn,
+              *gh_rec = a.adjoints + ((b * a.h + h_first) * records + rec) * pn;
+  T* gx = static_cast<T*>(a.gx) + ((b * a.t + t0) * a.h + h_first) * a.p;
+  const int rows = a.t - t0 < L ? static_cast<int>(a.t - t0) : L;
+  Steps steps(a, b, h_first);
+  const int64_t tp = (a.t + kSpan - 1) / kSpan * kSpan;
+  TokenSums to(a, b, h_first, records, kWaves);
+  const int64_t waves_step = records * kWaves;
   Rows<T, L, kTileP, kThreads> rx, rg;
   HalfRecord<T, NP> rh, rgh;
   float r_step = 0.f, r_near = 0.f, r_near_end = 0.f;  // of token threadIdx.x
   double r_base = 0., r_start = 0., r_end = 0.;
-  auto load_half = [&](int64_t h, int64_t p_first) {
-    rh.template load<FAST>(a.states + ((b * a.h + h) * records + rec) * pn, p_first, a.p, a.n);
-    rgh.template load<FAST>(a.adjoints + ((b * a.h + h) * records + rec) * pn, p_first, a.p, a.n);
+  auto load_half = [&](int p_first) {
+    rh.template load<FAST>(h_rec, p_first, np, nn);
+    rgh.template load<FAST>(gh_rec, p_first, np, nn);
   };
-  auto load = [&](int64_t h, int64_t p0) {
-    rx.template load<FAST>(static_cast<const T*>(a.x) + b * a.x_batch + t0 * a.x_row + h * a.x_head, a.x_row, live, p0,
-                           a.p);
-    rg.template load<FAST>(static_cast<const T*>(a.gy) + ((b * a.t + t0) * a.h + h) * a.p, a.h * a.p, live, p0, a.p);
-    load_half(h, p0);
+  auto load = [&](int p0) {
+    rx.template load<FAST>(x, a.x_row, live, p0, np);
+    rg.template load<FAST>(gy, gy_row, live, p0, np);
+    load_half(p0);
     const int at = anew(threadIdx.x);
     if (at < L) {
-      const Steps s(a, b, h);
       const int first = at / kTile * kTile;
-      r_step = s.step[t0 + at];
-      r_near = s.near[t0 + at];
-      r_near_end = s.near[t0 + first + kTile - 1];
-      r_base = s.base[(t0 + at) / kNear];
-      r_start = s.base[(t0 + first) / kNear];
-      r_end = s.base[(t0 + first) / kNear + kTile / kNear - 1];
+      r_step = steps.step[t0 + at];
+      r_near = steps.near[t0 + at];
+      r_near_end = steps.near[t0 + first + kTile - 1];
+      r_base = steps.base[(t0 + at) / kNear];
+      r_start = steps.base[(t0 + first) / kNear];
+      r_end = steps.base[(t0 + first) / kNear + kTile / kNear - 1];
     }
   };
-  load(h_first, 0);
+  load(0);
   for (int64_t h = h_first; h < h_last; ++h) {
     const float skip = a.skip == nullptr ? 0.f : a.skip[h];
     Own sum{0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     float dot_h = 0.f;
-    for (int64_t p0 = 0; p0 < a.p; p0 += kTileP) {
+    for (int p0 = 0; p0 < np; p0 += kTileP) {
       __syncthreads();
       rx.store(t.xs);
       rg.store(t.gs);
@@ -340,8 +352,8 @@ __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts
         if (at % kNear == 0) t.base[at / kNear] = r_base;
       }
       __syncthreads();
-      const bool second = p0 + kHalf < a.p;
-      if (second) load_half(h, p0 + kHalf);
+      const bool second = p0 + kHalf < np;
+      if (second) load_half(p0 + kHalf);
       v16f gu[kTileP / kTile];  // rows p, column own (as j)
 #pragma unroll
       for (int m = 0; m < kTileP / kTile; ++m) gu[m] = zeros();
@@ -357,33 +369,41 @@ __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts
           __syncthreads();
         }
         if (half == (second ? 1 : 0)) {
-          const bool more = p0 + kTileP < a.p;
-          if (more || h + 1 < h_last) load(more ? h : h + 1, more ? p0 + kTileP : 0);
+          const bool more = p0 + kTileP < np;
+          if (!more) {
+            x += a.x_head;
+            gy += np;
+            h_rec += rec_step;
+            gh_rec += rec_step;
+            steps.step += tp;
+            steps.near += tp;
+            steps.base += tp / kNear;
+          }
+          if (more || h + 1 < h_last) load(more ? p0 + kTileP : 0);
         }
         outside<T, NP, AS_I>(t, block, half, acc, gu[half], sum);
       }
       if (!AS_I) {
         const int ln = anew(threadIdx.x % kWave), g = ln / 32, own = block * kTile + ln % 32;
         const float d_own = t.step[own];
-        const int64_t row = a.h * a.p, rows = a.t - t0 < L ? a.t - t0 : L, cols = a.p - p0;
-        T* out = static_cast<T*>(a.gx) + (b * a.t + t0) * row + h * a.p + p0;
-        const Window w = window(out, ((rows - 1) * row + cols) * sizeof(T));
+        const int cols = np - p0;
+        T* out = gx + p0;
+        const Window w = window(out, ((rows - 1) * static_cast<uint32_t>(gy_row) + cols) * static_cast<uint32_t>(sizeof(T)));
 #pragma unroll
         for (int m = 0; m < kTileP / kTile; ++m)
 #pragma unroll
           for (int r = 0; r < 16; r += 4) {
-            const int c0 = m * kTile + result_row(r, g);
-            const Pack<T, 4> gi = lane::load_pack<T, 4>(t.gs + Lds<T, kTileP>::at(own, c0));
+            const int c0 = m * kTile + result_row(r, 0);
+            const Pack<T, 4> gi = lane::load_pack<T, 4>(t.gs + Lds<T, kTileP>::at(own, c0, 4 * g));
             Pack<T, 4> o;
 #pragma unroll
             for (int e = 0; e < 4; ++e) o.v[e] = lane::narrow<T>(fmaf(d_own, gu[m][r + e], skip * lane::widen(gi.v[e])));
-            put4<FAST>(w, out, own, row, c0, cols, own < rows, o);
+            put4<FAST>(w, out, own, gy_row, c0 + 4 * g, cols, own < rows, o);
           }
       }
     }
     // The head's token sums: the two halves of a column hold parts of them.
     const int ln = anew(threadIdx.x % kWave), g = ln / 32, own = block * kTile + ln % 32;
-    const TokenSums to(a, b, h, records, kWaves);
     auto both = [](float v) { return v + __shfl_xor(v, 32, kWave); };
     if (AS_I) {
       const float later = both(sum.row + sum.from_h);
@@ -397,11 +417,18 @@ __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts
         to.diagonal[t0 + own] = diagonal;
       }
     }
-    const float whole = lane::lanes_sum(dot_h), gx = lane::lanes_sum(sum.dot_x);
+    const float whole = lane::lanes_sum(dot_h), dot_x = lane::lanes_sum(sum.dot_x);
     if (ln == 0) {
       to.whole[rec * kWaves + wave] = whole;
-      to.skip[rec * kWaves + wave] = gx;
+      to.skip[rec * kWaves + wave] = dot_x;
     }
+    to.later += tp;
+    to.earlier += tp;
+    to.direct += tp;
+    to.diagonal += tp;
+    to.whole += waves_step;
+    to.skip += waves_step;
+    gx += np;
   }
   const int ln = threadIdx.x % kWave, g = ln / 32, own = block * kTile + ln % 32;
   if (t0 + own >= a.t) return;
@@ -507,7 +534,7 @@ __global__ __launch_bounds__(256) void parts_kernel(SelectArgs a, int64_t parts)
   out[i < all ? i : i - all] = lane::narrow<T>(s);
 }
 
-__global__ __launch_bounds__(256) void heads_kernel(SelectArgs a, int64_t rows) {
+__global__ __launch_bounds__(lane::kFoldThreads) void heads_kernel(SelectArgs a, int64_t rows) {
   lane::fold_columns(a.rows, rows, 3 * a.h, blockIdx.x, [&](int64_t c, float s) {
     float* out = c < a.h ? a.grate : c < 2 * a.h ? a.gskip : a.gdt_bias;
     if (out != nullptr) out[c % a.h] = s;
@@ -532,8 +559,7 @@ hipError_t launch(const SelectArgs& a, hipStream_t stream) {
       hipLaunchKernelGGL(parts_kernel<T>, dim3(static_cast<unsigned>((all + 255) / 256)), dim3(256), 0, stream, a, parts);
     }
   }
-  hipLaunchKernelGGL(heads_kernel, dim3(static_cast<unsigned>((3 * a.h + lane::kFoldColumns - 1) / lane::kFoldColumns)),
-                     dim3(256), 0, stream, a, a.b * records);
+  hipLaunchKernelGGL(heads_kernel, dim3(lane::fold_blocks(3 * a.h)), dim3(lane::kFoldThreads), 0, stream, a, a.b * records);
   return hipGetLastError();
 }
 

@@ -105,10 +105,10 @@ struct State {
   }
   // One [P, N] state of memory, P from p0 on.
   template <bool FAST>
-  __device__ __forceinline__ void add(const float* src, int64_t p0, int64_t np, int64_t n) {
+  __device__ __forceinline__ void add(const float* src, int p0, int np, int n) {
     if (src == nullptr) return;
-    src += p0 * n;
-    const Window w = window(src, (np - p0 < kTileP ? np - p0 : kTileP) * n * 4);
+    src += static_cast<int64_t>(p0) * n;
+    const Window w = window(src, static_cast<uint32_t>(np - p0 < kTileP ? np - p0 : kTileP) * n * 4u);
     each([&](v16f& t, int r, int c) {
       if constexpr (FAST) {
         const v4f o = load16(w, c < n ? static_cast<uint32_t>(p * n + c) * 4u : kPast);
@@ -122,9 +122,9 @@ struct State {
     });
   }
   template <bool FAST>
-  __device__ __forceinline__ void store(float* dst, int64_t p0, int64_t np, int64_t n) {
-    dst += p0 * n;
-    const Window w = window(dst, (np - p0 < kTileP ? np - p0 : kTileP) * n * 4);
+  __device__ __forceinline__ void store(float* dst, int p0, int np, int n) {
+    dst += static_cast<int64_t>(p0) * n;
+    const Window w = window(dst, static_cast<uint32_t>(np - p0 < kTileP ? np - p0 : kTileP) * n * 4u);
     each([&](v16f& t, int r, int c) {
       put4<FAST>(w, dst, p, n, c, n, p0 + p < np, Pack<float, 4>{{t[r], t[r + 1], t[r + 2], t[r + 3]}});
     });
@@ -135,7 +135,7 @@ struct State {
       Pack<T, 4> o;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o.v[e] = lane::narrow<T>(t[r + e]);
-      lane::store_pack<T, 4>(lds + Lds<T, NP>::at(p, c), o);
+      lane::store_pack<T, 4>(lds + Lds<T, NP>::at(p, c - 4 * g, 4 * g), o);
     });
   }
   // state = fade * state + sum_j k_j (w_j u_j)^T over the chunk's tokens j, w_j u_j in parts.
@@ -179,11 +179,13 @@ struct ChunkLoad {
       near[i] = s.near[t0 + r];
       base[i] = s.base[t0 / kNear + r / kNear];
     }
-    first = s.base[t0 / kNear];
-    half = s.base[t0 / kNear + kTile / kNear - 1];
-    last = s.base[t0 / kNear + kChunk / kNear - 1];
-    near_half = s.near[t0 + kTile - 1];
-    near_end = s.near[t0 + kChunk - 1];
+    // Through the vector unit like the rest: a scalar load's wait would hold up every LDS read that follows it.
+    const int none = anew(0);
+    first = s.base[t0 / kNear + none];
+    half = s.base[t0 / kNear + kTile / kNear - 1 + none];
+    last = s.base[t0 / kNear + kChunk / kNear - 1 + none];
+    near_half = s.near[t0 + kTile - 1 + none];
+    near_end = s.near[t0 + kChunk - 1 + none];
   }
   // log2 of the whole chunk's decay
   __device__ __forceinline__ float fade() const { return static_cast<float>(last - first + near_end); }
@@ -210,7 +212,8 @@ struct ChunkLoad {
 };
 
 struct Block {
-  int64_t b, h, p0, seg, first, last;  // chunks [first, last)
+  int64_t b, h, seg, first, last;  // chunks [first, last)
+  int p0, np, n;                   // first value of P, P, N
   __device__ __forceinline__ Block(const SelectArgs& a, int64_t segs) {
     // Sequences vary fastest, then segments: workgroups of one B and C meet on one XCD's L2.
     int64_t i = blockIdx.x;
@@ -219,7 +222,9 @@ struct Block {
     seg = i % segs;
     i /= segs;
     h = i % a.h;
-    p0 = i / a.h * kTileP;
+    p0 = static_cast<int>(i / a.h) * kTileP;
+    np = static_cast<int>(a.p);
+    n = static_cast<int>(a.n);
     const int64_t chunks = (a.t + kChunk - 1) / kChunk;
     // Whole records a segment.
     const int64_t per = ((chunks + segs - 1) / segs + 1) / 2 * 2;
@@ -248,6 +253,7 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t
   const T* x = static_cast<const T*>(a.x) + at.b * a.x_batch + at.h * a.x_head;
   const T* bk = static_cast<const T*>(a.bk) + at.b * a.bk_batch + grp * a.bk_group;
   const T* cq = static_cast<const T*>(a.cq) + at.b * a.cq_batch + grp * a.cq_group;
+  T* y_out = static_cast<T*>(a.y) + at.b * a.t * a.h * a.p + at.h * a.p + at.p0;
   const float skip = a.skip == nullptr ? 0.f : a.skip[at.h];
   const int64_t pn = a.p * a.n;
   const int64_t record = sizeof(T) == 2 ? kRecordsB16 : kRecordsF32, ratio = record / kChunk,
@@ -255,10 +261,10 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t
   const Steps steps(a, at.b, at.h);
   State<NP> st(wave);
   if (carries) {
-    st.template add<FAST>(a.state0 == nullptr ? nullptr : a.state0 + bh * pn, at.p0, a.p, a.n);
+    st.template add<FAST>(a.state0 == nullptr ? nullptr : a.state0 + bh * pn, at.p0, at.np, at.n);
     for (int64_t s = 0; s < at.seg; ++s) {
       st.scale(*segment_fade(a, segs, s, at.b, at.h));
-      st.template add<FAST>(segment_state(a, s, at.b, at.h), at.p0, a.p, a.n);
+      st.template add<FAST>(segment_state(a, s, at.b, at.h), at.p0, at.np, at.n);
     }
   }
   typedef Rows<T, kChunk, kTileP, kThreads> RowsX;
@@ -267,16 +273,14 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t
   ChunkLoad<RowsX> rs;
   auto load = [&](int64_t c) {
     const int64_t t0 = c * kChunk, live = n_live - t0;
-    rx.template load<FAST>(x + t0 * a.x_row, a.x_row, live, at.p0, a.p);
-    rk.template load<FAST>(bk + t0 * a.bk_row, a.bk_row, live, 0, a.n);
-    rq.template load<FAST>(cq + t0 * a.cq_row, a.cq_row, live, 0, a.n);
+    rx.template load<FAST>(x + t0 * a.x_row, a.x_row, live, at.p0, at.np);
+    rk.template load<FAST>(bk + t0 * a.bk_row, a.bk_row, live, 0, at.n);
+    rq.template load<FAST>(cq + t0 * a.cq_row, a.cq_row, live, 0, at.n);
     rs.load(steps, t0);
   };
   if (at.first < at.last) load(at.first);
   for (int64_t c = at.first; c < at.last; ++c) {
     const int64_t t0 = c * kChunk, live = n_live - t0;
-    if (carries && a.states != nullptr && c % ratio == 0)
-      st.template store<FAST>(a.states + (bh * records + c / ratio) * pn, at.p0, a.p, a.n);
     __syncthreads();
     if (carries) st.to_lds(hs);
     float weight[RowsX::kPieces];
@@ -288,6 +292,8 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t
     rs.store(cs);
     const float fade = rs.fade();
     __syncthreads();
+    if (carries && a.states != nullptr && c % ratio == 0)
+      st.template store<FAST>(a.states + (bh * records + c / ratio) * pn, at.p0, at.np, at.n);
     if (c + 1 < at.last) load(c + 1);
     if (carries) {
       st.advance(wx, ks, lane::exp2_(fade), wave);
@@ -343,25 +349,25 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t
         mma(y, across<true, kTileP>(xs, j0, pb * kTile, ln), m);
       }
     }
-    const int64_t y_row = a.h * a.p, y_rows = a.t - t0 < kChunk ? a.t - t0 : kChunk;
-    T* out = static_cast<T*>(a.y) + (at.b * a.t + t0) * y_row + at.h * a.p + at.p0;
-    const int64_t cols = a.p - at.p0;
-    const Window w = window(out, ((y_rows - 1) * y_row + cols) * sizeof(T));
+    const int64_t y_row = a.h * a.p;
+    const int y_rows = a.t - t0 < kChunk ? static_cast<int>(a.t - t0) : kChunk, cols = at.np - at.p0;
+    T* out = y_out + t0 * y_row;
+    const Window w = window(out, ((y_rows - 1) * static_cast<uint32_t>(y_row) + cols) * static_cast<uint32_t>(sizeof(T)));
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
-      const int c0 = pb * kTile + result_row(r, g);
-      const Pack<T, 4> xi = lane::load_pack<T, 4>(xs + Lds<T, kTileP>::at(own, c0));
+      const int c0 = pb * kTile + result_row(r, 0);
+      const Pack<T, 4> xi = lane::load_pack<T, 4>(xs + Lds<T, kTileP>::at(own, c0, 4 * g));
       Pack<T, 4> o;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float v = fmaf(skip, lane::widen(xi.v[e]), y[r + e]);
         o.v[e] = lane::narrow<T>(own < live ? v : 0.f);
       }
-      put4<FAST>(w, out, own, y_row, c0, cols, own < y_rows, o);
+      put4<FAST>(w, out, own, y_row, c0 + 4 * g, cols, own < y_rows, o);
     }
   }
   if (carries && at.seg == segs - 1 && a.state_out != nullptr)
-    st.template store<FAST>(a.state_out + bh * pn, at.p0, a.p, a.n);
+    st.template store<FAST>(a.state_out + bh * pn, at.p0, at.np, at.n);
 }
 
 // The state alone, along a segment.  Forward (BACK false): from zero, into the
@@ -388,10 +394,10 @@ __global__ __launch_bounds__(kCarryThreads, sizeof(T) == 2 ? 2 : 1) void carry_k
   State<NP> st(wave);
   float total = 0.f;
   if constexpr (!LOCAL) {
-    st.template add<FAST>(a.gstate_out == nullptr ? nullptr : a.gstate_out + bh * pn, at.p0, a.p, a.n);
+    st.template add<FAST>(a.gstate_out == nullptr ? nullptr : a.gstate_out + bh * pn, at.p0, at.np, at.n);
     for (int64_t s = segs - 1; s > at.seg; --s) {
       st.scale(*segment_fade(a, segs, s, at.b, at.h));
-      st.template add<FAST>(segment_state(a, s, at.b, at.h), at.p0, a.p, a.n);
+      st.template add<FAST>(segment_state(a, s, at.b, at.h), at.p0, at.np, at.n);
     }
   }
   typedef Rows<T, kChunk, kTileP, kCarryThreads> RowsU;
@@ -402,15 +408,13 @@ __global__ __launch_bounds__(kCarryThreads, sizeof(T) == 2 ? 2 : 1) void carry_k
   auto chunk = [&](int64_t i) { return BACK ? at.last - 1 - i : at.first + i; };
   auto load = [&](int64_t c) {
     const int64_t t0 = c * kChunk, live = n_live - t0;
-    ru.template load<FAST>(u + t0 * u_row, u_row, live, at.p0, a.p);
-    rk.template load<FAST>(k + t0 * k_row, k_row, live, 0, a.n);
+    ru.template load<FAST>(u + t0 * u_row, u_row, live, at.p0, at.np);
+    rk.template load<FAST>(k + t0 * k_row, k_row, live, 0, at.n);
     rs.load(steps, t0);
   };
   if (count > 0) load(chunk(0));
   for (int64_t i = 0; i < count; ++i) {
     const int64_t c = chunk(i);
-    if (!LOCAL && (c % ratio == ratio - 1 || c == chunks - 1))
-      st.template store<FAST>(a.adjoints + (bh * records + c / ratio) * pn, at.p0, a.p, a.n);
     __syncthreads();
     float weight[RowsU::kPieces];
     rs.template weights<BACK>(weight);
@@ -418,15 +422,17 @@ __global__ __launch_bounds__(kCarryThreads, sizeof(T) == 2 ? 2 : 1) void carry_k
     rk.store(ks);
     const float fade = rs.fade();
     __syncthreads();
+    if (!LOCAL && (c % ratio == ratio - 1 || c == chunks - 1))
+      st.template store<FAST>(a.adjoints + (bh * records + c / ratio) * pn, at.p0, at.np, at.n);
     if (i + 1 < count) load(chunk(i + 1));
     total += fade;
     st.advance(wu, ks, lane::exp2_(fade), wave);
   }
   if constexpr (LOCAL) {
-    st.template store<FAST>(segment_state(a, at.seg, at.b, at.h), at.p0, a.p, a.n);
+    st.template store<FAST>(segment_state(a, at.seg, at.b, at.h), at.p0, at.np, at.n);
     if (threadIdx.x == 0 && at.p0 == 0) *segment_fade(a, segs, at.seg, at.b, at.h) = lane::exp2_(total);
   } else if (at.seg == 0 && a.gstate0 != nullptr) {
-    st.template store<FAST>(a.gstate0 + bh * pn, at.p0, a.p, a.n);
+    st.template store<FAST>(a.gstate0 + bh * pn, at.p0, at.np, at.n);
   }
 }
 

@@ -26,7 +26,7 @@ struct ShortConvArgs {
   int64_t b, t, c;
   int w, bf16, param_bf16, silu;
 };
-int64_t short_conv_partial_rows(int64_t b, int64_t t, int64_t c, int bf16);
+int64_t short_conv_partial_rows(int64_t b, int64_t t, int64_t c);
 hipError_t launch_short_conv_forward(const ShortConvArgs& a, hipStream_t stream);
 hipError_t launch_short_conv_backward(const ShortConvArgs& a, hipStream_t stream);
 
@@ -56,14 +56,16 @@ struct DistillArgs {
   int64_t logits_row;            // row stride in elements
   const void* teacher;           // [R, K]
   const int64_t* index;          // [R, K]
-  float *loss, *lse;             // [R]; lse [R, 3]: maximum, sum of exponentials, 1 if the row has a teacher
+  float *loss, *stats;           // [R], [R, 3]: maximum, sum of exponentials, 1 if the row has a teacher
+  float* counts;                 // workspace of distill_count_floats, where the forward divides its gradient by the rows
   float* mean;                   // [3] or null: mean, 1 / rows with a teacher, sum
   const float* upstream;         // [R] or (upstream_scalar) [1]
-  void* grad;                    // [R, V]
+  void* grad;                    // [R, V]; null in a forward without gradient
   int64_t r, v, k;
   float tau;
-  int bf16, teacher_bf16, upstream_scalar;
+  int bf16, teacher_bf16, upstream_scalar, mean_of_rows, ready;
 };
+int64_t distill_count_floats();
 hipError_t launch_distill_forward(const DistillArgs& a, hipStream_t stream);
 hipError_t launch_distill_backward(const DistillArgs& a, hipStream_t stream);
 

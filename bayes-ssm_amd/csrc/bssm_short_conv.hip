@@ -10,9 +10,10 @@
 // The reverse computes pre again from x: that costs W multiply-adds, where
 // keeping it would cost a write and a read of the whole stream.
 //
-// Bound by memory: one read and one write a stream.  A thread owns a 16-byte
-// group of channels (one channel where C, the strides or an address do not
-// allow that) and walks a segment of tokens with the last W - 1 rows in
+// Bound by memory: one read and one write a stream.  A thread owns a group of
+// channels, 16 bytes of them (8 in the bfloat16 reverse, whose windows of x and
+// g and whose sums would leave two waves a SIMD with 16; one channel where C,
+// the strides or an address do not allow that) and walks a segment of tokens with the last W - 1 rows in
 // registers, so only the W - 1 rows in front of a segment (and, in the
 // reverse, behind it) are read twice.
 #include "bssm_lane.h"
@@ -27,15 +28,16 @@ using lane::kWave;
 
 constexpr int kWaves = 4;
 
-__device__ __forceinline__ int64_t row_length(const ShortConvArgs& a, int64_t b) {
-  if (a.lengths == nullptr) return a.t;
+__device__ __forceinline__ int row_length(const ShortConvArgs& a, int64_t b) {
+  const int t = static_cast<int>(a.t);
+  if (a.lengths == nullptr) return t;
   const int64_t n = a.lengths[b];
-  return n < 0 ? 0 : n > a.t ? a.t : n;
+  return n < 0 ? 0 : n > t ? t : static_cast<int>(n);
 }
 
 // Channels [c0, c0 + N) of input row t (t may lie before the sequence).
 template <typename T, int N, int W>
-__device__ __forceinline__ void input_row(const ShortConvArgs& a, int64_t b, int64_t t, int64_t c0, float (&x)[N]) {
+__device__ __forceinline__ void input_row(const ShortConvArgs& a, int64_t b, int t, int64_t c0, float (&x)[N]) {
   const T* p = nullptr;
   if (t >= 0) p = static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_row + c0;
   else if (a.state != nullptr) p = static_cast<const T*>(a.state) + (b * (W - 1) + t + W - 1) * a.c + c0;
@@ -68,19 +70,20 @@ __global__ __launch_bounds__(256) void forward_kernel(ShortConvArgs a, int seg) 
   const int64_t groups = a.c / N, segs = a.t > 0 ? (a.t + seg - 1) / seg : 1;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (id >= a.b * segs * groups) return;
-  const int64_t c0 = id % groups * N, s = id / groups % segs, b = id / groups / segs;
-  const int64_t n = row_length(a, b), t0 = s * seg, t1 = t0 + seg < a.t ? t0 + seg : a.t;
+  const int64_t c0 = id % groups * N, b = id / groups / segs;
+  const int s = static_cast<int>(id / groups % segs), end = static_cast<int>(a.t);
+  const int n = row_length(a, b), t0 = s * seg, t1 = t0 + seg < end ? t0 + seg : end;
   const Taps<N, W> k(a, c0);
   float h[W][N];  // h[j] = x[t - W + 1 + j]
 #pragma unroll
   for (int j = 1; j < W; ++j) input_row<T, N, W>(a, b, t0 - W + j, c0, h[j]);
   T* y = static_cast<T*>(a.y) + b * a.t * a.c + c0;
   const T* x = static_cast<const T*>(a.x) + b * a.x_batch + c0;
-  for (int64_t t = t0; t < t1; t += kAhead) {
+  for (int t = t0; t < t1; t += kAhead) {
     Pack<T, N> raw[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (t + u < t1) raw[u] = lane::load_pack<T, N>(x + (t + u) * a.x_row);
+      if (t + u < t1) raw[u] = lane::load_pack<T, N>(x + static_cast<int64_t>(t + u) * a.x_row);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (t + u >= t1) break;
@@ -96,7 +99,7 @@ __global__ __launch_bounds__(256) void forward_kernel(ShortConvArgs a, int seg) 
         if (a.silu) p *= lane::sigmoid_(p);
         out.v[i] = lane::narrow<T>(t + u < n ? p : 0.f);
       }
-      lane::store_pack<T, N>(y + (t + u) * a.c, out);
+      lane::store_pack<T, N>(y + static_cast<int64_t>(t + u) * a.c, out);
     }
   }
   if (s == 0 && a.final_state != nullptr) {
@@ -122,7 +125,8 @@ __global__ __launch_bounds__(kWave * kWaves) void backward_kernel(ShortConvArgs 
   const int wave = threadIdx.x / kWave, ln = threadIdx.x % kWave;
   const int64_t groups = a.c / N, cblocks = (groups + kWave - 1) / kWave;
   const int64_t g = blockIdx.x % cblocks * kWave + ln, part = blockIdx.x / cblocks;
-  const int64_t b = part / blocks_t, t0 = (part % blocks_t * kWaves + wave) * seg;
+  const int64_t b = part / blocks_t;
+  const int t0 = (static_cast<int>(part % blocks_t) * kWaves + wave) * seg, t_end = static_cast<int>(a.t);
   const bool active = g < groups;
   const int64_t c0 = (active ? g : 0) * N;
   float gw[W + 1][N];
@@ -130,8 +134,8 @@ __global__ __launch_bounds__(kWave * kWaves) void backward_kernel(ShortConvArgs 
   for (int j = 0; j <= W; ++j)
 #pragma unroll
     for (int i = 0; i < N; ++i) gw[j][i] = 0.f;
-  if (active && (t0 < a.t || (t0 == 0 && a.gstate != nullptr))) {
-    const int64_t n = row_length(a, b), t1 = t0 + seg < a.t ? t0 + seg : a.t;
+  if (active && (t0 < t_end || (t0 == 0 && a.gstate != nullptr))) {
+    const int n = row_length(a, b), t1 = t0 + seg < t_end ? t0 + seg : t_end;
     const Taps<N, W> k(a, c0);
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch + c0;
     const T* gy = static_cast<const T*>(a.gy) + b * a.t * a.c + c0;
@@ -147,24 +151,24 @@ __global__ __launch_bounds__(kWave * kWaves) void backward_kernel(ShortConvArgs 
 #pragma unroll
         for (int i = 0; i < N; ++i) h[j][i] = 0.f;
     }
-    const int64_t end = t1 + W - 1;
-    for (int64_t t = t0; t < end; t += kAhead) {
+    const int end = t1 + W - 1;
+    for (int t = t0; t < end; t += kAhead) {
       Pack<T, N> rx[kAhead], rg[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
         if (t + u < n && t + u < end) {
-          rx[u] = lane::load_pack<T, N>(x + (t + u) * a.x_row);
-          if (a.gy != nullptr) rg[u] = lane::load_pack<T, N>(gy + (t + u) * a.c);
+          rx[u] = lane::load_pack<T, N>(x + static_cast<int64_t>(t + u) * a.x_row);
+          if (a.gy != nullptr) rg[u] = lane::load_pack<T, N>(gy + static_cast<int64_t>(t + u) * a.c);
         }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int64_t tt = t + u;
+        const int tt = t + u;
         if (tt >= end) break;
         const bool live = tt < n, mine = tt < t1;
-        const int64_t s = tt - (W - 1);
+        const int s = tt - (W - 1);
         Pack<T, N> out;
         float gf[N];
-        const int64_t jf = s - n + W - 1;  // row of the final state that input s is
+        const int jf = s - n + W - 1;  // row of the final state that input s is
         const bool from_final = a.gfinal != nullptr && jf >= 0 && jf < W - 1;
         if (from_final) {
           const Pack<T, N> r = lane::load_pack<T, N>(static_cast<const T*>(a.gfinal) + (b * (W - 1) + jf) * a.c + c0);
@@ -225,7 +229,7 @@ __global__ __launch_bounds__(kWave * kWaves) void backward_kernel(ShortConvArgs 
   }
 }
 
-__global__ __launch_bounds__(256) void fold_kernel(ShortConvArgs a, int64_t rows) {
+__global__ __launch_bounds__(lane::kFoldThreads) void fold_kernel(ShortConvArgs a, int64_t rows) {
   lane::fold_columns(a.partials, rows, a.c * (a.w + 1), blockIdx.x, [&](int64_t col, float sum) {
     const int64_t j = col / a.c, c = col % a.c;
     if (j < a.w) {
@@ -273,36 +277,35 @@ template <typename T, int N, int W>
 hipError_t backward(const ShortConvArgs& a, hipStream_t stream) {
   const int64_t groups = a.c / N, cblocks = (groups + kWave - 1) / kWave;
   // The segment follows from the sizes alone, so that the partial rows do.
-  const int seg = backward_segment(a.b, a.t, a.c / (a.bf16 ? 8 : 4) + 1);
+  const int seg = backward_segment(a.b, a.t, a.c / 4 + 1);
   const int64_t blocks_t = (a.t + kWaves * seg - 1) / (kWaves * seg), bt = blocks_t > 0 ? blocks_t : 1;
   hipLaunchKernelGGL((backward_kernel<T, N, W>), dim3(static_cast<unsigned>(a.b * bt * cblocks)), dim3(kWave * kWaves),
                      0, stream, a, seg, bt);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (a.gweight == nullptr && a.gbias == nullptr) return hipSuccess;
-  const int64_t cols = a.c * (a.w + 1);
-  hipLaunchKernelGGL(fold_kernel, dim3(static_cast<unsigned>((cols + lane::kFoldColumns - 1) / lane::kFoldColumns)),
-                     dim3(256), 0, stream, a, a.b * bt);
+  hipLaunchKernelGGL(fold_kernel, dim3(lane::fold_blocks(a.c * (a.w + 1))), dim3(lane::kFoldThreads), 0, stream, a,
+                     a.b * bt);
   return hipGetLastError();
 }
 
-template <typename T, int N>
+template <typename T, int N, int NB>
 hipError_t taps(const ShortConvArgs& a, bool back, hipStream_t stream) {
   switch (a.w) {
-    case 2: return back ? backward<T, N, 2>(a, stream) : forward<T, N, 2>(a, stream);
-    case 3: return back ? backward<T, N, 3>(a, stream) : forward<T, N, 3>(a, stream);
-    default: return back ? backward<T, N, 4>(a, stream) : forward<T, N, 4>(a, stream);
+    case 2: return back ? backward<T, NB, 2>(a, stream) : forward<T, N, 2>(a, stream);
+    case 3: return back ? backward<T, NB, 3>(a, stream) : forward<T, N, 3>(a, stream);
+    default: return back ? backward<T, NB, 4>(a, stream) : forward<T, N, 4>(a, stream);
   }
 }
 hipError_t types(const ShortConvArgs& a, bool back, hipStream_t stream) {
-  if (vectors(a)) return a.bf16 ? taps<__bf16, 8>(a, back, stream) : taps<float, 4>(a, back, stream);
-  return a.bf16 ? taps<__bf16, 1>(a, back, stream) : taps<float, 1>(a, back, stream);
+  if (vectors(a)) return a.bf16 ? taps<__bf16, 8, 4>(a, back, stream) : taps<float, 4, 4>(a, back, stream);
+  return a.bf16 ? taps<__bf16, 1, 1>(a, back, stream) : taps<float, 1, 1>(a, back, stream);
 }
 
 }  // namespace
 }  // namespace short_conv
 
-int64_t short_conv_partial_rows(int64_t b, int64_t t, int64_t c, int bf16) {
-  const int seg = short_conv::backward_segment(b, t, c / (bf16 ? 8 : 4) + 1);
+int64_t short_conv_partial_rows(int64_t b, int64_t t, int64_t c) {
+  const int seg = short_conv::backward_segment(b, t, c / 4 + 1);
   const int64_t n = (t + short_conv::kWaves * seg - 1) / (short_conv::kWaves * seg);
   return b * (n > 0 ? n : 1);
 }

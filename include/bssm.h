@@ -689,7 +689,7 @@ int bssm_short_conv_backward(int bf16, int param_bf16, int width, int silu, cons
                              const int64_t* lengths, const void* grad_y, const void* grad_final_state, void* grad_x,
                              void* grad_state, float* partials, void* grad_weight, void* grad_bias, int64_t batch,
                              int64_t t, int64_t channels, void* stream);
-int64_t bssm_short_conv_partial_rows(int bf16, int64_t batch, int64_t t, int64_t channels);
+int64_t bssm_short_conv_partial_rows(int64_t batch, int64_t t, int64_t channels);
 
 /* Layer norm of rows [rows, width] (row stride x_row): y = (x - mean) rstd
  * weight + bias, rstd = 1 / sqrt(variance + eps); weight and bias [width] may
@@ -714,17 +714,25 @@ int64_t bssm_layer_norm_partial_rows(int bf16, int64_t rows, int64_t width);
  * vocabulary and a logit above -infinity, q = softmax(logits / temperature).
  * A row without such entries has loss 0 and gradient 0.  At most 1024
  * entries.  stats [rows, 3] is kept for the backward; mean (NULL: not wanted)
- * receives (mean over the rows with entries, 1 / their number, sum). */
+ * receives (mean over the rows with entries, 1 / their number, sum).
+ * grad_logits [rows, vocabulary] (NULL: not wanted) receives temperature * (q
+ * - p), the gradient for upstream gradients of 1, which costs no second read
+ * of the logits; with mean_of_rows divided by the number of rows with entries,
+ * for which counts, bssm_distill_count_floats() floats, is needed. */
 int bssm_distill_forward(int bf16, int teacher_bf16, const void* logits, int64_t logits_row, const void* teacher,
                          const int64_t* index, float temperature, float* loss, float* stats, float* mean,
-                         int64_t rows, int64_t vocabulary, int64_t entries, void* stream);
+                         void* grad_logits, int mean_of_rows, float* counts, int64_t rows, int64_t vocabulary,
+                         int64_t entries, void* stream);
+int64_t bssm_distill_count_floats(void);
 
 /* grad_logits [rows, vocabulary] = upstream * temperature * (q - p), upstream
  * one value (upstream_scalar) or one a row, float32 in device memory; with
- * `mean` from the forward also divided by the number of rows with entries. */
+ * `mean` from the forward also divided by the number of rows with entries.
+ * ready: grad_logits holds what the forward wrote, and rows whose upstream
+ * gradient is 1 are not touched. */
 int bssm_distill_backward(int bf16, int teacher_bf16, const void* logits, int64_t logits_row, const void* teacher,
                           const int64_t* index, float temperature, const float* stats, const float* mean,
-                          const float* upstream, int upstream_scalar, void* grad_logits, int64_t rows,
+                          const float* upstream, int upstream_scalar, int ready, void* grad_logits, int64_t rows,
                           int64_t vocabulary, int64_t entries, void* stream);
 
 /* Selective state space scan.  Per sequence, head (its group's b and c: heads

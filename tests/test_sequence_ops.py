@@ -216,8 +216,8 @@ def test_c_entry_points_refuse():
     assert conv(w=5) == 2 and conv(b=-1) == 1 and conv() == 1 and conv(b=0) == 0
     assert lib.bssm_layer_norm_forward(0, 0, None, 1, None, None, 1e-5, None, None, None, 0, 1, None) == 0
     assert lib.bssm_layer_norm_forward(0, 0, None, 1, None, None, -1.0, None, None, None, 0, 1, None) == 1
-    assert lib.bssm_distill_forward(0, 0, None, 1, None, None, 1.0, None, None, None, 1, 1, 2000, None) == 2
-    assert lib.bssm_distill_forward(0, 0, None, 1, None, None, 0.0, None, None, None, 1, 1, 1, None) == 1
+    assert lib.bssm_distill_forward(0, 0, None, 1, None, None, 1.0, None, None, None, None, 0, None, 1, 1, 2000, None) == 2
+    assert lib.bssm_distill_forward(0, 0, None, 1, None, None, 0.0, None, None, None, None, 0, None, 1, 1, 1, None) == 1
 
     def scan(h=4, n=8, g=2, b=1):
         return lib.bssm_select_forward(0, None, 0, 0, 0, 0, None, 0, 0, None, None, 0, 0, 0, None, 0, 0, 0, None, None, 1,
