@@ -34,7 +34,7 @@ using lane::kWave;
 typedef __amdgpu_buffer_rsrc_t Window;
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
-constexpr int kCountBlocks = 64;  // partial counts of rows with a teacher
+constexpr int kCountBlocks = 512;  // partial counts of rows with a teacher
 
 template <int THREADS>
 __device__ __forceinline__ float block_sum(float x, float* red) {
@@ -91,6 +91,7 @@ struct RowOf {
 struct Teacher {
   int at[kDistillMaxTeacher];  // vocabulary index, -1: does not count
   float p[kDistillMaxTeacher];
+  float top, sum, any;  // largest logit / 1 if an entry counts; p is not yet divided by its sum
 };
 
 __device__ __forceinline__ bool counts(const DistillArgs& a, int64_t at, float& l, int64_t& i) {
@@ -99,14 +100,13 @@ __device__ __forceinline__ bool counts(const DistillArgs& a, int64_t at, float& 
   return i >= 0 && i < a.v && !(l == -INFINITY);
 }
 
-// The row's teacher distribution into LDS, not yet divided by its sum; log p_k = (l_k - top) / tau - log sum.
-template <int THREADS>
-__device__ __forceinline__ bool teacher_row(const DistillArgs& a, int64_t r, Teacher& t, float* red, float& top,
-                                            float& sum) {
+// The row's teacher distribution into LDS, by one wave beside the others'
+// work on the logits; log p_k = (l_k - top) / tau - log sum.
+__device__ __forceinline__ void teacher_row(const DistillArgs& a, int64_t r, Teacher& t) {
   const float c = lane::kLog2e / a.tau;
-  const int entries = static_cast<int>(a.k);
+  const int entries = static_cast<int>(a.k), ln = threadIdx.x % kWave;
   float m = -INFINITY, any = 0.f;
-  for (int k = threadIdx.x; k < entries; k += THREADS) {
+  for (int k = ln; k < entries; k += kWave) {
     float l;
     int64_t i;
     const bool there = counts(a, r * a.k + k, l, i);
@@ -117,24 +117,28 @@ __device__ __forceinline__ bool teacher_row(const DistillArgs& a, int64_t r, Tea
       any = 1.f;
     }
   }
-  top = block_max<THREADS>(m, red);
-  any = block_max<THREADS>(any, red);
+  float top = lane::lanes_max(m);
+  any = lane::lanes_max(any);
   if (top == -INFINITY) top = 0.f;  // every entry that counts is NaN
   float s = 0.f;
-  for (int k = threadIdx.x; k < entries; k += THREADS) {
+  for (int k = ln; k < entries; k += kWave) {  // each lane the entries that it wrote
     const float e = t.at[k] >= 0 ? lane::exp2_((t.p[k] - top) * c) : 0.f;
     t.p[k] = e;
     s += e;
   }
-  sum = block_sum<THREADS>(s, red);
-  return any > 0.f;
+  s = lane::lanes_sum(s);
+  if (ln == 0) {
+    t.top = top;
+    t.sum = s;
+    t.any = any;
+  }
 }
 
 // The listed entries' gradient once more, from float32: an index that is
 // listed twice is written by its first place, with the sum of its p.
 template <typename T, int THREADS>
-__device__ __forceinline__ void listed(const DistillArgs& a, const Teacher& t, const T* x, T* g, float top, float inv_s,
-                                       float inv_t, float u) {
+__device__ __forceinline__ void listed(const DistillArgs& a, const Teacher& t, const T* x, T* g, float top,
+                                       float scale, float inv_t, float u) {
   const float c = lane::kLog2e / a.tau;
   const int entries = static_cast<int>(a.k);
   for (int k = threadIdx.x; k < entries; k += THREADS) {
@@ -147,7 +151,7 @@ __device__ __forceinline__ void listed(const DistillArgs& a, const Teacher& t, c
       if (j < k) first = false;
       p += t.p[j];
     }
-    if (first) g[at] = lane::narrow<T>(u * (lane::exp2_((lane::widen(x[at]) - top) * c) * inv_s - p * inv_t));
+    if (first) g[at] = lane::narrow<T>(lane::exp2_((lane::widen(x[at]) - top) * c) * scale - u * (p * inv_t));
   }
 }
 
@@ -167,10 +171,12 @@ __global__ __launch_bounds__(256) void count_kernel(DistillArgs a) {
   n = block_sum<256>(threadIdx.x % kWave == 0 ? n : 0.f, red);
   if (threadIdx.x == 0) a.counts[blockIdx.x] = n;
 }
+// The same sum, in the same order, in every wave.
 __device__ __forceinline__ float rows_with_teacher(const DistillArgs& a) {
   float n = 0.f;
-  for (int i = 0; i < kCountBlocks; ++i) n += a.counts[i];
-  return fmaxf(n, 1.f);
+#pragma unroll
+  for (int i = 0; i < kCountBlocks; i += kWave) n += a.counts[i + threadIdx.x % kWave];
+  return fmaxf(lane::lanes_sum(n), 1.f);
 }
 
 // PIECES > 0: the row is held, that many pieces a thread; 0: it is read again.
@@ -186,88 +192,105 @@ __global__ __launch_bounds__(THREADS) void forward_kernel(DistillArgs a) {
   const T* x = static_cast<const T*>(a.logits) + r * a.logits_row;
   const RowOf<T> row(x, static_cast<int>(a.v));
   const int pieces = (row.end + N - 1) / N;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / kWave));
   Pack<T, N> held[kHold];
-  float m = -INFINITY, s = 0.f;
-  auto top_of = [&](const Pack<T, N>& p, int piece) {
-    float best = -INFINITY;
-    if (row.whole(piece)) {
-#pragma unroll
-      for (int e = 0; e < N; ++e) best = fmaxf(best, lane::widen(p.v[e]));
-    } else {
+  float u = a.tau;
+  // Widened values are not kept from one pass to the next (they would double
+  // the registers of bfloat16 rows).
+  auto again = [](Pack<T, N>& p) {
+    v4u w = __builtin_bit_cast(v4u, p);
+    asm volatile("" : "+v"(w));
+    p = __builtin_bit_cast(Pack<T, N>, w);
+  };
+  // Elements outside the row count as -infinity: no maximum, and 0 in the sum.
+  auto masked = [&](Pack<T, N> p, int piece) {
+    if (!row.whole(piece)) {
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        if (row.has(piece, e)) best = fmaxf(best, lane::widen(p.v[e]));
+        if (!row.has(piece, e)) p.v[e] = lane::narrow<T>(-INFINITY);
     }
+    return p;
+  };
+  auto top_of = [&](const Pack<T, N>& p) {
+    float best = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < N; ++e) best = fmaxf(best, lane::widen(p.v[e]));
     return best;
   };
-  auto sum_of = [&](const Pack<T, N>& p, int piece, float base) {
+  auto sum_of = [&](const Pack<T, N>& p, float base) {
     float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float v = lane::exp2_((lane::widen(p.v[e]) - base) * c);
-      sum += row.whole(piece) || row.has(piece, e) ? v : 0.f;
-    }
+    for (int e = 0; e < N; ++e) sum += lane::exp2_((lane::widen(p.v[e]) - base) * c);
     return sum;
   };
-  float top, total;
+  float m = -INFINITY, s = 0.f, top, total;
   if constexpr (PIECES > 0) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) held[i] = row.load(i * THREADS + threadIdx.x);
+  }
+  if (wave == 0) teacher_row(a, r, t);
+  if (a.grad != nullptr && a.mean_of_rows) u /= rows_with_teacher(a);
+  if constexpr (PIECES > 0) {
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i)
-      if (const int piece = i * THREADS + threadIdx.x; piece < pieces) m = fmaxf(m, top_of(held[i], piece));
+    for (int i = 0; i < PIECES; ++i) {
+      held[i] = masked(held[i], i * THREADS + threadIdx.x);
+      again(held[i]);
+      m = fmaxf(m, top_of(held[i]));
+    }
     top = block_max<THREADS>(m, red);
     if (top == -INFINITY) top = 0.f;
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i)
-      if (const int piece = i * THREADS + threadIdx.x; piece < pieces) s += sum_of(held[i], piece, top);
+    for (int i = 0; i < PIECES; ++i) {
+      again(held[i]);
+      s += sum_of(held[i], top);
+    }
     total = block_sum<THREADS>(s, red);
   } else {
     for (int piece = threadIdx.x; piece < pieces; piece += THREADS) {
-      const Pack<T, N> p = row.load(piece);
-      const float best = fmaxf(m, top_of(p, piece));
+      const Pack<T, N> p = masked(row.load(piece), piece);
+      const float best = fmaxf(m, top_of(p));
       if (best > m) {
         s = m == -INFINITY ? s : s * lane::exp2_((m - best) * c);
         m = best;
       }
-      s += sum_of(p, piece, m == -INFINITY ? 0.f : m);
+      s += sum_of(p, m == -INFINITY ? 0.f : m);
     }
     top = block_max<THREADS>(m, red);
     if (top == -INFINITY) top = 0.f;
     total = block_sum<THREADS>(m == -INFINITY ? s : s * lane::exp2_((m - top) * c), red);
   }
-  float t_top, t_sum;
-  const bool any = teacher_row<THREADS>(a, r, t, red, t_top, t_sum);
-  const float inv_t = 1.f / t_sum;
-  float loss = 0.f;
-  const float log_t = logf(t_sum), log_s = logf(total), inv_tau = 1.f / a.tau;
-  for (int k = threadIdx.x; k < a.k; k += THREADS) {
-    if (t.at[k] < 0) continue;
-    const float p = t.p[k] * inv_t;
-    if (p == 0.f) continue;
-    const float l = lane::param(a.teacher, r * a.k + k, a.teacher_bf16);
-    const float log_p = (l - t_top) * inv_tau - log_t;
-    const float log_q = (lane::widen(x[t.at[k]]) - top) * inv_tau - log_s;
-    loss = fmaf(p, log_p - log_q, loss);
-  }
-  loss = block_sum<THREADS>(loss, red);
-  if (threadIdx.x == 0) {
-    a.loss[r] = any ? a.tau * a.tau * loss : 0.f;
-    a.stats[3 * r] = top;
-    a.stats[3 * r + 1] = total;
-    a.stats[3 * r + 2] = any ? 1.f : 0.f;
+  // Behind the barriers of the sums the teacher's row is there for all.
+  const bool any = t.any > 0.f;
+  const float inv_t = 1.f / t.sum, inv_s = 1.f / total;
+  if (wave == 0) {
+    float loss = 0.f;
+    const float log_t = logf(t.sum), log_s = logf(total), inv_tau = 1.f / a.tau;
+    for (int k = threadIdx.x; k < a.k; k += kWave) {
+      if (t.at[k] < 0) continue;
+      const float p = t.p[k] * inv_t;
+      if (p == 0.f) continue;
+      const float l = lane::param(a.teacher, r * a.k + k, a.teacher_bf16);
+      const float log_p = (l - t.top) * inv_tau - log_t;
+      const float log_q = (lane::widen(x[t.at[k]]) - top) * inv_tau - log_s;
+      loss = fmaf(p, log_p - log_q, loss);
+    }
+    loss = lane::lanes_sum(loss);
+    if (threadIdx.x == 0) {
+      a.loss[r] = any ? a.tau * a.tau * loss : 0.f;
+      a.stats[3 * r] = top;
+      a.stats[3 * r + 1] = total;
+      a.stats[3 * r + 2] = any ? 1.f : 0.f;
+    }
   }
   if (a.grad == nullptr) return;
-  const float u = a.tau / (a.mean_of_rows ? rows_with_teacher(a) : 1.f), inv_s = 1.f / total;
   T* g = static_cast<T*>(a.grad) + r * a.v;
   const RowOf<T> to(g, static_cast<int>(a.v));
+  const float scale = u * inv_s;
   auto gradient = [&](const Pack<T, N>& p, int piece) {
     Pack<T, N> o;
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float v = u * (lane::exp2_((lane::widen(p.v[e]) - top) * c) * inv_s);
-      o.v[e] = lane::narrow<T>(any ? v : 0.f);
-    }
+    for (int e = 0; e < N; ++e)
+      o.v[e] = lane::narrow<T>(any ? lane::exp2_((lane::widen(p.v[e]) - top) * c) * scale : 0.f);
     if (to.shift == row.shift) {
       to.store(g, piece, o);
     } else {  // bfloat16 rows of which one is odd
@@ -279,13 +302,16 @@ __global__ __launch_bounds__(THREADS) void forward_kernel(DistillArgs a) {
   if constexpr (PIECES > 0) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i)
-      if (const int piece = i * THREADS + threadIdx.x; piece < pieces) gradient(held[i], piece);
+      if (const int piece = i * THREADS + threadIdx.x; piece < pieces) {
+        again(held[i]);
+        gradient(held[i], piece);
+      }
   } else {
     for (int piece = threadIdx.x; piece < pieces; piece += THREADS) gradient(row.load(piece), piece);
   }
   if (!any) return;
   __syncthreads();
-  listed<T, THREADS>(a, t, x, g, top, inv_s, inv_t, u);
+  listed<T, THREADS>(a, t, x, g, top, scale, inv_t, u);
 }
 
 // mean[] = (sum / rows with a teacher, 1 / rows, sum), in a fixed order.
@@ -310,28 +336,25 @@ template <typename T>
 __global__ __launch_bounds__(512) void backward_kernel(DistillArgs a) {
   constexpr int THREADS = 512, N = RowOf<T>::kN;
   __shared__ Teacher t;
-  __shared__ float red[THREADS / kWave];
   const int64_t r = blockIdx.x;
   const float c = lane::kLog2e / a.tau;
   const T* x = static_cast<const T*>(a.logits) + r * a.logits_row;
   T* g = static_cast<T*>(a.grad) + r * a.v;
   const RowOf<T> row(x, static_cast<int>(a.v)), to(g, static_cast<int>(a.v));
   const int pieces = (row.end + N - 1) / N;
-  const float top = a.stats[3 * r], inv_s = 1.f / a.stats[3 * r + 1];
+  const float top = a.stats[3 * r];
   const bool any = a.stats[3 * r + 2] > 0.f;
   const float up = a.upstream[a.upstream_scalar ? 0 : r];
   if (a.ready && up == 1.f) return;
   const float u = a.tau * up * (a.mean == nullptr ? 1.f : a.mean[1]);
-  float t_top, t_sum;
-  teacher_row<THREADS>(a, r, t, red, t_top, t_sum);
+  const float scale = u / a.stats[3 * r + 1];
+  if (threadIdx.x < kWave) teacher_row(a, r, t);
   for (int piece = threadIdx.x; piece < pieces; piece += THREADS) {
     const Pack<T, N> p = row.load(piece);
     Pack<T, N> o;
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float v = u * (lane::exp2_((lane::widen(p.v[e]) - top) * c) * inv_s);
-      o.v[e] = lane::narrow<T>(any ? v : 0.f);
-    }
+    for (int e = 0; e < N; ++e)
+      o.v[e] = lane::narrow<T>(any ? lane::exp2_((lane::widen(p.v[e]) - top) * c) * scale : 0.f);
     if (to.shift == row.shift) {
       to.store(g, piece, o);
     } else {
@@ -342,7 +365,7 @@ __global__ __launch_bounds__(512) void backward_kernel(DistillArgs a) {
   }
   if (!any) return;
   __syncthreads();
-  listed<T, THREADS>(a, t, x, g, top, inv_s, 1.f / t_sum, u);
+  listed<T, THREADS>(a, t, x, g, top, scale, 1.f / t.sum, u);
 }
 
 // The fewest threads that hold the row in 8 pieces each, and 1024 with 16 for

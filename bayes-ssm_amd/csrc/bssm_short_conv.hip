@@ -19,6 +19,8 @@
 #include "bssm_lane.h"
 #include "bssm_sequence.h"
 
+#include <type_traits>
+
 namespace bssm {
 namespace short_conv {
 namespace {
@@ -51,42 +53,56 @@ __device__ __forceinline__ void input_row(const ShortConvArgs& a, int64_t b, int
   for (int i = 0; i < N; ++i) x[i] = lane::widen(r.v[i]);
 }
 
+// A thread's N * W weights lie together: loaded N at a time (one by one they
+// were 40 loads beside a segment's 16 rows, each touching 64 lines).
 template <int N, int W>
 struct Taps {
   float w[N][W], bias[N];
   __device__ __forceinline__ Taps(const ShortConvArgs& a, int64_t c0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int j = 0; j < W; ++j) {
+      float part[N];
+      lane::params<N>(a.weight, c0 * W + j * N, a.param_bf16, part);
 #pragma unroll
-      for (int j = 0; j < W; ++j) w[i][j] = lane::param(a.weight, (c0 + i) * W + j, a.param_bf16);
-      bias[i] = a.bias == nullptr ? 0.f : lane::param(a.bias, c0 + i, a.param_bf16);
+      for (int i = 0; i < N; ++i) w[(j * N + i) / W][(j * N + i) % W] = part[i];
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) bias[i] = 0.f;
+    if (a.bias != nullptr) lane::params<N>(a.bias, c0, a.param_bf16, bias);
   }
 };
 
+constexpr int kAhead = 4;  // rows loaded together, and before the sums of as many rows in front of them
+
+// Rows [t, t + kAhead) of a stream, the last row again past its end.
+template <typename T, int N>
+__device__ __forceinline__ void fetch(const T* p, int64_t row, int t, int end, Pack<T, N> (&raw)[kAhead]) {
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u)
+    raw[u] = lane::load_pack<T, N>(p + static_cast<int64_t>(t + u < end ? t + u : end - 1) * row);
+}
+
 template <typename T, int N, int W>
 __global__ __launch_bounds__(256) void forward_kernel(ShortConvArgs a, int seg) {
-  constexpr int kAhead = 4;  // rows loaded before their sums
   const int64_t groups = a.c / N, segs = a.t > 0 ? (a.t + seg - 1) / seg : 1;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (id >= a.b * segs * groups) return;
   const int64_t c0 = id % groups * N, b = id / groups / segs;
   const int s = static_cast<int>(id / groups % segs), end = static_cast<int>(a.t);
   const int n = row_length(a, b), t0 = s * seg, t1 = t0 + seg < end ? t0 + seg : end;
+  T* y = static_cast<T*>(a.y) + b * a.t * a.c + c0;
+  const T* x = static_cast<const T*>(a.x) + b * a.x_batch + c0;
+  Pack<T, N> raw[kAhead];
+  if (t0 < t1) fetch<T, N>(x, a.x_row, t0, t1, raw);
   const Taps<N, W> k(a, c0);
   float h[W][N];  // h[j] = x[t - W + 1 + j]
 #pragma unroll
   for (int j = 1; j < W; ++j) input_row<T, N, W>(a, b, t0 - W + j, c0, h[j]);
-  T* y = static_cast<T*>(a.y) + b * a.t * a.c + c0;
-  const T* x = static_cast<const T*>(a.x) + b * a.x_batch + c0;
   for (int t = t0; t < t1; t += kAhead) {
-    Pack<T, N> raw[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (t + u < t1) raw[u] = lane::load_pack<T, N>(x + static_cast<int64_t>(t + u) * a.x_row);
+    Pack<T, N> next[kAhead];
+    if (t + kAhead < t1) fetch<T, N>(x, a.x_row, t + kAhead, t1, next);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (t + u >= t1) break;
       Pack<T, N> out;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -99,7 +115,8 @@ __global__ __launch_bounds__(256) void forward_kernel(ShortConvArgs a, int seg) 
         if (a.silu) p *= lane::sigmoid_(p);
         out.v[i] = lane::narrow<T>(t + u < n ? p : 0.f);
       }
-      lane::store_pack<T, N>(y + static_cast<int64_t>(t + u) * a.c, out);
+      if (t + u < t1) lane::store_pack<T, N>(y + static_cast<int64_t>(t + u) * a.c, out);
+      raw[u] = next[u];
     }
   }
   if (s == 0 && a.final_state != nullptr) {
@@ -120,9 +137,8 @@ __global__ __launch_bounds__(256) void forward_kernel(ShortConvArgs a, int seg) 
 // the waves' weight and bias sums meet in LDS, one row of partials a block.
 template <typename T, int N, int W>
 __global__ __launch_bounds__(kWave * kWaves) void backward_kernel(ShortConvArgs a, int seg, int64_t blocks_t) {
-  constexpr int kAhead = 4;
   __shared__ float red[kWaves - 1][W + 1][N][kWave];
-  const int wave = threadIdx.x / kWave, ln = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / kWave)), ln = threadIdx.x % kWave;
   const int64_t groups = a.c / N, cblocks = (groups + kWave - 1) / kWave;
   const int64_t g = blockIdx.x % cblocks * kWave + ln, part = blockIdx.x / cblocks;
   const int64_t b = part / blocks_t;
@@ -136,9 +152,15 @@ __global__ __launch_bounds__(kWave * kWaves) void backward_kernel(ShortConvArgs 
     for (int i = 0; i < N; ++i) gw[j][i] = 0.f;
   if (active && (t0 < t_end || (t0 == 0 && a.gstate != nullptr))) {
     const int n = row_length(a, b), t1 = t0 + seg < t_end ? t0 + seg : t_end;
-    const Taps<N, W> k(a, c0);
+    const int end = t1 + W - 1, last = end < t_end ? end : t_end;  // rows [t1, last): for the inputs before t1
     const T* x = static_cast<const T*>(a.x) + b * a.x_batch + c0;
     const T* gy = static_cast<const T*>(a.gy) + b * a.t * a.c + c0;
+    Pack<T, N> rx[kAhead], rg[kAhead];
+    if (t_end > 0) {
+      fetch<T, N>(x, a.x_row, t0, last, rx);
+      if (a.gy != nullptr) fetch<T, N>(gy, a.c, t0, last, rg);
+    }
+    const Taps<N, W> k(a, c0);
     float h[W][N], q[W][N];  // h[j] = x[t - W + 1 + j], q[j] = g[t - W + 1 + j]
 #pragma unroll
     for (int j = 0; j < W; ++j)
@@ -151,61 +173,72 @@ __global__ __launch_bounds__(kWave * kWaves) void backward_kernel(ShortConvArgs 
 #pragma unroll
         for (int i = 0; i < N; ++i) h[j][i] = 0.f;
     }
-    const int end = t1 + W - 1;
-    for (int t = t0; t < end; t += kAhead) {
-      Pack<T, N> rx[kAhead], rg[kAhead];
+    // Token tt: its g, its terms of the weights' gradient, and the gradient of
+    // input tt - W + 1.  INNER: tt is this wave's own and before the row's
+    // end, and so is that input.
+    auto token = [&](auto kind, int tt, const Pack<T, N>& px, const Pack<T, N>& pg) {
+      constexpr bool INNER = decltype(kind)::value;
+      const bool live = INNER || tt < n, mine = INNER || tt < t1;
+      const int s = tt - (W - 1), jf = s - n + W - 1;  // jf: row of the final state that input s is
+      const bool from_final = !INNER && a.gfinal != nullptr && jf >= 0 && jf < W - 1;
+      Pack<T, N> out;
+      float gf[N];
+      if (from_final) {
+        const Pack<T, N> r = lane::load_pack<T, N>(static_cast<const T*>(a.gfinal) + (b * (W - 1) + jf) * a.c + c0);
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (t + u < n && t + u < end) {
-          rx[u] = lane::load_pack<T, N>(x + static_cast<int64_t>(t + u) * a.x_row);
-          if (a.gy != nullptr) rg[u] = lane::load_pack<T, N>(gy + static_cast<int64_t>(t + u) * a.c);
+        for (int i = 0; i < N; ++i) gf[i] = lane::widen(r.v[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int j = 0; j + 1 < W; ++j) {
+          h[j][i] = h[j + 1][i];
+          q[j][i] = q[j + 1][i];
         }
+        h[W - 1][i] = live ? lane::widen(px.v[i]) : 0.f;
+        float gi = live && a.gy != nullptr ? lane::widen(pg.v[i]) : 0.f;
+        if (a.silu) {
+          float p = k.bias[i];
+#pragma unroll
+          for (int j = 0; j < W; ++j) p = fmaf(k.w[i][j], h[j][i], p);
+          const float sg = lane::sigmoid_(p);
+          gi *= sg * fmaf(p, 1.f - sg, 1.f);
+          if (!live) gi = 0.f;
+        }
+        q[W - 1][i] = gi;
+        if (mine) {
+#pragma unroll
+          for (int j = 0; j < W; ++j) gw[j][i] = fmaf(gi, h[j][i], gw[j][i]);
+          gw[W][i] += gi;
+        }
+        float o = from_final ? gf[i] : 0.f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) o = fmaf(k.w[i][j], q[W - 1 - j][i], o);
+        out.v[i] = lane::narrow<T>(o);
+      }
+      if (INNER || s >= t0) lane::store_pack<T, N>(static_cast<T*>(a.gx) + (b * a.t + s) * a.c + c0, out);
+      else if (t0 == 0 && a.gstate != nullptr)
+        lane::store_pack<T, N>(static_cast<T*>(a.gstate) + (b * (W - 1) + s + W - 1) * a.c + c0, out);
+    };
+    const int inner = t1 < n ? t1 : n;
+    for (int t = t0; t < end; t += kAhead) {
+      Pack<T, N> nx[kAhead], ng[kAhead];
+      if (t + kAhead < last) {
+        fetch<T, N>(x, a.x_row, t + kAhead, last, nx);
+        if (a.gy != nullptr) fetch<T, N>(gy, a.c, t + kAhead, last, ng);
+      }
+      if (t >= t0 + W - 1 && t + kAhead <= inner) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) token(std::true_type{}, t + u, rx[u], rg[u]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (t + u < end) token(std::false_type{}, t + u, rx[u], rg[u]);
+      }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int tt = t + u;
-        if (tt >= end) break;
-        const bool live = tt < n, mine = tt < t1;
-        const int s = tt - (W - 1);
-        Pack<T, N> out;
-        float gf[N];
-        const int jf = s - n + W - 1;  // row of the final state that input s is
-        const bool from_final = a.gfinal != nullptr && jf >= 0 && jf < W - 1;
-        if (from_final) {
-          const Pack<T, N> r = lane::load_pack<T, N>(static_cast<const T*>(a.gfinal) + (b * (W - 1) + jf) * a.c + c0);
-#pragma unroll
-          for (int i = 0; i < N; ++i) gf[i] = lane::widen(r.v[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-#pragma unroll
-          for (int j = 0; j + 1 < W; ++j) {
-            h[j][i] = h[j + 1][i];
-            q[j][i] = q[j + 1][i];
-          }
-          h[W - 1][i] = live ? lane::widen(rx[u].v[i]) : 0.f;
-          float gi = live && a.gy != nullptr ? lane::widen(rg[u].v[i]) : 0.f;
-          if (a.silu) {
-            float p = k.bias[i];
-#pragma unroll
-            for (int j = 0; j < W; ++j) p = fmaf(k.w[i][j], h[j][i], p);
-            const float sg = lane::sigmoid_(p);
-            gi *= sg * fmaf(p, 1.f - sg, 1.f);
-            if (!live) gi = 0.f;
-          }
-          q[W - 1][i] = gi;
-          if (mine) {
-#pragma unroll
-            for (int j = 0; j < W; ++j) gw[j][i] = fmaf(gi, h[j][i], gw[j][i]);
-            gw[W][i] += gi;
-          }
-          float o = from_final ? gf[i] : 0.f;
-#pragma unroll
-          for (int j = 0; j < W; ++j) o = fmaf(k.w[i][j], q[W - 1 - j][i], o);
-          out.v[i] = lane::narrow<T>(o);
-        }
-        if (s >= t0) lane::store_pack<T, N>(static_cast<T*>(a.gx) + (b * a.t + s) * a.c + c0, out);
-        else if (t0 == 0 && a.gstate != nullptr)
-          lane::store_pack<T, N>(static_cast<T*>(a.gstate) + (b * (W - 1) + s + W - 1) * a.c + c0, out);
+        rx[u] = nx[u];
+        rg[u] = ng[u];
       }
     }
   }
@@ -256,11 +289,12 @@ int backward_segment(int64_t b, int64_t t, int64_t groups) {
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// 16-byte groups need every row of every stream on a 16-byte boundary.
+// 16-byte groups need every row of every stream, and the parameters, on a 16-byte boundary.
 bool vectors(const ShortConvArgs& a) {
   const int n = a.bf16 ? 8 : 4;
   return a.c % n == 0 && a.x_row % n == 0 && a.x_batch % n == 0 && aligned(a.x) && aligned(a.state) && aligned(a.y) &&
-         aligned(a.final_state) && aligned(a.gy) && aligned(a.gfinal) && aligned(a.gx) && aligned(a.gstate);
+         aligned(a.final_state) && aligned(a.gy) && aligned(a.gfinal) && aligned(a.gx) && aligned(a.gstate) &&
+         aligned(a.weight) && aligned(a.bias);
 }
 
 template <typename T, int N, int W>
