@@ -116,7 +116,7 @@ def distillation_loss(logits: Tensor, teacher_logits: Tensor, teacher_index: Ten
         raise ValueError('reduction must be "mean", "sum" or "none"')
     v, k, lead = logits.shape[-1], teacher_index.shape[-1], logits.shape[:-1]
     rows = math.prod(lead)
-    x = logits.reshape(rows, v)
+    x = logits if logits.ndim == 2 else logits.reshape(rows, v)
     teacher, index = teacher_logits.detach().reshape(rows, k), teacher_index.reshape(rows, k).long()
     if logits.device.type != "cuda" or logits.dtype not in (torch.bfloat16, torch.float32):
         losses, has = _formula(x, teacher, index, float(temperature))

@@ -31,18 +31,22 @@ def _formula(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: f
 class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
+        shape, dev = x.shape, x.device
+        if x.ndim != 2:
+            x = x.reshape(-1, shape[-1])
         r, d = x.shape
-        dev = x.device
-        y = torch.empty(r, d, device=dev, dtype=x.dtype)
+        if (d > 1 and x.stride(1) != 1) or (r > 1 and x.stride(0) < d):
+            x = x.contiguous()
+        y = torch.empty(shape, device=dev, dtype=x.dtype)
         keep = any(ctx.needs_input_grad)
         stats = torch.empty(2, r, device=dev, dtype=torch.float32) if keep else None
-        mean, rstd = (None, None) if stats is None else (stats[0], stats[1])
         weight, bias = (None if z is None else z.contiguous() for z in (weight, bias))
         params = [z for z in (weight, bias) if z is not None]
         param_bf16 = int(bool(params) and params[0].dtype == torch.bfloat16)
         P = _hip.ptr
+        mean = P(stats)
         _hip.launch(dev, "bssm_layer_norm_forward", int(x.dtype == torch.bfloat16), param_bf16, P(x), x.stride(0),
-                    P(weight), P(bias), eps, P(y), P(mean), P(rstd), r, d, _hip.stream_of(dev))
+                    P(weight), P(bias), eps, P(y), mean, mean and mean + 4 * r, r, d, _hip.stream_of(dev))
         ctx.save_for_backward(x, weight, bias, stats)
         ctx.param_bf16 = param_bf16
         return y
@@ -55,18 +59,17 @@ class _LayerNormFunction(torch.autograd.Function):
         need = ctx.needs_input_grad
         bf16 = int(x.dtype == torch.bfloat16)
         gy = grad_y.contiguous()
-        gx = torch.empty(r, d, device=dev, dtype=x.dtype) if need[0] else None
+        gx = torch.empty_like(gy) if need[0] else None
         gw = torch.empty_like(weight) if need[1] else None
         gb = torch.empty_like(bias) if need[2] else None
         partials = None
         if gw is not None or gb is not None:
-            rows = _hip.function("bssm_layer_norm_partial_rows")(bf16, r, d)
-            partials = torch.empty(rows, 2, d, device=dev, dtype=torch.float32)
-            if r == 0:
-                partials = torch.empty(1, 2, d, device=dev, dtype=torch.float32)
+            rows = max(_hip.function("bssm_layer_norm_partial_rows")(bf16, r, d), 1)
+            partials = torch.empty(rows * 2 * d, device=dev, dtype=torch.float32)
         P = _hip.ptr
-        _hip.launch(dev, "bssm_layer_norm_backward", bf16, ctx.param_bf16, P(x), x.stride(0), P(weight), P(stats[0]),
-                    P(stats[1]), P(gy), P(gx), P(partials), P(gw), P(gb), r, d, _hip.stream_of(dev))
+        mean = P(stats)
+        _hip.launch(dev, "bssm_layer_norm_backward", bf16, ctx.param_bf16, P(x), x.stride(0), P(weight), mean,
+                    mean + 4 * r, P(gy), P(gx), P(partials), P(gw), P(gb), r, d, _hip.stream_of(dev))
         return gx, gw, gb, None
 
 
@@ -97,10 +100,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     kinds = {z.dtype for z in (weight, bias) if z is not None}
     if len(kinds) > 1 or not kinds <= {torch.bfloat16, torch.float32}:
         weight, bias = (None if z is None else z.float() for z in (weight, bias))
-    rows = x.reshape(-1, d)
-    if (d > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < d):
-        rows = rows.contiguous()
-    return _LayerNormFunction.apply(rows, weight, bias, float(eps)).reshape(x.shape)
+    return _LayerNormFunction.apply(x, weight, bias, float(eps))
 
 
 class LayerNorm(nn.Module):

@@ -34,6 +34,7 @@ using lane::kWave;
 typedef __amdgpu_buffer_rsrc_t Window;
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
+constexpr int kStream = 2;  // non-temporal
 constexpr int kCountBlocks = 512;  // partial counts of rows with a teacher
 
 template <int THREADS>
@@ -79,7 +80,7 @@ struct RowOf {
   // A gradient row of the same shift, elements outside left alone.
   __device__ __forceinline__ void store(T* row, int piece, const Pack<T, kN>& p) const {
     if (whole(piece)) {
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, p), w, piece * 16, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, p), w, piece * 16, 0, kStream);
     } else {
 #pragma unroll
       for (int e = 0; e < kN; ++e)
@@ -183,7 +184,7 @@ __device__ __forceinline__ float rows_with_teacher(const DistillArgs& a) {
 // a.grad: the gradient for an upstream gradient of 1 is wanted.
 // stats[r] = (maximum, sum of exponentials, 1 if the row has a teacher).
 template <typename T, int THREADS, int PIECES>
-__global__ __launch_bounds__(THREADS) void forward_kernel(DistillArgs a) {
+__global__ __launch_bounds__(THREADS, PIECES <= 8 ? 8 : 4) void forward_kernel(DistillArgs a) {
   constexpr int N = RowOf<T>::kN, kHold = PIECES > 0 ? PIECES : 1;
   __shared__ Teacher t;
   __shared__ float red[THREADS / kWave];
@@ -246,14 +247,23 @@ __global__ __launch_bounds__(THREADS) void forward_kernel(DistillArgs a) {
     }
     total = block_sum<THREADS>(s, red);
   } else {
-    for (int piece = threadIdx.x; piece < pieces; piece += THREADS) {
-      const Pack<T, N> p = masked(row.load(piece), piece);
-      const float best = fmaxf(m, top_of(p));
+    constexpr int kTogether = 4;
+    for (int piece = threadIdx.x; piece < pieces; piece += kTogether * THREADS) {
+      Pack<T, N> p[kTogether];
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) p[i] = row.load(piece + i * THREADS);
+      float best = m;
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) {
+        p[i] = masked(p[i], piece + i * THREADS);
+        best = fmaxf(best, top_of(p[i]));
+      }
       if (best > m) {
         s = m == -INFINITY ? s : s * lane::exp2_((m - best) * c);
         m = best;
       }
-      s += sum_of(p, m == -INFINITY ? 0.f : m);
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) s += sum_of(p[i], m == -INFINITY ? 0.f : m);
     }
     top = block_max<THREADS>(m, red);
     if (top == -INFINITY) top = 0.f;
@@ -377,6 +387,7 @@ hipError_t forward(const DistillArgs& a, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(a.r));
   if (pieces <= 256 * 2) hipLaunchKernelGGL((forward_kernel<T, 256, 2>), grid, dim3(256), 0, stream, a);
   else if (pieces <= 256 * 8) hipLaunchKernelGGL((forward_kernel<T, 256, 8>), grid, dim3(256), 0, stream, a);
+  else if (a.grad == nullptr) hipLaunchKernelGGL((forward_kernel<T, 1024, 0>), grid, dim3(1024), 0, stream, a);
   else if (pieces <= 512 * 8) hipLaunchKernelGGL((forward_kernel<T, 512, 8>), grid, dim3(512), 0, stream, a);
   else if (pieces <= 1024 * 8) hipLaunchKernelGGL((forward_kernel<T, 1024, 8>), grid, dim3(1024), 0, stream, a);
   else if (pieces <= 1024 * 16) hipLaunchKernelGGL((forward_kernel<T, 1024, 16>), grid, dim3(1024), 0, stream, a);
