@@ -285,12 +285,11 @@ struct Steps {
   }
 };
 
-// Inclusive sum over the wave's lanes.
+// Inclusive sum over the lanes up to a lane, of every `width` of them.
 template <typename V>
-__device__ __forceinline__ V lanes_prefix(V x) {
-  const int ln = threadIdx.x % kWave;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
+__device__ __forceinline__ V lanes_prefix(V x, int width = kWave) {
+  const int ln = threadIdx.x % width;
+  for (int o = 1; o < width; o <<= 1) {
     const V up = __shfl_up(x, o, kWave);
     if (ln >= o) x += up;
   }

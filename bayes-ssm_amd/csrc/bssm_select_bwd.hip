@@ -44,8 +44,12 @@ hipError_t launch_adjoints(const SelectArgs& a, hipStream_t stream);  // bssm_se
 namespace {
 
 constexpr int kHalf = 32;  // rows of h and gh in LDS at a time
+constexpr int kHalfTokens = 64;  // of a record of 128 (one of 64 has the first half alone)
 
 static_assert(kTileP == 2 * kHalf, "two halves");
+
+template <typename T>
+constexpr int kHeld = sizeof(T) == 2 ? 2 : 1;  // parts of h and gh
 
 template <typename T>
 struct Sizes {
@@ -54,19 +58,22 @@ struct Sizes {
   static constexpr int kThreads = 2 * kBlocks * kWave;
 };
 
-// The token sums in memory, each [B, H, padded T]: row + C . gC', B . gB' / d, col and the diagonal; then, a wave each,
-// <gh, h> and gy . x of a record: [2, B, H, records, waves].
+// The token sums in memory, each [B, H, padded T]: row and col (with the tokens
+// of the same half), C . gC', B . gB' / d, col or row with the other half's
+// tokens, the diagonal; then, a wave each, <gh, h> and gy . x of a record:
+// [2, B, H, records, waves].
+enum TokenSum { kRows, kCols, kLater, kEarlier, kFar, kDiagonal, kTokenSums };
 struct TokenSums {
-  float *later, *earlier, *direct, *diagonal, *whole, *skip;
+  float *token, *wave;       // of one head
+  int64_t sums_on, waves_on; // from one kind to the next
   __device__ __forceinline__ TokenSums(const SelectArgs& a, int64_t b, int64_t h, int64_t records, int waves) {
     const int64_t tp = (a.t + kSpan - 1) / kSpan * kSpan, all = a.b * a.h, at = b * a.h + h;
-    later = a.token_sums + at * tp;
-    earlier = later + all * tp;
-    direct = earlier + all * tp;
-    diagonal = direct + all * tp;
-    whole = a.token_sums + 4 * all * tp + at * records * waves;
-    skip = whole + all * records * waves;
+    sums_on = all * tp;
+    waves_on = all * records * waves;
+    token = a.token_sums + at * tp;
+    wave = a.token_sums + kTokenSums * sums_on + at * records * waves;
   }
+  __device__ __forceinline__ float* operator[](TokenSum k) const { return token + k * sums_on; }
 };
 
 // A half (32 values of P) of a [P, N] record in registers.
@@ -108,7 +115,7 @@ struct HalfRecord {
       if (at >= kHalf * NP) break;
       v4f rest = v[k];
 #pragma unroll
-      for (int s = 0; s < kParts<T>; ++s) {
+      for (int s = 0; s < kHeld<T>; ++s) {
         Pack<T, 4> o;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -126,7 +133,7 @@ template <typename T, int NP>
 struct Tiles {
   static constexpr int L = Sizes<T>::kL;
   alignas(16) T xs[L * kTileP], gs[L * kTileP], ks[L * NP], qs[L * NP];
-  alignas(16) T hs[kParts<T>][kHalf * NP], ghs[kParts<T>][kHalf * NP];
+  alignas(16) T hs[kHeld<T>][kHalf * NP], ghs[kHeld<T>][kHalf * NP];
   // since: decay from the start of the token's 32 to it; until: its step times the decay from it to their end.
   alignas(16) float step[L], near[L], since[L], until[L];
   double base[L / kNear];
@@ -135,8 +142,9 @@ struct Tiles {
 
 // A lane's sums for its own token.
 struct Own {
-  float row, col, diagonal, dot_x;  // inside the record: as i, as j, of the diagonal, gy . x
-  float from_h, from_gh;            // with what comes from h and gh
+  float near, far;        // row (as i) or col (as j): with the tokens of its half of the record, and of the other
+  float diagonal, dot_x;  // of the diagonal: W, gy . x
+  float outside;          // with what comes from h (as i) or gh (as j)
 };
 
 // The record's tokens with each other, the wave's own as i (AS_I: gC) or as j (gB and gu).
@@ -150,19 +158,17 @@ __device__ __forceinline__ void inside(const Tiles<T, NP>& t, int block, v16f (&
           *other_p = AS_I ? t.xs : t.gs;
   const float d_own = t.step[own], near_own = t.near[own];
   const double base_own = t.base[own / kNear];
-  Operand<T> n_own[NP / kDepth];
-#pragma unroll
-  for (int k = 0; k < NP / kDepth; ++k) n_own[k] = along<NP>(own_n, own, k * kDepth, g);
 #pragma unroll 1
   for (int blk = AS_I ? 0 : block; blk <= (AS_I ? block : kBlocks - 1); ++blk) {
     const int here = anew(own);  // 16 registers less than kept operands would take
     v16f s = zeros(), gx = zeros();
 #pragma unroll
-    for (int k = 0; k < NP / kDepth; ++k) mma(s, along<NP>(other_n, blk * kTile + ln % 32, k * kDepth, g), n_own[k]);
+    for (int k = 0; k < NP / kDepth; ++k) mma(s, along<NP>(other_n, blk * kTile + ln % 32, k * kDepth, g), along<NP>(own_n, here, k * kDepth, g));
 #pragma unroll
     for (int k = 0; k < kTileP / kDepth; ++k)
       mma(gx, along<kTileP>(other_p, blk * kTile + ln % 32, k * kDepth, g), along<kTileP>(own_p, here, k * kDepth, g));
     Operand<T> es[2], eg[2];
+    float part = 0.f;  // of the own row's or column's sum
     if (blk != block) {
       // Border between the blocks: the end of the rows' block (AS_I) or its start.
       const int first = blk * kTile, last = first + kTile - 1;
@@ -178,42 +184,44 @@ __device__ __forceinline__ void inside(const Tiles<T, NP>& t, int block, v16f (&
           if (AS_I) {
             const float egv = decay[e] * border * gx[el];
             eg[q4 / 2].set(el % 8, egv);
-            sum.row = fmaf(egv, s[el], sum.row);
+            part = fmaf(egv, s[el], part);
           } else {
             const float esv = decay[e] * border * s[el];
             es[q4 / 2].set(el % 8, esv);
             eg[q4 / 2].set(el % 8, decay[e] * border_d * gx[el]);
-            sum.col = fmaf(esv, gx[el], sum.col);
+            part = fmaf(esv, gx[el], part);
           }
         }
       }
     } else {
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
-        const int row = blk * kTile + 8 * q4 + 4 * g;
+        const int at0 = blk * kTile + 8 * q4 + 4 * g;
         const float gap = static_cast<float>(t.base[(blk * kTile + 8 * q4) / kNear] - base_own) - near_own;
-        const v4f nr = *reinterpret_cast<const v4f*>(t.near + row), dr = *reinterpret_cast<const v4f*>(t.step + row);
+        const v4f nr = *reinterpret_cast<const v4f*>(t.near + at0), dr = *reinterpret_cast<const v4f*>(t.step + at0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int at = row + e, el = 4 * q4 + e;
+          const int at = at0 + e, el = 4 * q4 + e;
           const float diff = nr[e] + gap;  // s_row - s_own
           const bool in = AS_I ? at <= own : at >= own;
           // Selected after the exponential, which is as good outside as in, so that no lane branches.
           const float ex = lane::exp2_(AS_I ? -diff : diff), ev = in ? ex : 0.f;
-          const float sv = in ? s[el] : 0.f, gv = in ? gx[el] : 0.f, esv = ev * sv, w = esv * gv;
-          if (!AS_I) es[q4 / 2].set(el % 8, esv);
-          eg[q4 / 2].set(el % 8, ev * gv * (AS_I ? dr[e] : d_own));
+          const float sv = in ? s[el] : 0.f, egv = in ? ev * gx[el] : 0.f, w = egv * sv;
+          if (!AS_I) es[q4 / 2].set(el % 8, ev * sv);
+          eg[q4 / 2].set(el % 8, egv * (AS_I ? dr[e] : d_own));
           if (AS_I) {
-            sum.row = fmaf(at == own ? 0.f : w, dr[e], sum.row);
+            part = fmaf(at == own ? 0.f : w, dr[e], part);
           } else {
             const float dw = at == own ? w : 0.f;
-            sum.col += w - dw;
+            part += w - dw;
             sum.diagonal += dw;
             sum.dot_x += at == own ? gx[el] : 0.f;
           }
         }
       }
     }
+    if (blk * kTile / kHalfTokens == block * kTile / kHalfTokens) sum.near += part;
+    else sum.far += part;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int r0 = blk * kTile + half * kDepth;
@@ -242,7 +250,7 @@ __device__ __forceinline__ void outside(const Tiles<T, NP>& t, int block, int ha
   for (int k = 0; k < NP / kDepth; ++k) {
     const Operand<T> n_own = along<NP>(own_n, own, k * kDepth, g);
 #pragma unroll
-    for (int s = 0; s < kParts<T>; ++s) mma(z, along<NP>(AS_I ? t.hs[s] : t.ghs[s], ln % 32, k * kDepth, g), n_own);
+    for (int s = 0; s < kHeld<T>; ++s) mma(z, along<NP>(AS_I ? t.hs[s] : t.ghs[s], ln % 32, k * kDepth, g), n_own);
   }
   float dot = 0.f;
 #pragma unroll
@@ -254,16 +262,17 @@ __device__ __forceinline__ void outside(const Tiles<T, NP>& t, int block, int ha
       if (!AS_I) gu[r + e] = fmaf(z[r + e], fade, gu[r + e]);
     }
   }
-  if (AS_I) sum.from_h = fmaf(dot, fade, sum.from_h);
-  else sum.from_gh = fmaf(dot, fade, sum.from_gh);
+  sum.outside = fmaf(dot, fade, sum.outside);
+  // Scaled as results, in float32: a token's factor is its column's.
 #pragma unroll
-  for (int k = 0; k < kHalf / kDepth; ++k) {
-    Operand<T> p_own = along<kTileP>(own_p, own, half * kHalf + k * kDepth, g);
+  for (int n = 0; n < NP / kTile; ++n) {
+    v16f from = zeros();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p_own.set(e, p_own.get(e) * into);
+    for (int k = 0; k < kHalf / kDepth; ++k)
+      mma(from, across<false, NP>(AS_I ? t.hs[0] : t.ghs[0], k * kDepth, n * kTile, ln),
+          along<kTileP>(own_p, own, half * kHalf + k * kDepth, g));
 #pragma unroll
-    for (int n = 0; n < NP / kTile; ++n)
-      mma(acc[n], across<false, NP>(AS_I ? t.hs[0] : t.ghs[0], k * kDepth, n * kTile, ln), p_own);
+    for (int r = 0; r < 16; ++r) acc[n][r] = fmaf(from[r], into, acc[n][r]);
   }
 }
 
@@ -335,7 +344,7 @@ __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts
   load(0);
   for (int64_t h = h_first; h < h_last; ++h) {
     const float skip = a.skip == nullptr ? 0.f : a.skip[h];
-    Own sum{0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    Own sum{0.f, 0.f, 0.f, 0.f, 0.f};
     float dot_h = 0.f;
     for (int p0 = 0; p0 < np; p0 += kTileP) {
       __syncthreads();
@@ -353,11 +362,11 @@ __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts
       }
       __syncthreads();
       const bool second = p0 + kHalf < np;
-      if (second) load_half(p0 + kHalf);
       v16f gu[kTileP / kTile];  // rows p, column own (as j)
 #pragma unroll
       for (int m = 0; m < kTileP / kTile; ++m) gu[m] = zeros();
       inside<T, NP, AS_I>(t, block, acc, gu, sum);
+      if (second) load_half(p0 + kHalf);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         if (half == 1) {
@@ -405,29 +414,22 @@ __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts
     // The head's token sums: the two halves of a column hold parts of them.
     const int ln = anew(threadIdx.x % kWave), g = ln / 32, own = block * kTile + ln % 32;
     auto both = [](float v) { return v + __shfl_xor(v, 32, kWave); };
-    if (AS_I) {
-      const float later = both(sum.row + sum.from_h);
-      if (g == 0) to.later[t0 + own] = later;
+    const float near = both(sum.near), far = both(sum.far), outside = both(sum.outside), diagonal = both(sum.diagonal);
+    if (g == 0) {
+      to[AS_I ? kRows : kCols][t0 + own] = near;
+      to[AS_I ? kLater : kEarlier][t0 + own] = outside;
     } else {
-      const float earlier = both(sum.from_gh), direct = both(sum.col), diagonal = both(sum.diagonal);
-      if (g == 0) {
-        to.earlier[t0 + own] = earlier;
-        to.direct[t0 + own] = direct;
-      } else {
-        to.diagonal[t0 + own] = diagonal;
-      }
+      if (!AS_I) to[kDiagonal][t0 + own] = diagonal;
+      // The first half's tokens are the others' columns, the second's their rows.
+      if (AS_I == (own >= kHalfTokens)) to[kFar][t0 + own] = far;
     }
     const float whole = lane::lanes_sum(dot_h), dot_x = lane::lanes_sum(sum.dot_x);
     if (ln == 0) {
-      to.whole[rec * kWaves + wave] = whole;
-      to.skip[rec * kWaves + wave] = dot_x;
+      to.wave[rec * kWaves + wave] = whole;
+      to.wave[to.waves_on + rec * kWaves + wave] = dot_x;
     }
-    to.later += tp;
-    to.earlier += tp;
-    to.direct += tp;
-    to.diagonal += tp;
-    to.whole += waves_step;
-    to.skip += waves_step;
+    to.token += tp;
+    to.wave += waves_step;
     gx += np;
   }
   const int ln = threadIdx.x % kWave, g = ln / 32, own = block * kTile + ln % 32;
@@ -473,45 +475,54 @@ __global__ __launch_bounds__(256) void tokens_kernel(SelectArgs a, int record, i
   const float rate = a.rate[h], bias = a.dt_bias == nullptr ? 0.f : a.dt_bias[h];
   const Steps s(a, b, h);
   const TokenSums from(a, b, h, records, waves);
-  const int per = record / kWave;  // tokens a lane, 1 or 2
-  float f[2], e[2], direct[2], diagonal[2], d[2], slope[2];
-  float f_sum = 0.f, e_sum = 0.f;
+  const int per = record / kWave;         // tokens a lane, 1 or 2
+  const int half = kHalfTokens / per;     // lanes of a half
+  const bool first = ln < half;
+  float inside[2], later[2], earlier[2], far[2], direct[2], d[2], slope[2];
+  float inside_sum = 0.f, later_sum = 0.f, earlier_sum = 0.f, far_sum = 0.f;
   for (int k = 0; k < per; ++k) {
     const int64_t t = t0 + per * ln + k;
+    const float col = from[kCols][t], c = from[kEarlier][t], other = from[kFar][t];
     d[k] = s.step[t];
-    direct[k] = from.direct[t];
-    diagonal[k] = from.diagonal[t];
-    const float c = from.earlier[t];
-    f[k] = from.later[t] - d[k] * direct[k];
-    e[k] = d[k] * c;
-    direct[k] += diagonal[k] + c;
+    inside[k] = from[kRows][t] - d[k] * col;
+    later[k] = from[kLater][t];
+    earlier[k] = d[k] * c;
+    far[k] = first ? d[k] * other : other;
+    direct[k] = col + (first ? other : 0.f) + from[kDiagonal][t] + c;
     slope[k] = 1.f;
     if (per * ln + k < live && a.softplus)
       slope[k] = lane::softplus_slope_(lane::param(a.dt, b * a.dt_batch + t * a.dt_row + h, a.dt_bf16) + bias);
-    f_sum += f[k];
-    e_sum += e[k];
+    inside_sum += inside[k];
+    later_sum += later[k];
+    earlier_sum += earlier[k];
+    far_sum += far[k];
   }
   float whole = 0.f, skip = 0.f;
   if (ln < waves) {
-    whole = from.whole[rec * waves + ln];
-    skip = from.skip[rec * waves + ln];
+    whole = from.wave[rec * waves + ln];
+    skip = from.wave[from.waves_on + rec * waves + ln];
   }
   const int64_t last = (t0 + record - 1) / kNear;
   whole = lane::lanes_sum(whole) *
           lane::exp2_(static_cast<float>(s.base[last] - s.base[t0 / kNear] + s.near[t0 + record - 1]));
   skip = lane::lanes_sum(skip);
-  const float f_up = lanes_prefix(f_sum);
-  float later = __shfl(f_up, kWave - 1, kWave) - f_up + f_sum, earlier = lanes_prefix(e_sum) - e_sum;
+  // Sums over the tokens before a lane's first, and from it on.
+  auto before = [&](float x, int width) { return lanes_prefix(x, width) - x; };
+  auto from_here = [&](float x, int width) {
+    const float up = lanes_prefix(x, width);
+    return __shfl(up, ln / width * width + width - 1, kWave) - up + x;
+  };
+  const float ends = from_here(far_sum, half), starts = before(far_sum, half);
+  float ga = from_here(inside_sum, half) + from_here(later_sum, kWave) + before(earlier_sum, kWave) +
+             (first ? starts : ends) + whole;
   float g_rate = 0.f, g_bias = 0.f;
   for (int k = 0; k < per; ++k) {
     const int64_t t = t0 + per * ln + k;
-    const float ga = later + earlier + whole;
-    later -= f[k];
-    earlier += e[k];
     const float gd = per * ln + k < live ? fmaf(rate, ga, direct[k]) * slope[k] : 0.f;
     g_rate = fmaf(d[k], ga, g_rate);
     g_bias += gd;
     if (t < a.t) lane::put_param(a.gdt, (b * a.t + t) * a.h + h, gd, a.dt_bf16);
+    ga += earlier[k] - later[k] - inside[k] + (first ? far[k] : -far[k]);
   }
   g_rate = lane::lanes_sum(g_rate);
   g_bias = lane::lanes_sum(g_bias);
@@ -574,10 +585,10 @@ int64_t select_parts(const SelectArgs& a) {
   return want < most ? want : most;
 }
 
-// Four sums a token, two of a record's waves (at most 8 of them).
+// Six sums a token, two of a record's waves (at most 8 of them).
 int64_t select_token_floats(const SelectArgs& a) {
   const int64_t tp = (a.t + select_scan::kSpan - 1) / select_scan::kSpan * select_scan::kSpan, record = select_record(a.bf16);
-  return a.b * a.h * (4 * tp + 2 * 8 * ((a.t + record - 1) / record));
+  return a.b * a.h * (6 * tp + 2 * 8 * ((a.t + record - 1) / record));
 }
 
 hipError_t launch_select_backward(const SelectArgs& a, hipStream_t stream) {
