@@ -43,6 +43,13 @@ __device__ __forceinline__ int anew(int x) {
   asm volatile("" : "+v"(x));
   return x;
 }
+// x, computed here: what follows in the source is not moved before it.  A value
+// that is formed of registers behind the loads that refill them would keep
+// those, and the copies would wait for the loads.
+__device__ __forceinline__ float now(float x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 template <typename T>
 struct Operand;

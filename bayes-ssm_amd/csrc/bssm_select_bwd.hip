@@ -320,8 +320,8 @@ __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts
   const int64_t waves_step = records * kWaves;
   Rows<T, L, kTileP, kThreads> rx, rg;
   HalfRecord<T, NP> rh, rgh;
-  float r_step = 0.f, r_near = 0.f, r_near_end = 0.f;  // of token threadIdx.x
-  double r_base = 0., r_start = 0., r_end = 0.;
+  float r_step = 0.f, r_near = 0.f;  // of token threadIdx.x
+  double r_base = 0.;
   auto load_half = [&](int p_first) {
     rh.template load<FAST>(h_rec, p_first, np, nn);
     rgh.template load<FAST>(gh_rec, p_first, np, nn);
@@ -332,13 +332,9 @@ __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts
     load_half(p0);
     const int at = anew(threadIdx.x);
     if (at < L) {
-      const int first = at / kTile * kTile;
       r_step = steps.step[t0 + at];
       r_near = steps.near[t0 + at];
-      r_near_end = steps.near[t0 + first + kTile - 1];
       r_base = steps.base[(t0 + at) / kNear];
-      r_start = steps.base[(t0 + first) / kNear];
-      r_end = steps.base[(t0 + first) / kNear + kTile / kNear - 1];
     }
   };
   load(0);
@@ -356,6 +352,9 @@ __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts
       if (const int at = anew(threadIdx.x); at < L) {
         t.step[at] = r_step;
         t.near[at] = r_near;
+        const int last = at % kWave | (kTile - 1);
+        const double r_start = __shfl(r_base, last - (kTile - 1), kWave), r_end = __shfl(r_base, last, kWave);
+        const float r_near_end = __shfl(r_near, last, kWave);
         t.since[at] = lane::exp2_(static_cast<float>(r_base - r_start + r_near));
         t.until[at] = r_step * lane::exp2_(static_cast<float>(r_end + r_near_end - r_base - r_near));
         if (at % kNear == 0) t.base[at / kNear] = r_base;

@@ -36,8 +36,7 @@ namespace select_scan {
 namespace {
 
 constexpr int kChunk = kSelectChunk;
-constexpr int kThreads = 512;       // of the full pass
-constexpr int kCarryThreads = 256;  // of the state's passes
+constexpr int kThreads = 512;  // of the full pass
 constexpr int kRecordsB16 = 128, kRecordsF32 = 64;  // tokens between two kept states
 
 // Steps and running sums of every token: a wave takes kSpan tokens of a head, two a lane.
@@ -72,24 +71,24 @@ __global__ __launch_bounds__(256) void steps_kernel(SelectArgs a) {
       v2f{n0, static_cast<float>(before - start + log2_fade[0] + log2_fade[1])};
 }
 
-// The part of the state that one of four waves carries, transposed: tile m holds, of the
-// wave's 32 values of P (column l % 32), the states 32 (wave % 2 + 2 m) on.
-template <int NP>
+// The part of the state that one of 2 WAYS waves carries, transposed: tile m holds, of the
+// wave's 32 values of P (column l % 32), the states 32 (wave % WAYS + WAYS m) on.
+template <int NP, int WAYS>
 struct State {
-  static constexpr int kTiles = NP <= kTile ? 1 : NP / kTile / 2;
+  static constexpr int kTiles = NP <= WAYS * kTile ? 1 : NP / kTile / WAYS;
   v16f v[kTiles];
   int n_first, p, g;
-  bool any;  // with 32 states the odd waves carry none
+  bool any;  // with too few states the last waves carry none
   __device__ __forceinline__ explicit State(int wave) {
     const int ln = threadIdx.x % kWave;
-    n_first = wave % 2 * kTile;
-    p = wave / 2 * kTile + ln % 32;
+    n_first = wave % WAYS * kTile;
+    p = wave / WAYS * kTile + ln % 32;
     g = ln / 32;
     any = n_first < NP;
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) v[m] = zeros();
   }
-  static constexpr int kStride = 2 * kTile;  // between a wave's tiles
+  static constexpr int kStride = WAYS * kTile;  // between a wave's tiles
   // fn(tile, first element, state of that): 4 consecutive states each.
   template <typename Fn>
   __device__ __forceinline__ void each(Fn fn) {
@@ -142,7 +141,7 @@ struct State {
   template <typename T>
   __device__ __forceinline__ void advance(const T (*wu)[kChunk * kTileP], const T* ks, float fade, int wave) {
     if (!any) return;
-    const int ln = anew(threadIdx.x % kWave), p_first = wave / 2 * kTile;
+    const int ln = anew(threadIdx.x % kWave), p_first = wave / WAYS * kTile;
     scale(fade);
 #pragma unroll
     for (int k0 = 0; k0 < kChunk; k0 += kDepth) {
@@ -241,11 +240,18 @@ __device__ __forceinline__ float* segment_fade(const SelectArgs& a, int64_t segs
   return a.segments + segs * a.b * a.h * a.p * a.n + (seg * a.b + b) * a.h + h;
 }
 
+// A chunk's tiles in LDS.
+template <typename T, int NP>
+struct Chunk {
+  alignas(16) T xs[kChunk * kTileP], wx[kParts<T>][kChunk * kTileP], ks[kChunk * NP], qs[kChunk * NP];
+  alignas(16) ChunkSteps steps;
+};
+
 template <typename T, int NP, bool FAST>
 __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t segs) {
-  __shared__ __align__(16) T xs[kChunk * kTileP], wx[kParts<T>][kChunk * kTileP], ks[kChunk * NP], qs[kChunk * NP],
-      hs[kTileP * NP];
-  __shared__ __align__(16) ChunkSteps cs;
+  constexpr int kBuffers = sizeof(T) == 2 && NP > 64 ? 2 : 1;
+  __shared__ Chunk<T, NP> tiles[kBuffers];
+  __shared__ __align__(16) T hs[kTileP * NP];
   const Block at(a, segs);
   const int wave = wave_index() % 4, ib = wave % 2, pb = wave / 2;
   const bool carries = wave_index() >= 4;
@@ -259,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t
   const int64_t record = sizeof(T) == 2 ? kRecordsB16 : kRecordsF32, ratio = record / kChunk,
                 records = (a.t + record - 1) / record;
   const Steps steps(a, at.b, at.h);
-  State<NP> st(wave);
+  State<NP, 2> st(wave);
   if (carries) {
     st.template add<FAST>(a.state0 == nullptr ? nullptr : a.state0 + bh * pn, at.p0, at.np, at.n);
     for (int64_t s = 0; s < at.seg; ++s) {
@@ -278,27 +284,43 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t
     rq.template load<FAST>(cq + t0 * a.cq_row, a.cq_row, live, 0, at.n);
     rs.load(steps, t0);
   };
-  if (at.first < at.last) load(at.first);
-  for (int64_t c = at.first; c < at.last; ++c) {
-    const int64_t t0 = c * kChunk, live = n_live - t0;
-    __syncthreads();
-    if (carries) st.to_lds(hs);
+  float fade = 0.f, next_fade = 0.f;  // of the chunk computed, and of the chunk in the tiles last
+  // Chunk c from registers into its tiles; the one after it is asked for.
+  auto stage = [&](int64_t c) {
+    Chunk<T, NP>& to = tiles[(c - at.first) % kBuffers];
     float weight[RowsX::kPieces];
     rs.template weights<false>(weight);
-    rx.store(xs);
-    rx.store_weighted(wx, weight);
-    rk.store(ks);
-    rq.store(qs);
-    rs.store(cs);
-    const float fade = rs.fade();
+    rx.store(to.xs);
+    rx.store_weighted(to.wx, weight);
+    rk.store(to.ks);
+    rq.store(to.qs);
+    rs.store(to.steps);
+    next_fade = now(rs.fade());
+    load(c + 1 < at.last ? c + 1 : c);  // without a branch, which would cost the wait for what it loads
+  };
+  if (at.first < at.last) {
+    load(at.first);
+    stage(at.first);
+  }
+  for (int64_t c = at.first; c < at.last; ++c) {
+    const int64_t t0 = c * kChunk, live = n_live - t0;
+    if (kBuffers == 1 && c > at.first) stage(c);
+    if (carries) st.to_lds(hs);
+    fade = next_fade;
     __syncthreads();
-    if (carries && a.states != nullptr && c % ratio == 0)
-      st.template store<FAST>(a.states + (bh * records + c / ratio) * pn, at.p0, at.np, at.n);
-    if (c + 1 < at.last) load(c + 1);
+    const Chunk<T, NP>& in = tiles[(c - at.first) % kBuffers];
+    const T *xs = in.xs, *ks = in.ks, *qs = in.qs;
+    const ChunkSteps& cs = in.steps;
     if (carries) {
-      st.advance(wx, ks, lane::exp2_(fade), wave);
+      if (a.states != nullptr && c % ratio == 0)
+        st.template store<FAST>(a.states + (bh * records + c / ratio) * pn, at.p0, at.np, at.n);
+      st.advance(in.wx, ks, lane::exp2_(fade), wave);
+      // The next chunk's tiles: these waves after their products, the others before.
+      if (kBuffers == 2 && c + 1 < at.last) stage(c + 1);
+      __syncthreads();
       continue;
     }
+    if (kBuffers == 2 && c + 1 < at.last) stage(c + 1);
     const int ln = anew(threadIdx.x % kWave), g = ln / 32, own = ib * kTile + ln % 32;
     // Outputs, transposed: rows p, column own.
     Operand<T> q[NP / kDepth];
@@ -365,6 +387,7 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t
       }
       put4<FAST>(w, out, own, y_row, c0 + 4 * g, cols, own < y_rows, o);
     }
+    __syncthreads();
   }
   if (carries && at.seg == segs - 1 && a.state_out != nullptr)
     st.template store<FAST>(a.state_out + bh * pn, at.p0, at.np, at.n);
@@ -375,9 +398,14 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t
 //   gh0 = exp(s_64) gh0' + sum_i exp(s_i) C_i gy_i^T;
 // LOCAL: from zero, into the workspace; else from the later segments', keeping
 // the adjoint behind every record's last token and the one before the first.
+template <int NP>
+constexpr int kCarryWays = NP / kTile;  // waves that share N
+template <int NP>
+constexpr int kCarryThreads = NP > 64 ? 512 : 256;
+
 template <typename T, int NP, bool FAST, bool BACK, bool LOCAL>
-__global__ __launch_bounds__(kCarryThreads, sizeof(T) == 2 ? 2 : 1) void carry_kernel(SelectArgs a, int64_t segs) {
-  __shared__ __align__(16) T wu[kParts<T>][kChunk * kTileP], ks[kChunk * NP];
+__global__ __launch_bounds__(kCarryThreads<NP>, 2) void carry_kernel(SelectArgs a, int64_t segs) {
+  __shared__ __align__(16) T wu[2][kParts<T>][kChunk * kTileP], ks[2][kChunk * NP];
   const Block at(a, segs);
   const int wave = wave_index();
   const int64_t grp = at.h / (a.h / a.g), n_live = row_length(a, at.b), bh = at.b * a.h + at.h;
@@ -391,7 +419,8 @@ __global__ __launch_bounds__(kCarryThreads, sizeof(T) == 2 ? 2 : 1) void carry_k
   const int64_t record = sizeof(T) == 2 ? kRecordsB16 : kRecordsF32, ratio = record / kChunk,
                 records = (a.t + record - 1) / record, chunks = (a.t + kChunk - 1) / kChunk;
   const Steps steps(a, at.b, at.h);
-  State<NP> st(wave);
+  State<NP, kCarryWays<NP>> st(wave);
+  st.any = st.any && wave < 2 * kCarryWays<NP>;
   float total = 0.f;
   if constexpr (!LOCAL) {
     st.template add<FAST>(a.gstate_out == nullptr ? nullptr : a.gstate_out + bh * pn, at.p0, at.np, at.n);
@@ -400,33 +429,50 @@ __global__ __launch_bounds__(kCarryThreads, sizeof(T) == 2 ? 2 : 1) void carry_k
       st.template add<FAST>(segment_state(a, s, at.b, at.h), at.p0, at.np, at.n);
     }
   }
-  typedef Rows<T, kChunk, kTileP, kCarryThreads> RowsU;
-  RowsU ru;
-  Rows<T, kChunk, NP, kCarryThreads> rk;
-  ChunkLoad<RowsU> rs;
+  typedef Rows<T, kChunk, kTileP, kCarryThreads<NP>> RowsU;
+  struct Ahead {  // a chunk between memory and LDS
+    RowsU u;
+    Rows<T, kChunk, NP, kCarryThreads<NP>> k;
+    ChunkLoad<RowsU> s;
+  } even, odd;
   const int64_t count = at.last - at.first;
   auto chunk = [&](int64_t i) { return BACK ? at.last - 1 - i : at.first + i; };
-  auto load = [&](int64_t c) {
-    const int64_t t0 = c * kChunk, live = n_live - t0;
-    ru.template load<FAST>(u + t0 * u_row, u_row, live, at.p0, at.np);
-    rk.template load<FAST>(k + t0 * k_row, k_row, live, 0, at.n);
-    rs.load(steps, t0);
+  auto load = [&](int64_t i, Ahead& to) {  // past the end the last chunk again: a branch here would cost the wait for it
+    const int64_t t0 = chunk(i < count ? i : count - 1) * kChunk, live = n_live - t0;
+    to.u.template load<FAST>(u + t0 * u_row, u_row, live, at.p0, at.np);
+    to.k.template load<FAST>(k + t0 * k_row, k_row, live, 0, at.n);
+    to.s.load(steps, t0);
   };
-  if (count > 0) load(chunk(0));
-  for (int64_t i = 0; i < count; ++i) {
-    const int64_t c = chunk(i);
-    __syncthreads();
+  float fade = 0.f, next_fade = 0.f;
+  // The i'th chunk from registers into its tiles; the next but one is asked for.
+  auto stage = [&](int64_t i, Ahead& from, int buffer) {
     float weight[RowsU::kPieces];
-    rs.template weights<BACK>(weight);
-    ru.store_weighted(wu, weight);
-    rk.store(ks);
-    const float fade = rs.fade();
-    __syncthreads();
+    from.s.template weights<BACK>(weight);
+    from.u.store_weighted(wu[buffer], weight);
+    from.k.store(ks[buffer]);
+    next_fade = now(from.s.fade());
+    load(i + 2, from);
+  };
+  auto step = [&](int64_t i, Ahead& next, int buffer) {
+    const int64_t c = chunk(i);
+    __syncthreads();  // the i'th tiles are whole, the products from the others' are done
+    fade = next_fade;
+    stage(i + 1, next, 1 - buffer);
     if (!LOCAL && (c % ratio == ratio - 1 || c == chunks - 1))
       st.template store<FAST>(a.adjoints + (bh * records + c / ratio) * pn, at.p0, at.np, at.n);
-    if (i + 1 < count) load(chunk(i + 1));
     total += fade;
-    st.advance(wu, ks, lane::exp2_(fade), wave);
+    st.advance(wu[buffer], ks[buffer], lane::exp2_(fade), wave);
+  };
+  if (count > 0) {
+    load(0, even);
+    load(1, odd);
+    stage(0, even, 0);
+    for (int64_t i = 0;; i += 2) {
+      step(i, odd, 0);
+      if (i + 1 == count) break;
+      step(i + 1, even, 1);
+      if (i + 2 == count) break;
+    }
   }
   if constexpr (LOCAL) {
     st.template store<FAST>(segment_state(a, at.seg, at.b, at.h), at.p0, at.np, at.n);
@@ -443,7 +489,7 @@ unsigned blocks(const SelectArgs& a, int64_t segs) {
 template <typename T, int NP, bool FAST>
 hipError_t launch(const SelectArgs& a, bool back, hipStream_t stream) {
   const int64_t segs = select_segments(a);
-  const dim3 grid(blocks(a, segs)), block(kCarryThreads);
+  const dim3 grid(blocks(a, segs)), block(kCarryThreads<NP>);
   if (back) {
     if (segs > 1) hipLaunchKernelGGL((carry_kernel<T, NP, FAST, true, true>), grid, block, 0, stream, a, segs);
     hipLaunchKernelGGL((carry_kernel<T, NP, FAST, true, false>), grid, block, 0, stream, a, segs);
@@ -503,12 +549,14 @@ int64_t select_step_floats(const SelectArgs& a) {
 }
 
 // One segment where the sequences, heads and P tiles alone give every compute
-// unit a workgroup; else two a unit, each of 8 chunks or more: a segment costs
-// the pass that gives its state from zero.
+// unit a workgroup; else two a unit, each of 4 chunks or more.  A chunk takes a
+// workgroup 5 us, and half as much again in the pass that gives a segment's
+// state from zero: 2 x 777 tokens of 6 heads in float32, on 12 workgroups, took
+// 66 us in one segment.
 int64_t select_segments(const SelectArgs& a) {
   const int64_t have = a.b * a.h * ((a.p + select_scan::kTileP - 1) / select_scan::kTileP);
   if (have >= 256 || have == 0) return 1;
-  const int64_t chunks = (a.t + kSelectChunk - 1) / kSelectChunk, want = (512 + have - 1) / have, most = chunks / 8;
+  const int64_t chunks = (a.t + kSelectChunk - 1) / kSelectChunk, want = (512 + have - 1) / have, most = chunks / 4;
   return want < most ? want : most > 1 ? most : 1;
 }
 int64_t select_segment_floats(const SelectArgs& a) {
