@@ -70,6 +70,17 @@ def _inner(x: Tensor) -> Tensor:
     return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
 
 
+def _room(device: torch.device, *sizes: int) -> tuple[Tensor, list[Optional[int]]]:
+    """One float32 allocation and the address of each of its parts (None for 0 floats), on 16-byte boundaries."""
+    starts, end = [], 0
+    for n in sizes:
+        starts.append(end)
+        end += (n + 3) & ~3
+    room = torch.empty(end, device=device, dtype=torch.float32)
+    base = room.data_ptr()
+    return room, [base + 4 * at if n else None for at, n in zip(starts, sizes)]
+
+
 class _ScanFunction(torch.autograd.Function):
     """Autograd boundary of the scan (C ABI ``bssm_select_forward/backward``)."""
 
@@ -92,22 +103,21 @@ class _ScanFunction(torch.autograd.Function):
         keep = any(ctx.needs_input_grad)
         y = torch.empty(b, t, h, p, device=dev, dtype=x.dtype)
         last = torch.empty(b, h, p, n, device=dev, dtype=torch.float32)
-        states = torch.empty(b, h, size(0), p, n, device=dev, dtype=torch.float32) if keep else None
-        work = size(1)
-        segments = torch.empty(work, device=dev, dtype=torch.float32) if work else None
-        steps = torch.empty(size(3), device=dev, dtype=torch.float32)
+        steps_at = b * h * size(0) * p * n if keep else 0  # the kept states, and the tokens' steps behind them
+        kept, (states, steps) = _room(dev, steps_at, size(3))
+        _segments, (segments,) = _room(dev, size(1))
         P = _hip.ptr
         _hip.launch(dev, "bssm_select_forward", *_ScanFunction._head(x, dt, A, B, C, D, dt_bias, softplus, lengths),
-                    P(state), P(y), P(last), P(states), P(steps), P(segments), b, t, h, p, n, g, _hip.stream_of(dev))
+                    P(state), P(y), P(last), states, steps, segments, b, t, h, p, n, g, _hip.stream_of(dev))
         if keep:
-            ctx.save_for_backward(x, dt, A, B, C, D, dt_bias, lengths, states, steps)
+            ctx.save_for_backward(x, dt, A, B, C, D, dt_bias, lengths, kept)
             ctx.softplus = softplus
         ctx.set_materialize_grads(False)
         return y, last
 
     @staticmethod
     def backward(ctx, grad_y, grad_last):
-        x, dt, A, B, C, D, dt_bias, lengths, states, steps = ctx.saved_tensors
+        x, dt, A, B, C, D, dt_bias, lengths, kept = ctx.saved_tensors
         b, t, h, p = x.shape
         g, n = B.shape[2:]
         dev = x.device
@@ -116,16 +126,16 @@ class _ScanFunction(torch.autograd.Function):
         size = lambda what: _hip.function("bssm_select_sizes")(what, bf16, b, t, h, p, n, g)  # noqa: E731
         gy = torch.zeros(b, t, h, p, device=dev, dtype=x.dtype) if grad_y is None else _hip.aligned(grad_y)
         gl = None if grad_last is None else _hip.aligned(grad_last.float())
-        records, work, parts = size(0), size(1), size(2)
+        records, parts = size(0), size(2)
 
         def f32(*shape):
             return torch.empty(*shape, device=dev, dtype=torch.float32)
 
-        adjoints = f32(b, h, records, p, n)
-        segments = f32(work) if work else None
-        token_sums = f32(size(4))
-        partial = f32(parts, 2, b, t, g, n) if parts > 1 else None
-        rows = f32(max(1, b * records), 3, h)
+        of_states = b * h * records * p * n
+        states = kept.data_ptr()
+        steps = states + 4 * ((of_states + 3) & ~3)
+        _work, (adjoints, segments, token_sums, partial, rows) = _room(
+            dev, of_states, size(1), size(4), parts * 2 * b * t * g * n if parts > 1 else 0, max(1, b * records) * 3 * h)
         gx = torch.empty(b, t, h, p, device=dev, dtype=x.dtype)
         gdt = torch.empty(b, t, h, device=dev, dtype=dt.dtype)
         gB, gC = (torch.empty(b, t, g, n, device=dev, dtype=x.dtype) for _ in range(2))
@@ -135,9 +145,9 @@ class _ScanFunction(torch.autograd.Function):
             gstate = torch.zeros_like(gstate) if gl is None else gl.clone()
         P = _hip.ptr
         _hip.launch(dev, "bssm_select_backward",
-                    *_ScanFunction._head(x, dt, A, B, C, D, dt_bias, ctx.softplus, lengths), P(states), P(steps), P(gy),
-                    P(gl), P(adjoints), P(segments), P(token_sums), P(partial), P(rows), P(gx), P(gdt), P(gA), P(gB), P(gC), P(gD), P(gbias),
-                    P(gstate), b, t, h, p, n, g, _hip.stream_of(dev))
+                    *_ScanFunction._head(x, dt, A, B, C, D, dt_bias, ctx.softplus, lengths), states, steps, P(gy),
+                    P(gl), adjoints, segments, token_sums, partial, rows, P(gx), P(gdt), P(gA), P(gB), P(gC), P(gD),
+                    P(gbias), P(gstate), b, t, h, p, n, g, _hip.stream_of(dev))
         grads = (gx, gdt, gA, gB, gC, gD, gbias, gstate)
         return (*(z if need[i] else None for i, z in enumerate(grads)), None, None)
 

@@ -533,15 +533,21 @@ __global__ __launch_bounds__(256) void tokens_kernel(SelectArgs a, int record, i
   }
 }
 
-// Gradients of B and C: their sums over the parts of a group's heads.
-template <typename T>
+// Gradients of B and C: their sums over the parts of a group's heads, W values a thread.
+template <typename T, int W>
 __global__ __launch_bounds__(256) void parts_kernel(SelectArgs a, int64_t parts) {
-  const int64_t all = a.b * a.t * a.g * a.n, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t all = a.b * a.t * a.g * a.n, i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * W;
   if (i >= 2 * all) return;
-  float s = 0.f;
-  for (int64_t k = 0; k < parts; ++k) s += a.gparts[2 * k * all + i];
-  T* out = static_cast<T*>(i < all ? a.gbk : a.gcq);
-  out[i < all ? i : i - all] = lane::narrow<T>(s);
+  float s[W] = {};
+  for (int64_t k = 0; k < parts; ++k) {
+    const Pack<float, W> v = lane::load_pack<float, W>(a.gparts + 2 * k * all + i);
+#pragma unroll
+    for (int e = 0; e < W; ++e) s[e] += v.v[e];
+  }
+  Pack<T, W> o;
+#pragma unroll
+  for (int e = 0; e < W; ++e) o.v[e] = lane::narrow<T>(s[e]);
+  lane::store_pack<T, W>(static_cast<T*>(i < all ? a.gbk : a.gcq) + (i < all ? i : i - all), o);
 }
 
 __global__ __launch_bounds__(lane::kFoldThreads) void heads_kernel(SelectArgs a, int64_t rows) {
@@ -566,7 +572,14 @@ hipError_t launch(const SelectArgs& a, hipStream_t stream) {
                        Z::kL, Z::kThreads / kWave);
     if (parts > 1) {
       const int64_t all = 2 * a.b * a.t * a.g * a.n;
-      hipLaunchKernelGGL(parts_kernel<T>, dim3(static_cast<unsigned>((all + 255) / 256)), dim3(256), 0, stream, a, parts);
+      // 4 values where a token's N are whole fours on such boundaries.
+      const uintptr_t at = reinterpret_cast<uintptr_t>(a.gbk) | reinterpret_cast<uintptr_t>(a.gcq) | reinterpret_cast<uintptr_t>(a.gparts);
+      if (a.n % 4 == 0 && at % 16 == 0)
+        hipLaunchKernelGGL((parts_kernel<T, 4>), dim3(static_cast<unsigned>((all / 4 + 255) / 256)), dim3(256), 0, stream,
+                           a, parts);
+      else
+        hipLaunchKernelGGL((parts_kernel<T, 1>), dim3(static_cast<unsigned>((all + 255) / 256)), dim3(256), 0, stream, a,
+                           parts);
     }
   }
   hipLaunchKernelGGL(heads_kernel, dim3(lane::fold_blocks(3 * a.h)), dim3(lane::kFoldThreads), 0, stream, a, a.b * records);
@@ -576,11 +589,13 @@ hipError_t launch(const SelectArgs& a, hipStream_t stream) {
 }  // namespace
 }  // namespace select_scan
 
-// Two workgroups a compute unit where a group has the heads for it.
+// As many workgroups as the compute units hold at once (one a unit, two with
+// at most 32 states), where a group has the heads for it: more parts write and
+// read more partial gradients.
 int64_t select_parts(const SelectArgs& a) {
   const int64_t record = select_record(a.bf16), have = a.b * a.g * ((a.t + record - 1) / record);
   if (have == 0) return 1;
-  const int64_t want = (512 + have - 1) / have, most = a.h / a.g;
+  const int64_t slots = a.n > 32 ? 256 : 512, want = (slots + have - 1) / have, most = a.h / a.g;
   return want < most ? want : most;
 }
 

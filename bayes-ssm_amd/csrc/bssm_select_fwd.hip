@@ -30,6 +30,7 @@
 #include "bssm_select.h"
 
 #include <initializer_list>
+#include <type_traits>
 
 namespace bssm {
 namespace select_scan {
@@ -120,12 +121,14 @@ struct State {
       }
     });
   }
+  // on = false: into an empty window.  Loads are waited for by the number of
+  // accesses behind them, so that a branch here would cost the wait for all.
   template <bool FAST>
-  __device__ __forceinline__ void store(float* dst, int p0, int np, int n) {
+  __device__ __forceinline__ void store(float* dst, int p0, int np, int n, bool on = true) {
     dst += static_cast<int64_t>(p0) * n;
-    const Window w = window(dst, static_cast<uint32_t>(np - p0 < kTileP ? np - p0 : kTileP) * n * 4u);
+    const Window w = window(dst, on ? static_cast<uint32_t>(np - p0 < kTileP ? np - p0 : kTileP) * n * 4u : 0u);
     each([&](v16f& t, int r, int c) {
-      put4<FAST>(w, dst, p, n, c, n, p0 + p < np, Pack<float, 4>{{t[r], t[r + 1], t[r + 2], t[r + 3]}});
+      put4<FAST>(w, dst, p, n, c, n, on && p0 + p < np, Pack<float, 4>{{t[r], t[r + 1], t[r + 2], t[r + 3]}});
     });
   }
   template <typename T>
@@ -312,8 +315,8 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(SelectArgs a, int64_t
     const T *xs = in.xs, *ks = in.ks, *qs = in.qs;
     const ChunkSteps& cs = in.steps;
     if (carries) {
-      if (a.states != nullptr && c % ratio == 0)
-        st.template store<FAST>(a.states + (bh * records + c / ratio) * pn, at.p0, at.np, at.n);
+      st.template store<FAST>(a.states + (bh * records + c / ratio) * pn, at.p0, at.np, at.n,
+                              a.states != nullptr && c % ratio == 0);
       st.advance(in.wx, ks, lane::exp2_(fade), wave);
       // The next chunk's tiles: these waves after their products, the others before.
       if (kBuffers == 2 && c + 1 < at.last) stage(c + 1);
@@ -404,7 +407,7 @@ template <int NP>
 constexpr int kCarryThreads = NP > 64 ? 512 : 256;
 
 template <typename T, int NP, bool FAST, bool BACK, bool LOCAL>
-__global__ __launch_bounds__(kCarryThreads<NP>, 2) void carry_kernel(SelectArgs a, int64_t segs) {
+__global__ __launch_bounds__(kCarryThreads<NP>, sizeof(T) == 2 && NP > 64 ? 4 : 2) void carry_kernel(SelectArgs a, int64_t segs) {
   __shared__ __align__(16) T wu[2][kParts<T>][kChunk * kTileP], ks[2][kChunk * NP];
   const Block at(a, segs);
   const int wave = wave_index();
@@ -453,26 +456,35 @@ __global__ __launch_bounds__(kCarryThreads<NP>, 2) void carry_kernel(SelectArgs 
     next_fade = now(from.s.fade());
     load(i + 2, from);
   };
-  auto step = [&](int64_t i, Ahead& next, int buffer) {
+  // FIRST waves fill the next tiles before their products and the others after
+  // them: a SIMD has one of either, and so vector and matrix work at once.
+  auto step = [&](auto kind, int64_t i, Ahead& next, int buffer) {
+    constexpr bool FIRST = decltype(kind)::value;
     const int64_t c = chunk(i);
     __syncthreads();  // the i'th tiles are whole, the products from the others' are done
     fade = next_fade;
-    stage(i + 1, next, 1 - buffer);
-    if (!LOCAL && (c % ratio == ratio - 1 || c == chunks - 1))
-      st.template store<FAST>(a.adjoints + (bh * records + c / ratio) * pn, at.p0, at.np, at.n);
+    if (FIRST) stage(i + 1, next, 1 - buffer);
+    if (!LOCAL)
+      st.template store<FAST>(a.adjoints + (bh * records + c / ratio) * pn, at.p0, at.np, at.n,
+                              c % ratio == ratio - 1 || c == chunks - 1);
     total += fade;
     st.advance(wu[buffer], ks[buffer], lane::exp2_(fade), wave);
+    if (!FIRST) stage(i + 1, next, 1 - buffer);
+  };
+  auto walk = [&](auto kind) {
+    for (int64_t i = 0;; i += 2) {
+      step(kind, i, odd, 0);
+      if (i + 1 == count) break;
+      step(kind, i + 1, even, 1);
+      if (i + 2 == count) break;
+    }
   };
   if (count > 0) {
     load(0, even);
     load(1, odd);
     stage(0, even, 0);
-    for (int64_t i = 0;; i += 2) {
-      step(i, odd, 0);
-      if (i + 1 == count) break;
-      step(i + 1, even, 1);
-      if (i + 2 == count) break;
-    }
+    if (wave < kCarryThreads<NP> / kWave / 2) walk(std::true_type{});
+    else walk(std::false_type{});
   }
   if constexpr (LOCAL) {
     st.template store<FAST>(segment_state(a, at.seg, at.b, at.h), at.p0, at.np, at.n);
