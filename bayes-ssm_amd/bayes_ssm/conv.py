@@ -200,8 +200,8 @@ class _ShortConvFunction(torch.autograd.Function):
         rows = _hip.function("bssm_short_conv_partial_rows")(b, t, c)
         partials = torch.empty(rows, w + 1, c, device=dev, dtype=torch.float32)
         P = _hip.ptr
-        _hip.launch(dev, "bssm_short_conv_backward", int(x.dtype == torch.bfloat16), int(weight.dtype == torch.bfloat16), w, int(ctx.silu), P(x),
-                    batch_stride, row_stride, P(weight), P(bias), P(state), P(lengths), P(gy), P(gf), P(gx), P(gs),
+        _hip.launch(dev, "bssm_short_conv_backward", int(x.dtype == torch.bfloat16),
+                    int(weight.dtype == torch.bfloat16), w, int(ctx.silu), P(x), batch_stride, row_stride, P(weight), P(bias), P(state), P(lengths), P(gy), P(gf), P(gx), P(gs),
                     P(partials), P(gw), P(gb), b, t, c, _hip.stream_of(dev))
         return gx if need[0] else None, gw if need[1] else None, gb if need[2] else None, gs, None, None
 

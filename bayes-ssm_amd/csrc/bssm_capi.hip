@@ -1449,8 +1449,8 @@ int bssm_select_backward(int bf16, const void* x, int64_t x_batch, int64_t x_row
                          int64_t bk_batch, int64_t bk_row, int64_t bk_group, const void* cq, int64_t cq_batch,
                          int64_t cq_row, int64_t cq_group, const float* skip, const float* dt_bias, int softplus,
                          const int64_t* lengths, const float* states, const float* steps, const void* grad_y,
-                         const float* grad_state_out, float* adjoints, float* segments, float* token_sums, float* parts, float* rows, void* grad_x, void* grad_dt,
-                         float* grad_rate, void* grad_b, void* grad_c, float* grad_skip, float* grad_dt_bias,
+                         const float* grad_state_out, float* adjoints, float* segments, float* token_sums,
+                         float* parts, float* rows, void* grad_x, void* grad_dt, float* grad_rate, void* grad_b, void* grad_c, float* grad_skip, float* grad_dt_bias,
                          float* grad_state0, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t n,
                          int64_t groups, void* stream) {
   const char* fn = "bssm_select_backward";
@@ -1458,12 +1458,14 @@ int bssm_select_backward(int bf16, const void* x, int64_t x_batch, int64_t x_row
                                    bk_row, bk_group, cq, cq_batch, cq_row, cq_group, skip, dt_bias, softplus, lengths,
                                    batch, t, heads, values, n, groups);
   a.states = const_cast<float*>(states); a.gy = grad_y; a.gstate_out = grad_state_out; a.adjoints = adjoints;
-  a.steps = const_cast<float*>(steps); a.token_sums = token_sums; a.segments = segments; a.gparts = parts; a.rows = rows; a.gx = grad_x; a.gdt = grad_dt; a.gbk = grad_b;
+  a.steps = const_cast<float*>(steps); a.token_sums = token_sums; a.segments = segments; a.gparts = parts;
+  a.rows = rows; a.gx = grad_x; a.gdt = grad_dt; a.gbk = grad_b;
   a.gcq = grad_c; a.grate = grad_rate; a.gskip = grad_skip; a.gdt_bias = grad_dt_bias; a.gstate0 = grad_state0;
   if (int rc = select_check(fn, batch, t, heads, values, n, groups)) return rc;
   if (batch > 0 && t > 0) {
     if (int rc = need(fn, {{rate, "rate"}, {x, "x"}, {dt, "dt"}, {bk, "b"}, {cq, "c"}, {states, "states"},
-                           {steps, "steps"}, {token_sums, "token_sums"}, {grad_y, "grad_y"}, {adjoints, "adjoints"}, {rows, "rows"}, {grad_x, "grad_x"},
+                           {steps, "steps"}, {token_sums, "token_sums"}, {grad_y, "grad_y"}, {adjoints, "adjoints"},
+                           {rows, "rows"}, {grad_x, "grad_x"},
                            {grad_dt, "grad_dt"}, {grad_b, "grad_b"}, {grad_c, "grad_c"}}))
       return rc;
     if (bssm::select_segment_floats(a) > 0 && segments == nullptr)

@@ -15,7 +15,14 @@
 // in it) from there.  The backward leaves a row whose upstream gradient is 1,
 // which is what a plain loss.backward() gives, as it is, and forms the others
 // from the logits again (multiplied, the gradient would be rounded twice).
-// Longer rows are read a second time by the forward.
+// Longer rows are read a second time by the forward.  Without a gradient rows
+// of more than 2048 pieces are read piece by piece with a running maximum: no
+// registers held, so that two workgroups of 16 waves share a compute unit.
+//
+// Measured: training step of 4096 x 32000 bfloat16 with 64 entries, forward
+// 109 us (4.8 TB/s; 125 before its stores were non-temporal), 124 us with the
+// counts, the mean and the backward; losses of 301 x 50257 float32 14.6 us
+// (4.1 TB/s; 20 us with the row held).
 //
 // Rows lie where they lie: pieces start at the row's first 4-byte boundary at
 // or before its start (an odd bfloat16 row shares its first 4 bytes with the
@@ -34,7 +41,7 @@ using lane::kWave;
 typedef __amdgpu_buffer_rsrc_t Window;
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
-constexpr int kStream = 2;  // non-temporal
+constexpr int kStream = 2;  // non-temporal: the gradient of a large vocabulary is larger than the caches
 constexpr int kCountBlocks = 512;  // partial counts of rows with a teacher
 
 template <int THREADS>

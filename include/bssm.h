@@ -761,8 +761,8 @@ int bssm_select_forward(int bf16, const void* x, int64_t x_batch, int64_t x_row,
  * as the forward left them.  grad_y [batch, t, heads, values] contiguous;
  * grad_state_out may be NULL (zero).  Workspaces (float32): adjoints of the
  * size of states; segments as in the forward; token_sums of
- * bssm_select_sizes(4, ...) floats; parts [bssm_select_sizes(2, ...), 2, batch, t, groups, n] (may be
- * NULL where that is 1); rows [batch * bssm_select_sizes(0, ...), 3, heads].
+ * bssm_select_sizes(4, ...) floats; parts [bssm_select_sizes(2, ...), 2,
+ * batch, t, groups, n] (may be NULL where that is 1); rows [batch * bssm_select_sizes(0, ...), 3, heads].
  * grad_rate, grad_skip, grad_dt_bias [heads] and grad_state0 may be NULL. */
 int bssm_select_backward(int bf16, const void* x, int64_t x_batch, int64_t x_row, int64_t x_head, int dt_bf16,
                          const void* dt, int64_t dt_batch, int64_t dt_row, const float* rate, const void* b,
@@ -770,7 +770,8 @@ int bssm_select_backward(int bf16, const void* x, int64_t x_batch, int64_t x_row
                          int64_t c_row, int64_t c_group, const float* skip, const float* dt_bias, int softplus,
                          const int64_t* lengths, const float* states, const float* steps, const void* grad_y,
                          const float* grad_state_out, float* adjoints, float* segments, float* token_sums,
-                         float* parts, float* rows, void* grad_x, void* grad_dt, float* grad_rate, void* grad_b, void* grad_c, float* grad_skip, float* grad_dt_bias,
+                         float* parts, float* rows, void* grad_x, void* grad_dt, float* grad_rate, void* grad_b,
+                        void* grad_c, float* grad_skip, float* grad_dt_bias,
                          float* grad_state0, int64_t batch, int64_t t, int64_t heads, int64_t values, int64_t n,
                          int64_t groups, void* stream);
 

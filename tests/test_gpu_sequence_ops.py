@@ -552,3 +552,20 @@ def test_refusals_on_the_gpu(cuda_device):
         distillation_loss(many, many, many.long())
     with pytest.raises(ValueError, match="device"):
         selective_scan(z[..., :8], z[..., 0], torch.zeros(1), z, z)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("p,n,groups", [(64, 128, 1), (40, 24, 2)])
+def test_scan_single_token_without_state(cuda_device, dtype, p, n, groups):
+    """One token from a zero state has no decay in its output: A's gradient is 0, not the rounding of what cancels."""
+    from bayes_ssm.selective import selective_scan
+
+    torch.manual_seed(3)
+    b, h = 5, 2 * groups
+    x, B, C = (torch.randn(b, 1, *s, device=cuda_device).to(dtype).requires_grad_(True)
+               for s in ((h, p), (groups, n), (groups, n)))
+    dt = torch.randn(b, 1, h, device=cuda_device).to(dtype)
+    A = (-torch.rand(h, device=cuda_device) - 0.1).requires_grad_(True)
+    y, _ = selective_scan(x, dt, A, B, C)
+    (gA,) = torch.autograd.grad(y, (A,), torch.randn_like(y))
+    assert torch.equal(gA, torch.zeros_like(gA))
