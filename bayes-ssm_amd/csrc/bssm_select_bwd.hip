@@ -35,8 +35,8 @@
 // the way allows: the registers that it occupies are what spills.  The token
 // sums row, col, ... go to memory, where tokens_kernel closes them.
 //
-// Measured at 8 x 2048 tokens, 32 heads of 64 x 128, bfloat16: 272 us (the
-// adjoint before it 87, tokens_kernel 16, parts_kernel 8), of which the traffic
+// Measured at 8 x 2048 tokens, 32 heads of 64 x 128, bfloat16: 272 to 280 us (the
+// adjoint before it 87, tokens_kernel 15, parts_kernel 8), of which the traffic
 // of 0.5 GB would take 95 and the products 60.  A SIMD has two waves and
 // issues vector instructions in under half of its cycles; the rest waits on LDS
 // reads and on the four barriers of a head.  With 121 spilled registers it was
